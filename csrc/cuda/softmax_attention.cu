@@ -1,0 +1,531 @@
+// Softmax attention over the paged KV cache for few query rows per sequence (single tokens, beams), forward (sm_100a).
+//
+//   o = sum_j w_j v_j / sum_j w_j,   w_j = exp(scale q.k_j - max),   lse = max + log sum_j w_j
+//
+// over the keys that the row sees: up to its own position, of those the last `window` and the first `sinks`.  One pass
+// over K and V with a running maximum and sum; both are kept in fp32, as is o.  w is rounded to the inputs' type for the
+// product with V (the sum takes it unrounded): a rounding of at most half a step per weight, which averages out over the
+// keys to about the rounding of the result itself.
+//
+// Bound: the bytes of K and V.  The G query heads that share a key head are the rows of one 16-row mma.sync tile (a
+// 128-row tcgen05 tile would be mostly padding here and the matrix rate does not matter), so K and V are read once for all
+// of them.  The keys of all (sequence, row tile, key head) items are laid end to end in units of NW tiles of 32 keys and every
+// CTA takes an equal, contiguous share, found from the offsets on the device: uneven histories cost nothing, no length is
+// needed on the host and a captured graph stays right for other lengths.  An item cut by a share's border leaves partial
+// results (normalised o and its lse) that a second kernel joins.
+//
+// Inside a CTA every warp streams its own tiles through its own TMA ring (128-byte swizzle, read with ldmatrix), with no
+// CTA-wide synchronisation until the warps' results are joined at the end of an item.
+#include "softmax_attention.cuh"
+
+namespace {
+
+using namespace rb_attn;
+
+constexpr int KT = 32;      // keys per tile
+constexpr int RT = 16;      // rows per tile
+constexpr int NW = 4;       // warps per CTA
+
+template <int D> struct Cfg {
+  static constexpr int CH = D / 64;
+  static constexpr int TILE = KT * D * 2;                       // bytes of a K or a V tile
+  static constexpr int STAGES = D == 64 ? 4 : 3;
+  static constexpr int RING = NW * STAGES * 2 * TILE;
+  static constexpr int SMEM = RING + 1024 + 2048;
+};
+
+struct Meta { int valid, seq, qt, h, c0, c1, n, pad; long long t0, total; };
+
+struct Outs {
+  void* out; long long ld_o; float* lse;   // final results: 16-bit rows [Tq][ld_o], lse [Tq][H] or null
+  float* part_o; float* part_lse;          // when not null: fp32 [2][Tq][H][D] and log2 [2][Tq][H] instead, by Seq::part
+  float* cut_o; float* cut_lse;            // [CTAs][2][RT][D], [CTAs][2][RT]: items cut by a share's border
+  Meta* meta;                              // [CTAs]
+};
+
+struct Items { int qt, units; };           // row tiles of a sequence, units of keys of each
+
+template <int D>
+__device__ __forceinline__ Items items_of(const Batch& p, const Seq& s) {
+  Items r;
+  r.qt = (s.len_q * p.G + RT - 1) / RT;
+  int tiles;
+  if (r.qt <= 1) {
+    tiles = span_of<KT>(p, s, 0, max(s.len_q - 1, 0)).tiles;
+  } else {                                  // as many for every row tile: the most that one can need
+    tiles = (s.len_k + KT - 1) / KT;
+    if (s.causal && p.window > 0)
+      tiles = static_cast<int>(min(static_cast<long long>(tiles),
+                                   (p.sinks + KT - 1LL) / KT + (static_cast<long long>(p.window) + (RT - 1) / p.G + 2 + 2 * KT) / KT));
+  }
+  r.units = max((tiles + NW - 1) / NW, 1);
+  return r;
+}
+
+__device__ __forceinline__ long long share(int c, int n, long long total) { return total * c / n; }
+
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
+}
+
+// one finished row (or a third of it): o normalised, lse in log2
+template <int D, bool BF16, int N>
+__device__ __forceinline__ void write_row(const Batch& p, const Outs& w, const Seq& s, int row, int h, int col, const float (&o)[N],
+                                          float lse2) {
+  const long long t = s.q_begin + row / p.G;
+  const int head = h * p.G + row % p.G;
+  if (w.part_o) {
+    const long long at = (static_cast<long long>(s.part) * p.Tq + t) * p.H + head;
+    float* dst = w.part_o + at * D + col;
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+    if (col == 0) w.part_lse[at] = lse2;
+  } else {
+    uint16_t* dst = reinterpret_cast<uint16_t*>(w.out) + t * w.ld_o + static_cast<long long>(head) * D + col;
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      *reinterpret_cast<uint2*>(dst + i) = make_uint2(pack16<BF16>(o[i], o[i + 1]), pack16<BF16>(o[i + 2], o[i + 3]));
+    if (col == 0 && w.lse) w.lse[t * p.H + head] = lse2 * LN2;
+  }
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(NW * 32) attn_rows_kernel(const __grid_constant__ CUtensorMap tm, const Batch p, const Outs w) {
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* tail = smem + C::RING;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tail);                          // [NW][STAGES]
+  float* ml = reinterpret_cast<float*>(tail + 256);                            // [NW][RT][2]
+  long long* sums = reinterpret_cast<long long*>(tail + 1024);                 // [NW], then base of the first item
+  int* found = reinterpret_cast<int*>(tail + 1024 + 64);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 1024 + 96);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nb = p.a.B + p.b.B;
+  if (tid == 0) {
+    for (int i = 0; i < NW * C::STAGES; ++i) rb::mbar_init(&bars[i], 1);
+    *abort_flag = 0;
+    rb::mbar_fence_init();
+  }
+  // ---- this CTA's share of the keys
+  const int per = (nb + NW * 32 - 1) / (NW * 32);
+  long long mine = 0;
+  for (int i = tid * per; i < min((tid + 1) * per, nb); ++i) {
+    const Seq s = seq_of(p, i);
+    const Items it = items_of<D>(p, s);
+    mine += static_cast<long long>(it.qt) * it.units * p.Hkv;
+  }
+  long long incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+  long long before = incl - mine, total = 0;
+  for (int i = 0; i < NW; ++i) {
+    if (i < warp) before += sums[i];
+    total += sums[i];
+  }
+  const int n_sh = static_cast<int>(min(static_cast<long long>(gridDim.x), total));   // no share is empty
+  const int cta = blockIdx.x;
+  const long long p0 = cta < n_sh ? share(cta, n_sh, total) : 0, p1 = cta < n_sh ? share(cta + 1, n_sh, total) : 0;
+  if (p0 < p1 && before <= p0 && p0 < before + mine) {
+    long long base = before;
+    for (int i = tid * per;; ++i) {
+      const Seq s = seq_of(p, i);
+      const Items it = items_of<D>(p, s);
+      const long long n = static_cast<long long>(it.qt) * it.units * p.Hkv;
+      if (p0 < base + n) { *found = i; sums[NW] = base; break; }
+      base += n;
+    }
+  }
+  __syncthreads();
+  Meta m;
+  m.valid = 0;
+  if (p0 < p1) {
+    int b = *found;
+    long long base = sums[NW], pos = p0;
+    uint8_t* ring = smem + warp * (C::STAGES * 2 * C::TILE);
+    uint64_t* bar = bars + warp * C::STAGES;
+    int issued = 0, used = 0;                                                  // tiles of this warp so far
+    bool dead = false;
+    while (pos < p1 && b < nb) {
+      const Seq s = seq_of(p, b);
+      const Items it = items_of<D>(p, s);
+      const long long n_b = static_cast<long long>(it.qt) * it.units * p.Hkv;
+      if (pos >= base + n_b) { base += n_b; ++b; continue; }
+      const int off = static_cast<int>((pos - base) % it.units);
+      const int item = static_cast<int>((pos - base) / it.units);
+      const int u1 = static_cast<int>(min(static_cast<long long>(it.units), off + (p1 - pos)));
+      const int qt = item / p.Hkv, h = item % p.Hkv;
+      const int rows = min(s.len_q * p.G - qt * RT, RT);
+      const Span sp = span_of<KT>(p, s, qt * RT / p.G, (qt * RT + rows - 1) / p.G);
+      const long long t0 = pos - off;
+      if (pos == p0 && off > 0 && share(cta - 1, n_sh, total) <= t0) {
+        // the first border inside this item: the second kernel joins its pieces
+        m.valid = 1; m.seq = b; m.qt = qt; m.h = h; m.t0 = t0; m.total = total; m.n = n_sh;
+        m.c0 = cta - 1;
+        m.c1 = static_cast<int>(((t0 + it.units) * n_sh - 1) / total);        // the share that holds the item's last unit
+      }
+      const int v0 = off * NW + warp, v1 = min(u1 * NW, sp.tiles);
+      auto issue = [&](int v) {
+        if (lane == 0) {
+          const int st = issued % C::STAGES;
+          uint8_t* k_dst = ring + st * 2 * C::TILE;
+          uint8_t* v_dst = k_dst + C::TILE;
+          rb::mbar_expect_tx(&bar[st], 2 * C::TILE);
+          const int j0 = sp.tile(v) * KT;
+          for (int x = 0; x < KT; x += p.box_rows) {
+            const int row = box_row(p, s, sp, j0 + x);
+#pragma unroll
+            for (int c = 0; c < C::CH; ++c) {
+              rb::tma_load_2d(k_dst + c * (KT * 128) + x * 128, &tm, &bar[st], h * D + c * 64, row);
+              rb::tma_load_2d(v_dst + c * (KT * 128) + x * 128, &tm, &bar[st], h * D + c * 64, row + p.page_size);
+            }
+          }
+        }
+        ++issued;
+      };
+      int nxt = v0;
+      for (int i = 0; i < C::STAGES && nxt < v1 && !dead; ++i, nxt += NW) issue(nxt);
+      // ---- the 16 query rows as A fragments: this thread's rows are lane / 4 and lane / 4 + 8
+      uint32_t qf[D / 16][4];
+      int rpos[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = (lane >> 2) + 8 * e;
+        const bool live = r < rows;
+        const int row = qt * RT + (live ? r : 0);
+        rpos[e] = row / p.G + s.delta();
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (s.q_begin + row / p.G) * p.ld_q +
+                              static_cast<long long>(h * p.G + row % p.G) * D + (lane & 3) * 2;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          qf[kk][e] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16)) : 0u;
+          qf[kk][e + 2] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16 + 8)) : 0u;
+        }
+      }
+      float o[D / 8][4];
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+      for (int v = v0; v < v1 && !dead; v += NW) {
+        const int st = used % C::STAGES;
+        const bool ok = rb::mbar_wait(&bar[st], (used / C::STAGES) & 1, abort_flag, p.status);
+        if (!__all_sync(0xffffffffu, ok)) { dead = true; break; }
+        ++used;
+        const uint32_t k_addr = rb::smem_u32(ring + st * 2 * C::TILE), v_addr = k_addr + C::TILE;
+        const int j0 = sp.tile(v) * KT;
+        const bool full = (s.causal ? j0 + KT - 1 <= sp.p_min : j0 + KT <= sp.hi) &&
+                          (!s.causal || p.window <= 0 || j0 > sp.p_max - p.window || j0 + KT <= p.sinks);
+        float sc[KT / 8][4];
+#pragma unroll
+        for (int i = 0; i < KT / 8; ++i) sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.f;
+        // S = Q K^T: ldmatrix x4 = 16 keys x 16 columns
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+#pragma unroll
+          for (int n = 0; n < KT / 16; ++n) {
+            const int r = n * 16 + (lane & 7) + ((lane >> 4) << 3);
+            const int unit = (kk & 3) * 2 + ((lane >> 3) & 1);
+            uint32_t b0, b1, b2, b3;
+            ldsm4(k_addr + (kk >> 2) * (KT * 128) + r * 128 + ((unit ^ (r & 7)) << 4), b0, b1, b2, b3);
+            mma16816<BF16>(sc[2 * n], qf[kk], b0, b1);
+            mma16816<BF16>(sc[2 * n + 1], qf[kk], b2, b3);
+          }
+        }
+        float mn[2] = {mx[0], mx[1]};
+#pragma unroll
+        for (int i = 0; i < KT / 8; ++i) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = sc[i][e] * p.scale_log2;
+            if (!full) {
+              const int j = j0 + i * 8 + (lane & 3) * 2 + (e & 1);
+              if (!sees(rpos[e >> 1], j, s.len_k, s.causal, p.window, p.sinks)) x = -INFINITY;
+            }
+            sc[i][e] = x;
+            mn[e >> 1] = fmaxf(mn[e >> 1], x);
+          }
+        }
+        float corr[2], base_m[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          mn[e] = fmaxf(mn[e], __shfl_xor_sync(0xffffffffu, mn[e], 1));
+          mn[e] = fmaxf(mn[e], __shfl_xor_sync(0xffffffffu, mn[e], 2));
+          base_m[e] = mn[e] == -INFINITY ? 0.f : mn[e];
+          corr[e] = exp2_approx(mx[e] - base_m[e]);
+          mx[e] = mn[e];
+          sum[e] *= corr[e];
+        }
+        uint32_t pf[KT / 16][4];
+#pragma unroll
+        for (int i = 0; i < KT / 8; ++i) {
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = exp2_approx(sc[i][e] - base_m[e >> 1]);
+            sum[e >> 1] += x[e];
+          }
+          pf[i >> 1][(i & 1) * 2] = pack16<BF16>(x[0], x[1]);
+          pf[i >> 1][(i & 1) * 2 + 1] = pack16<BF16>(x[2], x[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1];
+        }
+        if (!full) {
+          // V of keys that no row of the block sees may be anything (0 x NaN is NaN): clear it
+          const int j = j0 + lane;
+          if (!(j < sp.hi && (j >= sp.lo || j < sp.sinks))) {
+            uint4* vr = reinterpret_cast<uint4*>(ring + st * 2 * C::TILE + C::TILE + lane * 128);
+#pragma unroll
+            for (int c = 0; c < C::CH; ++c)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) vr[c * (KT * 8) + i] = make_uint4(0, 0, 0, 0);
+          }
+          rb::fence_proxy_async_smem();
+          __syncwarp();
+        }
+        // O += P V
+#pragma unroll
+        for (int kk = 0; kk < KT / 16; ++kk) {
+#pragma unroll
+          for (int n = 0; n < D / 16; ++n) {
+            const int r = kk * 16 + (lane & 15);
+            const int unit = (n & 3) * 2 + (lane >> 4);
+            uint32_t b0, b1, b2, b3;
+            ldsm4_trans(v_addr + (n >> 2) * (KT * 128) + r * 128 + ((unit ^ (r & 7)) << 4), b0, b1, b2, b3);
+            mma16816<BF16>(o[2 * n], pf[kk], b0, b1);
+            mma16816<BF16>(o[2 * n + 1], pf[kk], b2, b3);
+          }
+        }
+        __syncwarp();
+        if (nxt < v1) { issue(nxt); nxt += NW; }
+      }
+      if (dead) {                                                              // the kernel's own copies end before it does
+        for (; used < issued; ++used)
+          for (uint32_t i = 0; i < (1u << 20) && !rb::mbar_try_wait(&bar[used % C::STAGES], (used / C::STAGES) & 1); ++i) {}
+      }
+      // ---- join the warps: o [RT][D] in the warp's own, now idle ring
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
+        sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
+        const int r = (lane >> 2) + 8 * e;
+        float* dst = reinterpret_cast<float*>(ring) + r * D + (lane & 3) * 2;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
+        if ((lane & 3) == 0) { ml[(warp * RT + r) * 2] = mx[e]; ml[(warp * RT + r) * 2 + 1] = sum[e]; }
+      }
+      __syncthreads();
+      {
+        constexpr int TPR = NW * 32 / RT, N = 4;                               // threads per row, elements at a time
+        const int r = tid / TPR;
+        if (r < rows) {
+          float mm = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < NW; ++i) mm = fmaxf(mm, ml[(i * RT + r) * 2]);
+          const float bm = mm == -INFINITY ? 0.f : mm;
+          float f[NW], l = 0.f;
+#pragma unroll
+          for (int i = 0; i < NW; ++i) {
+            f[i] = exp2_approx(ml[(i * RT + r) * 2] - bm);
+            l += f[i] * ml[(i * RT + r) * 2 + 1];
+          }
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          const float lse2 = l == 0.f ? -INFINITY : mm + log2f(l);
+          const bool whole = off == 0 && u1 == it.units;
+          const long long cut = static_cast<long long>(cta) * 2 + (pos == p0 ? 0 : 1);
+          for (int col = (tid % TPR) * N; col < D; col += TPR * N) {
+            float x[N] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+              const float4 y = *reinterpret_cast<const float4*>(smem + i * (C::STAGES * 2 * C::TILE) + (r * D + col) * 4);
+              x[0] += f[i] * y.x; x[1] += f[i] * y.y; x[2] += f[i] * y.z; x[3] += f[i] * y.w;
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] *= inv;
+            if (whole) {
+              write_row<D, BF16, N>(p, w, s, qt * RT + r, h, col, x, lse2);
+            } else {
+              *reinterpret_cast<float4*>(w.cut_o + (cut * RT + r) * D + col) = make_float4(x[0], x[1], x[2], x[3]);
+              if (col == 0) w.cut_lse[cut * RT + r] = lse2;
+            }
+          }
+        }
+      }
+      rb::fence_proxy_async_smem();
+      __syncthreads();
+      pos += u1 - off;
+    }
+  }
+  if (tid == 0) w.meta[cta] = m;
+}
+
+// Joins the pieces of the items that borders cut: CTA c looks after the item whose first border is share c's begin.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(128) attn_join_kernel(const Batch p, const Outs w) {
+  const Meta m = w.meta[blockIdx.x];
+  if (!m.valid) return;
+  const Seq s = seq_of(p, m.seq);
+  const int rows = min(s.len_q * p.G - m.qt * RT, RT);
+  constexpr int TPR = 128 / RT, N = 4;
+  const int r = threadIdx.x / TPR;
+  if (r >= rows) return;
+  auto cut = [&](int c) {
+    const long long b = share(c, m.n, m.total);
+    return (static_cast<long long>(c) * 2 + (b >= m.t0 ? 0 : 1)) * RT + r;
+  };
+  float mm = -INFINITY;
+  for (int c = m.c0; c <= m.c1; ++c) mm = fmaxf(mm, w.cut_lse[cut(c)]);
+  const float bm = mm == -INFINITY ? 0.f : mm;
+  float l = 0.f;
+  float x[D / (TPR * N)][N];
+#pragma unroll
+  for (int k = 0; k < D / (TPR * N); ++k) x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0.f;
+#pragma unroll 4
+  for (int c = m.c0; c <= m.c1; ++c) {
+    const long long at = cut(c);
+    const float f = exp2_approx(w.cut_lse[at] - bm);
+    l += f;
+#pragma unroll
+    for (int k = 0; k < D / (TPR * N); ++k) {
+      const float4 y = *reinterpret_cast<const float4*>(w.cut_o + at * D + (threadIdx.x % TPR) * N + k * TPR * N);
+      x[k][0] += f * y.x; x[k][1] += f * y.y; x[k][2] += f * y.z; x[k][3] += f * y.w;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float lse2 = l == 0.f ? -INFINITY : mm + log2f(l);
+#pragma unroll
+  for (int k = 0; k < D / (TPR * N); ++k) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[k][i] *= inv;
+    write_row<D, BF16, N>(p, w, s, m.qt * RT + r, m.h, (threadIdx.x % TPR) * N + k * TPR * N, x[k], lse2);
+  }
+}
+
+// out = the two parts of every row (prefix, suffix), weighted by their sums
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) attn_merge_kernel(const Batch p, const Outs w) {
+  constexpr int TPR = D / 4;
+  const long long rows = static_cast<long long>(p.Tq) * p.H;
+  const long long row = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / TPR;
+  if (row >= rows) return;
+  const int col = (threadIdx.x % TPR) * 4;
+  // tokens of requests in no group have no first part, tokens of no request neither
+  const int t = static_cast<int>(row / p.H);
+  const int* go = p.a.group_offsets;
+  const bool has_a = t >= p.a.q_offsets[min(max(go[0], 0), p.a.num_requests)] && t < p.a.q_offsets[min(max(go[p.a.B], 0), p.a.num_requests)];
+  const bool has_b = t >= p.b.q_offsets[0] && t < p.b.q_offsets[p.b.B];
+  const float a = has_a ? w.part_lse[row] : -INFINITY, b = has_b ? w.part_lse[rows + row] : -INFINITY;
+  const float mm = fmaxf(a, b), bm = mm == -INFINITY ? 0.f : mm;
+  const float fa = exp2_approx(a - bm), fb = exp2_approx(b - bm), l = fa + fb;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+  if (has_a) x = *reinterpret_cast<const float4*>(w.part_o + row * D + col);
+  if (has_b) y = *reinterpret_cast<const float4*>(w.part_o + (rows + row) * D + col);
+  const float z0 = (fa * x.x + fb * y.x) * inv, z1 = (fa * x.y + fb * y.y) * inv, z2 = (fa * x.z + fb * y.z) * inv,
+              z3 = (fa * x.w + fb * y.w) * inv;
+  uint16_t* dst = reinterpret_cast<uint16_t*>(w.out) + t * w.ld_o + (row % p.H) * D + col;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<BF16>(z0, z1), pack16<BF16>(z2, z3));
+  if (col == 0 && w.lse) w.lse[row] = l == 0.f ? -INFINITY : (mm + log2f(l)) * LN2;
+}
+
+constexpr long long align256(long long n) { return (n + 255) / 256 * 256; }
+
+struct Space { long long cut_o, cut_lse, meta, part_o, part_lse, total; };
+
+Space space_of(int n_cta, int D, long long rows, bool parts) {
+  Space s;
+  s.cut_o = 0;
+  s.cut_lse = align256(s.cut_o + static_cast<long long>(n_cta) * 2 * RT * D * 4);
+  s.meta = align256(s.cut_lse + static_cast<long long>(n_cta) * 2 * RT * 4);
+  s.part_o = align256(s.meta + static_cast<long long>(n_cta) * static_cast<long long>(sizeof(Meta)));
+  s.part_lse = align256(s.part_o + (parts ? 2 * rows * D * 4 : 0));
+  s.total = align256(s.part_lse + (parts ? 2 * rows * 4 : 0));
+  return s;
+}
+
+template <int D, bool BF16>
+int launch(const CUtensorMap& tm, const Batch& p, Outs w, int n_cta, bool parts, cudaStream_t st) {
+  RB_CUDA_CHECK(cudaFuncSetAttribute(attn_rows_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM));
+  attn_rows_kernel<D, BF16><<<n_cta, NW * 32, Cfg<D>::SMEM, st>>>(tm, p, w);
+  RB_CUDA_CHECK(cudaGetLastError());
+  attn_join_kernel<D, BF16><<<n_cta, 128, 0, st>>>(p, w);
+  RB_CUDA_CHECK(cudaGetLastError());
+  if (parts) {
+    const long long rows = static_cast<long long>(p.Tq) * p.H;
+    const int per = 256 / (D / 4);
+    attn_merge_kernel<D, BF16><<<static_cast<int>((rows + per - 1) / per), 256, 0, st>>>(p, w);
+    RB_CUDA_CHECK(cudaGetLastError());
+  }
+  return 0;
+}
+
+}  // namespace
+
+// Bytes of workspace that rb_softmax_attn_paged needs.
+RB_API long long rb_softmax_attn_workspace(int num_sms, long long Tq, int H, int D, int prefix) {
+  return space_of(num_sms > 0 ? num_sms : 148, D, Tq * H, prefix != 0).total;
+}
+
+// q [Tq][H][D] (token stride ld_q), cache [num_pages][2][page_size][Hkv][D], bf16 or fp16; int32 offsets and page tables on
+// the device.  B requests own the queries q_offsets[b]..q_offsets[b+1] and k_offsets[b+1] - k_offsets[b] keys, the last of which are
+// the queries' own.  G groups (0: none) of requests group_offsets[g]..group_offsets[g+1] - or, without group_offsets, ONE
+// group of all requests - see prefix_offsets[g+1] - prefix_offsets[g] more keys in front of their own; window and sinks
+// are for calls without groups.  out [Tq][H][D] (token stride ld_o), lse [Tq][H] fp32 or null.
+RB_API int rb_softmax_attn_paged(const void* q, long long ld_q, long long Tq, int H, int Hkv, int D, const void* cache,
+                                 long long num_pages, int page_size, const int* q_offsets, const int* k_offsets,
+                                 const int* page_ids, const int* page_indptr, int num_page_ids, int B, const int* group_offsets,
+                                 const int* prefix_offsets, const int* prefix_page_ids, const int* prefix_page_indptr,
+                                 int num_prefix_page_ids, int groups, int window, int sinks, float scale, int is_bf16, void* out,
+                                 long long ld_o, float* lse, void* workspace, long long workspace_bytes, int num_sms, int* status,
+                                 cudaStream_t st) {
+  if (Tq == 0 || B == 0) return 0;
+  if ((D != 64 && D != 128) || Hkv <= 0 || H % Hkv) return -1;
+  if (ld_q % 8 || ld_o % 8) return -2;
+  if (page_size % 16 || page_size <= 0 || (groups > 0 && window > 0)) return -3;
+  const long long rows = num_pages * 2 * page_size;
+  if (Tq * H > 0x7fffffffLL || rows + page_size > 0x7fffffffLL) return -4;
+  const int n_cta = num_sms > 0 ? num_sms : 148;
+  const Space sp = space_of(n_cta, D, Tq * H, groups > 0);
+  if (workspace_bytes < sp.total) return -5;
+  Batch p;
+  const Seqs own = {q_offsets, nullptr, k_offsets, page_ids, page_indptr, num_page_ids, B, B, 1};
+  const Seqs none = {nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0, 0, 0};
+  const Seqs pre = {q_offsets, group_offsets, prefix_offsets, prefix_page_ids, prefix_page_indptr, num_prefix_page_ids, groups, B, 0};
+  p.a = groups > 0 ? pre : own;
+  p.b = groups > 0 ? own : none;
+  p.q = q; p.ld_q = ld_q; p.Tq = static_cast<int>(Tq); p.H = H; p.Hkv = Hkv; p.G = H / Hkv; p.page_size = page_size;
+  p.box_rows = page_size % KT == 0 ? KT : 16; p.total_rows = static_cast<int>(rows); p.window = window; p.sinks = sinks;
+  p.scale_log2 = scale * LOG2E; p.status = status;
+  char* ws = static_cast<char*>(workspace);
+  Outs w;
+  w.out = out; w.ld_o = ld_o; w.lse = lse;
+  w.part_o = groups > 0 ? reinterpret_cast<float*>(ws + sp.part_o) : nullptr;
+  w.part_lse = reinterpret_cast<float*>(ws + sp.part_lse);
+  w.cut_o = reinterpret_cast<float*>(ws + sp.cut_o);
+  w.cut_lse = reinterpret_cast<float*>(ws + sp.cut_lse);
+  w.meta = reinterpret_cast<Meta*>(ws + sp.meta);
+  CUtensorMap tm;
+  const int rc = rb_host::make_map_2d(&tm, cache, rows, static_cast<long long>(Hkv) * D, static_cast<long long>(Hkv) * D, 64,
+                                      p.box_rows, is_bf16 != 0);
+  if (rc) return rc;
+  if (D == 64) return is_bf16 ? launch<64, true>(tm, p, w, n_cta, groups > 0, st) : launch<64, false>(tm, p, w, n_cta, groups > 0, st);
+  return is_bf16 ? launch<128, true>(tm, p, w, n_cta, groups > 0, st) : launch<128, false>(tm, p, w, n_cta, groups > 0, st);
+}

@@ -1,0 +1,119 @@
+// What the softmax-attention kernels over the paged KV cache share: the description of a batch, which keys a block of
+// query rows sees, and how their partial results are laid out.
+#pragma once
+#include "common.cuh"
+
+namespace rb_attn {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+// One list of sequences whose keys live in pages.  A query row is (token, head); the rows of the G = H / Hkv heads that
+// share a key head are packed: row r of a sequence is token r / G, head r % G of the group.
+struct Seqs {
+  const int* q_offsets;       // [B+1] rows of q per sequence ...
+  const int* group_offsets;   // ... or null; [B+1] into q_offsets: sequence g holds the queries of requests go[g]..go[g+1]-1
+  const int* k_offsets;       // [B+1] keys per sequence (differences are used)
+  const int* page_ids;
+  const int* page_indptr;     // [B+1]
+  int num_page_ids;
+  int B;
+  int num_requests;           // q_offsets has num_requests + 1 entries
+  int causal;                 // a row sees the keys up to its own position; 0: all of them
+};
+
+struct Batch {
+  Seqs a, b;                  // sequences of b (may be none) are numbered after those of a
+  const void* q; long long ld_q;
+  int Tq, H, Hkv, G;
+  int page_size, box_rows, total_rows;   // of the cache as a matrix [pages * 2 * page_size][Hkv * D]
+  int window, sinks;          // window 0: no limit
+  float scale_log2;           // scale * log2(e)
+  int* status;
+};
+
+struct Seq {
+  int q_begin, len_q, len_k, page_begin, page_end, causal, part;
+  const int* page_ids;
+  __device__ __forceinline__ int delta() const { return len_k - len_q; }
+};
+
+__device__ __forceinline__ Seq seq_of(const Batch& p, int i) {
+  const bool second = i >= p.a.B;
+  const Seqs& s = second ? p.b : p.a;
+  const int j = second ? i - p.a.B : i;
+  Seq r;
+  int q0 = j, q1 = j + 1;
+  if (s.group_offsets) {
+    q0 = min(max(s.group_offsets[j], 0), s.num_requests);
+    q1 = min(max(s.group_offsets[j + 1], q0), s.num_requests);
+  }
+  // rows outside q are never touched, whatever the offsets say
+  r.q_begin = min(max(s.q_offsets[q0], 0), p.Tq);
+  r.len_q = min(max(s.q_offsets[q1], r.q_begin), p.Tq) - r.q_begin;
+  r.len_k = max(s.k_offsets[j + 1] - s.k_offsets[j], 0);
+  r.page_begin = max(s.page_indptr[j], 0);
+  r.page_end = min(s.page_indptr[j + 1], s.num_page_ids);
+  r.page_ids = s.page_ids;
+  r.causal = s.causal;
+  r.part = second ? 1 : 0;
+  return r;
+}
+
+// Keys that a block of consecutive rows may see, in tiles of T keys aligned to multiples of T: first the tiles that hold
+// sinks, then the tiles of the window.
+struct Span {
+  int p_min, p_max;           // positions of the first and the last token of the block
+  int hi;                     // keys at or past it are seen by no row of the block
+  int lo;                     // keys before it are seen by no row, unless they are sinks
+  int sinks;
+  int sink_tiles, first, tiles;   // tile v is v < sink_tiles ? v : first + v - sink_tiles
+  __device__ __forceinline__ int tile(int v) const { return v < sink_tiles ? v : first + v - sink_tiles; }
+};
+
+template <int T>
+__device__ __forceinline__ Span span_of(const Batch& p, const Seq& s, int t_lo, int t_hi) {
+  Span r;
+  const int delta = s.delta();
+  r.p_min = s.causal ? t_lo + delta : s.len_k - 1;
+  r.p_max = s.causal ? t_hi + delta : s.len_k - 1;
+  r.hi = max(min(s.len_k, r.p_max + 1), 0);
+  const bool win = s.causal && p.window > 0;
+  r.lo = win ? max(r.p_min - p.window + 1, 0) : 0;
+  r.sinks = win ? min(p.sinks, r.hi) : 0;
+  const int end = (r.hi + T - 1) / T;
+  r.first = r.lo / T;
+  r.sink_tiles = min((r.sinks + T - 1) / T, r.first);
+  r.tiles = r.sink_tiles + max(end - r.first, 0);
+  return r;
+}
+
+// whether the row at position pos sees key j (j < len_k)
+__device__ __forceinline__ bool sees(int pos, int j, int hi, int causal, int window, int sinks) {
+  return j < hi && (!causal || (j <= pos && (window <= 0 || j > pos - window || j < sinks)));
+}
+
+// Row of the cache matrix where the box of keys j.. starts (K; V is page_size rows further), or a row past the end, which
+// a TMA load fills with zeros: for boxes of keys that no row of the block sees, whose pages may be gone, and - reported -
+// for pages that are not there.
+__device__ __forceinline__ int box_row(const Batch& p, const Seq& s, const Span& r, int j) {
+  if (j >= r.hi || (j + p.box_rows <= r.lo && j >= r.sinks)) return p.total_rows;
+  const int at = s.page_begin + j / p.page_size;
+  const int per_page = 2 * p.page_size;
+  if (at < s.page_end) {
+    const int page = __ldg(s.page_ids + at);
+    if (page >= 0 && page < p.total_rows / per_page) return page * per_page + j % p.page_size;
+  }
+  if (p.status) atomicCAS(p.status, 0, RB_ERR_BOUNDS);
+  return p.total_rows;
+}
+
+template <bool BF16> __device__ __forceinline__ uint32_t pack16(float a, float b) { return BF16 ? rb::pack_bf16(a, b) : rb::pack_f16(a, b); }
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace rb_attn

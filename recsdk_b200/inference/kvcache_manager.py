@@ -29,6 +29,7 @@ import torch
 from ..host import host
 from ..ops import _lib
 from ..ops import embedding_ops as E
+from ..ops.softmax_attention import append_kv_rotary
 
 
 class KVCacheOffloadMode(str, enum.Enum):
@@ -408,6 +409,15 @@ class GPUKVCacheManager:
         cache[page, 1, p % ps] = v.to(cache.dtype)
 
     put = append_kvcache
+
+    def append_kvcache_rotary(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, md: KVCacheMetadata,
+                              table: torch.Tensor, interleaved: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """:meth:`append_kvcache` for models with rotary positions: the keys (and the queries ``[nnz, q_heads, head_dim]``,
+        which are returned) are turned by the tokens' positions on the way (:func:`~recsdk_b200.ops.softmax_attention.append_kv_rotary`).
+        Rows behind ``md.new_history_nnz_npu`` (the padding of preallocated metadata) are left alone."""
+        n = q.shape[0]
+        return append_kv_rotary(q, k, v, self.cache[layer], md.batch_indices[:n], md.position[:n], md.kv_indices, md.kv_indptr,
+                                self.cfg.page_size, table, interleaved, num_tokens=md.new_history_nnz_npu, out=out)
 
     # ---- offload bookkeeping (thin wrappers over the native allocator)
     def check_for_offload(self, user_ids: torch.Tensor) -> torch.Tensor:

@@ -14,13 +14,14 @@ The request flow (lookup -> allocate -> onboard -> layers -> offload) is the ref
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
 from ..inference.kvcache_manager import HostKVTaskStatus, KVCacheManager, KVIndexMeta
 from ..ops import gemm, hstu_ops
 from ..ops.hstu_attention import hstu_attention_paged, hstu_attention_ref
+from ..ops.sampling import sample_scores
 from .hstu import HSTU
 
 
@@ -96,6 +97,17 @@ class HSTURanker:
         kv.gpu.truncate(meta.user_ids, history_lengths)
         kv.offload_launch(KVIndexMeta(meta.user_ids, history_lengths.cpu().int()), md)
         return scores
+
+    def recommend(self, user_ids: torch.Tensor, history_lengths: torch.Tensor, num_candidates: torch.Tensor, x_new: torch.Tensor,
+                  uniform: torch.Tensor, timestamps: Optional[torch.Tensor] = None, temperature=1.0, top_k=0, top_p=1.0,
+                  min_p=0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+        """:meth:`rank`, then one of every user's candidates drawn from their scores
+        (:func:`~recsdk_b200.ops.sampling.sample_scores` with the given ``uniform [B]``): its index among the user's
+        candidates (-1: none) and the log of its probability, the propensity of off-policy training."""
+        scores = self.rank(user_ids, history_lengths, num_candidates, x_new, timestamps)
+        offsets = torch.zeros(num_candidates.numel() + 1, dtype=torch.int64)
+        torch.cumsum(num_candidates, 0, out=offsets[1:])
+        return sample_scores(scores, uniform, offsets.to(scores.device), temperature, top_k, top_p, min_p)
 
     def plan(self, user_ids: torch.Tensor, history_lengths: torch.Tensor) -> torch.Tensor:
         """How many history tokens of each user are already cached (either tier): the caller sends embeddings

@@ -40,7 +40,8 @@ def _declare(lib: ctypes.CDLL) -> None:
 
 # kernels launched by one call of a launcher (default 1); used for the launch counter only
 _KERNELS_PER_CALL = {"rb_sort_segments": 8, "rb_sort_pairs_i64_i32": 4, "rb_tbe_backward_update": 2, "rb_tbe_backward_update_rows": 2, "rb_a2a_ctl_ints": 0, "rb_a2a_loc_ints": 0, "rb_a2a_loc_n_owned_index": 0,
-                     "rb_allreduce_push_staging_bytes": 0, "rb_allreduce_push_max_blocks": 0, "rb_sort_segments_temp_bytes": 0}
+                     "rb_allreduce_push_staging_bytes": 0, "rb_allreduce_push_max_blocks": 0, "rb_sort_segments_temp_bytes": 0,
+                     "rb_softmax_attn_paged": 2, "rb_softmax_attn_workspace": 0}
 launch_count = 0
 
 
@@ -101,6 +102,25 @@ def available() -> bool:
 
 def stream_ptr(device: Optional[torch.device] = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class on_device:
+    """Makes the tensors' device current for a launch (a stream only takes launches of its own device)."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device: torch.device) -> None:
+        self.index, self.before = device.index, None
+
+    def __enter__(self) -> None:
+        now = torch.cuda.current_device()
+        if self.index is not None and now != self.index:
+            self.before = now
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.before is not None:
+            torch.cuda.set_device(self.before)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -1,0 +1,125 @@
+"""Drawing one item per row from its scores on ``csrc/cuda/sampling.cu``: temperature, top-k, top-p and min-p, from given
+uniform numbers.  Rows are dense ``[B, V]`` or jagged (the scores of every user's own candidates, as
+``HSTURanker.rank`` returns them).  ``sample_scores_ref`` states the same in 64-bit PyTorch for CPU tensors and the tests."""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _lib
+
+Param = Union[float, int, torch.Tensor]
+
+
+def _param(name: str, value: Param, rows: int, dtype: torch.dtype, device, lo: float, hi: float, open_lo: bool = False):
+    """-> (per-row tensor or None, scalar).  Scalars are checked; what tensors hold is taken as it is."""
+    if isinstance(value, torch.Tensor):
+        if value.shape != (rows,) or value.device != device:
+            raise ValueError("%s must be a scalar or a [%d] tensor on %s, got %s on %s"
+                             % (name, rows, device, tuple(value.shape), value.device))
+        if dtype is torch.int32 and value.dtype not in (torch.int32, torch.int64):
+            raise ValueError("%s must hold integers, got %s" % (name, value.dtype))
+        return value.to(dtype).contiguous(), 0
+    if not (value >= lo and value <= hi) or (open_lo and value == lo):
+        raise ValueError("%s = %r is outside %s%g, %g]" % (name, value, "(" if open_lo else "[", lo, hi))
+    return None, value
+
+
+def sample_scores(scores: torch.Tensor, uniform: torch.Tensor, offsets: Optional[torch.Tensor] = None, temperature: Param = 1.0,
+                  top_k: Param = 0, top_p: Param = 1.0, min_p: Param = 0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """One item per row -> ``(ids [B] int64, logprobs [B] fp32)``.
+
+    ``scores``: fp32 / fp16 / bf16, ``[B, V]`` (any row stride) or, with ``offsets [B + 1]`` (int32 / int64), the rows one
+    after another ``[T]``.  ``uniform [B]`` fp32: numbers in ``[0, 1)``.  In the order (score descending, index ascending)
+    the filters keep the first ``top_k`` items (0: all); of those, up to and with the one at which the running sum of
+    ``exp(score / temperature)`` reaches ``top_p`` of their sum; of those, the ones with at least ``min_p`` times the
+    largest weight.  The item drawn is the first one, in index order, whose running sum over the kept items exceeds
+    ``uniform`` times their sum.  ``temperature = 0`` takes the largest score (the first of equals).  Every parameter is a
+    number or a ``[B]`` tensor on the scores' device; in a tensor ``top_k <= 0`` and ``top_p >= 1`` are off and
+    ``temperature <= 0`` takes the largest score.
+
+    ``ids`` count within the row; ``logprobs`` is the log of the drawn item's share of what was kept (0 for
+    ``temperature = 0``) - the propensity to log.  NaN and ``-inf`` are never drawn; a row with nothing else, or with
+    nothing at all, gives ``-1`` and ``-inf``.  Sums are in 64 bits and the result does not depend on the launch."""
+    if offsets is None:
+        if scores.dim() != 2:
+            raise ValueError("scores must be [B, V], or [T] with offsets; got %s" % (tuple(scores.shape),))
+        rows, width = scores.shape
+    else:
+        if scores.dim() != 1 or offsets.dim() != 1 or offsets.numel() < 1:
+            raise ValueError("jagged scores must be [T] with offsets [B + 1]; got %s and %s"
+                             % (tuple(scores.shape), tuple(offsets.shape)))
+        if offsets.dtype not in (torch.int32, torch.int64) or offsets.device != scores.device:
+            raise ValueError("offsets must be int32 or int64 on the scores' device")
+        rows, width = offsets.numel() - 1, scores.shape[0]
+    dev = scores.device
+    if uniform.shape != (rows,) or uniform.dtype != torch.float32 or uniform.device != dev:
+        raise ValueError("uniform must be [%d] fp32 on %s" % (rows, dev))
+    if scores.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError("scores must be fp32, fp16 or bf16, got %s" % (scores.dtype,))
+    if width >= 1 << 31:
+        raise ValueError("rows of 2^31 and more scores are not supported")
+    big = torch.finfo(torch.float32).max
+    t_t, t_v = _param("temperature", temperature, rows, torch.float32, dev, 0.0, big)
+    k_t, k_v = _param("top_k", top_k, rows, torch.int32, dev, 0, (1 << 31) - 1)
+    p_t, p_v = _param("top_p", top_p, rows, torch.float32, dev, 0.0, 1.0, open_lo=True)
+    m_t, m_v = _param("min_p", min_p, rows, torch.float32, dev, 0.0, 1.0)
+    if not scores.is_cuda:
+        return sample_scores_ref(scores, uniform, offsets, temperature, top_k, top_p, min_p)
+    with _lib.on_device(dev):
+        if scores.stride(-1) != 1 and width > 1:
+            scores = scores.contiguous()
+        uniform = uniform.contiguous()
+        if offsets is not None:
+            offsets = offsets.contiguous()
+        ids = torch.empty(rows, dtype=torch.int64, device=dev)
+        logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
+        rc = _lib.lib().rb_sample_scores(scores.data_ptr(), scores.stride(0) if offsets is None else 0, _lib.ptr(offsets),
+                                         int(offsets is not None and offsets.dtype == torch.int64), width, rows,
+                                         uniform.data_ptr(), _lib.ptr(t_t), _lib.ptr(k_t), _lib.ptr(p_t), _lib.ptr(m_t),
+                                         float(t_v), int(k_v), float(p_v), float(m_v), ids.data_ptr(), logprobs.data_ptr(),
+                                         _lib.dtype_code(scores.dtype), _lib.stream_ptr(dev))
+        _lib.check(rc, "rb_sample_scores")
+    return ids, logprobs
+
+
+def sample_scores_ref(scores, uniform, offsets=None, temperature: Param = 1.0, top_k: Param = 0, top_p: Param = 1.0,
+                      min_p: Param = 0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The definition of :func:`sample_scores`, row by row in 64 bits (parameters are taken as their fp32 values)."""
+    rows = scores.shape[0] if offsets is None else offsets.numel() - 1
+    off = None if offsets is None else offsets.tolist()
+    at = lambda v, r: float(torch.as_tensor(v[r] if isinstance(v, torch.Tensor) else v, dtype=torch.float32))  # noqa: E731
+    ids = torch.full((rows,), -1, dtype=torch.int64)
+    logprobs = torch.full((rows,), -math.inf, dtype=torch.float64)
+    for r in range(rows):
+        x = (scores[r] if off is None else scores[off[r]:off[r + 1]]).double().cpu()
+        x = torch.where(torch.isnan(x), torch.full_like(x, -math.inf), x)
+        if x.numel() == 0 or float(x.max()) == -math.inf:
+            continue
+        order = torch.sort(x, descending=True, stable=True)[1]
+        order = order[x[order] > -math.inf]
+        t = at(temperature, r)
+        if not t > 0:
+            ids[r], logprobs[r] = order[0], 0.0
+            continue
+        top = x[order[0]]
+        w = torch.where(x[order] == top, torch.ones((), dtype=torch.float64), torch.exp((x[order] - top) / t))
+        k = int(top_k[r] if isinstance(top_k, torch.Tensor) else top_k)
+        if k > 0:
+            order, w = order[:k], w[:k]
+        if at(top_p, r) < 1.0:
+            run = torch.cumsum(w, 0)
+            n = 1 + int((run[:-1] < at(top_p, r) * run[-1]).sum())
+            order, w = order[:n], w[:n]
+        keep = w >= at(min_p, r)
+        keep[0] = True
+        order, w = order[keep], w[keep]
+        order, back = torch.sort(order)
+        run = torch.cumsum(w[back], 0)
+        u = float(uniform[r])
+        over = (run > max(u if u == u else 0.0, 0.0) * run[-1]) & (w[back] > 0)
+        i = int(over.nonzero()[0]) if bool(over.any()) else int((w[back] > 0).nonzero()[-1])
+        ids[r], logprobs[r] = order[i], math.log(float(w[back][i] / run[-1]))
+    return ids.to(scores.device), logprobs.float().to(scores.device)

@@ -1,0 +1,293 @@
+"""Softmax attention over the paged KV cache, for serving: the counterparts of ``append_kvcache`` and
+``hstu_attention_paged`` for models with rotary positions and ordinary attention.
+
+* ``append_kv_rotary`` writes the new tokens' keys (turned by their positions) and values into their pages and returns the
+  turned queries (``csrc/cuda/kv_rotary.cu``),
+* ``softmax_attention_paged`` attends from the new tokens to the cache: causal, optionally only to a sliding window and
+  the first few tokens; grouped query heads (``csrc/cuda/softmax_attention.cu``),
+* ``softmax_attention_shared_prefix`` does so for groups of requests - one user's candidates or beams - whose histories
+  begin with the same tokens: those are read and multiplied once per group.
+
+The cache is the manager's ``[pages, 2, page_size, kv_heads, head_dim]`` of one layer; offsets, page ids and positions are
+those of :class:`~recsdk_b200.inference.KVCacheMetadata`.  There is no gradient.  CPU tensors take the fp32 statements
+(``*_ref``), which are also what the tests compare with."""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+_HEAD_DIMS = (64, 128)
+
+
+def rotary_table(max_positions: int, rotary_dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """fp32 ``[max_positions, rotary_dim]``: ``rotary_dim / 2`` cosines, then as many sines of ``position * base^(-2i /
+    rotary_dim)``, computed in 64 bits (a far position times a frequency has no correct digit of its angle left in 32)."""
+    if rotary_dim <= 0 or rotary_dim % 16 or max_positions <= 0:
+        raise ValueError("rotary_dim must be a positive multiple of 16 and max_positions positive")
+    half = rotary_dim // 2
+    freq = torch.pow(torch.tensor(base, dtype=torch.float64), -torch.arange(half, dtype=torch.float64) / half)
+    ang = torch.arange(max_positions, dtype=torch.float64)[:, None] * freq[None, :]
+    return torch.cat([ang.cos(), ang.sin()], dim=1).float().to(device if device is not None else "cpu")
+
+
+# ----------------------------------------------------------------------------- checks
+def _rows(name: str, x: torch.Tensor, heads: Optional[int], dim: int, like: torch.Tensor) -> torch.Tensor:
+    """[T, heads, dim] with adjacent heads and 16-byte aligned rows (others are copied)."""
+    if x.dim() != 3 or (heads is not None and x.shape[1] != heads) or x.shape[2] != dim:
+        raise ValueError("%s must be [tokens, %s, %d], got %s" % (name, "heads" if heads is None else heads, dim, tuple(x.shape)))
+    if x.dtype != like.dtype or x.device != like.device:
+        raise ValueError("%s must be %s on %s like the cache, got %s on %s" % (name, like.dtype, like.device, x.dtype, x.device))
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError("%s requires a gradient, which this operator does not have (use torch.no_grad())" % name)
+    if x.is_cuda and x.numel() and (x.stride(2) != 1 or x.stride(1) != dim or x.stride(0) % 8 or x.stride(0) < 0 or x.data_ptr() % 16):
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    return x
+
+
+def _ints(name: str, x: torch.Tensor, device, n: Optional[int] = None) -> torch.Tensor:
+    if x.dim() != 1 or (n is not None and x.numel() != n):
+        raise ValueError("%s must be a vector%s, got %s" % (name, "" if n is None else " of %d" % n, tuple(x.shape)))
+    if x.dtype not in (torch.int32, torch.int64) or x.device != device:
+        raise ValueError("%s must be int32 or int64 on %s, got %s on %s" % (name, device, x.dtype, x.device))
+    return x if x.dtype == torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+
+
+def _cache(kv_cache: torch.Tensor, page_size: int, dims=None) -> torch.Tensor:
+    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2 or kv_cache.shape[2] != page_size or not kv_cache.is_contiguous():
+        raise ValueError("kv_cache must be a contiguous [pages, 2, %d, kv_heads, head_dim], got %s" % (page_size, tuple(kv_cache.shape)))
+    if kv_cache.is_cuda:
+        if kv_cache.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("kv_cache must be bf16 or fp16, got %s" % (kv_cache.dtype,))
+        if dims is not None and kv_cache.shape[4] not in dims:
+            raise ValueError("head_dim must be one of %s, got %d" % (dims, kv_cache.shape[4]))
+        if kv_cache.data_ptr() % 16:
+            raise ValueError("kv_cache must be 16-byte aligned")
+    return kv_cache
+
+
+# ----------------------------------------------------------------------------- append
+def _rotate_ref(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool) -> torch.Tensor:
+    half = cos.shape[-1]
+    y = x.to(torch.float64 if x.dtype == torch.float64 else torch.float32).clone()
+    first = slice(0, 2 * half, 2) if interleaved else slice(0, half)
+    second = slice(1, 2 * half, 2) if interleaved else slice(half, 2 * half)
+    a, b = y[..., first].clone(), y[..., second].clone()
+    y[..., first], y[..., second] = a * cos - b * sin, b * cos + a * sin
+    return y.to(x.dtype)
+
+
+def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor, batch_indices: torch.Tensor,
+                     positions: torch.Tensor, page_ids: torch.Tensor, page_indptr: torch.Tensor, page_size: int,
+                     table: torch.Tensor, interleaved: bool = False, num_tokens: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Turn the new tokens' queries and keys by their positions, write keys and values into their pages, return the queries.
+
+    ``q [n, heads, head_dim]``, ``k`` / ``v [n, kv_heads, head_dim]`` (token stride free, e.g. slices of one projection);
+    token ``i`` is token ``positions[i]`` of request ``batch_indices[i]``, whose pages are
+    ``page_ids[page_indptr[b]:page_indptr[b + 1]]``.  ``table`` is :func:`rotary_table`'s ``[max_positions, rotary_dim]``
+    (or any cosines and sines); the first ``rotary_dim`` elements of a head turn, element ``i`` with ``i + rotary_dim / 2``
+    or, ``interleaved``, ``2i`` with ``2i + 1``.  No two tokens of a call may name the same position of a request.
+
+    ``num_tokens``: optional device int32 ``[1]`` (``new_history_nnz_npu``): only that many tokens are there, the rows
+    behind them are neither appended nor written to the result - for static buffers under a captured graph.  ``out``: where the
+    queries go (may be ``q``).  A token whose position or page does not exist is left out and reported by
+    ``_lib.check_status``."""
+    cache = _cache(kv_cache, page_size)
+    Hkv, D = cache.shape[3], cache.shape[4]
+    dev, n = cache.device, q.shape[0]
+    if D % 16:
+        raise ValueError("head_dim must be a multiple of 16, got %d" % D)
+    q, k, v = _rows("q", q, None, D, cache), _rows("k", k, Hkv, D, cache), _rows("v", v, Hkv, D, cache)
+    if k.shape[0] != n or v.shape[0] != n:
+        raise ValueError("q, k and v must hold the same tokens, got %d, %d and %d" % (n, k.shape[0], v.shape[0]))
+    if table.dim() != 2 or table.dtype != torch.float32 or table.device != dev or not table.is_contiguous() \
+            or table.shape[1] % 16 or not 0 < table.shape[1] <= D or (table.is_cuda and table.data_ptr() % 16):
+        raise ValueError("table must be a contiguous fp32 [max_positions, rotary_dim] on %s with rotary_dim a multiple of 16 and "
+                         "at most %d, got %s %s on %s" % (dev, D, table.dtype, tuple(table.shape), table.device))
+    batch_indices, positions = _ints("batch_indices", batch_indices, dev, n), _ints("positions", positions, dev, n)
+    page_ids, page_indptr = _ints("page_ids", page_ids, dev), _ints("page_indptr", page_indptr, dev)
+    if num_tokens is not None:
+        num_tokens = _ints("num_tokens", num_tokens, dev, 1)
+    if page_indptr.numel() < 1:
+        raise ValueError("page_indptr must be [requests + 1]")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or (out.numel() and (
+            out.stride(2) != 1 or out.stride(1) != D or out.stride(0) % 8 or out.stride(0) < out.shape[1] * D or out.data_ptr() % 16)):
+        raise ValueError("out must be %s %s on %s with adjacent heads and 16-byte aligned rows" % (tuple(q.shape), q.dtype, dev))
+    if n == 0:
+        return out
+    if not cache.is_cuda:
+        m = n if num_tokens is None else min(n, int(num_tokens))
+        pos, b = positions[:m].long(), batch_indices[:m].long()
+        cos, sin = table[pos][:, None, :].chunk(2, dim=-1)
+        at = page_ids.long()[page_indptr.long()[b] + pos // page_size]
+        out[:m] = _rotate_ref(q[:m], cos, sin, interleaved)
+        cache[at, 0, pos % page_size] = _rotate_ref(k[:m], cos, sin, interleaved)
+        cache[at, 1, pos % page_size] = v[:m]
+        return out
+    with _lib.on_device(dev):
+        rc = _lib.lib().rb_kv_append_rotary(
+            q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0),
+            cache.data_ptr(), batch_indices.data_ptr(), positions.data_ptr(), page_ids.data_ptr(), page_indptr.data_ptr(),
+            _lib.ptr(num_tokens), n, q.shape[1], Hkv, D, page_indptr.numel() - 1, page_size, page_ids.numel(), cache.shape[0],
+            table.data_ptr(), table.shape[0], table.shape[1], int(interleaved), int(q.dtype == torch.bfloat16), _lib.num_sms(dev),
+            _lib.status_tensor(dev).data_ptr(), _lib.stream_ptr(dev))
+        _lib.check(rc, "rb_kv_append_rotary")
+    return out
+
+
+# ----------------------------------------------------------------------------- attention
+def _attention_ref(q, keys, values, sees, scale: float):
+    """q [n, H, D], keys / values [m, Hkv, D], sees [n, m] -> (o [n, H, D], lse [n, H]); rows that see nothing: 0, -inf."""
+    n, H, D = q.shape
+    G = H // keys.shape[1]
+    x = torch.einsum("nhgd,mhd->hgnm", q.view(n, -1, G, D), keys) * scale
+    x = x.masked_fill(~sees, -math.inf)
+    lse = torch.logsumexp(x, dim=-1)
+    p = torch.exp(x - lse.masked_fill(lse == -math.inf, 0.0).unsqueeze(-1))
+    seen = sees.any(dim=0)                                              # what nobody sees may be anything
+    o = torch.einsum("hgnm,mhd->nhgd", p, values.masked_fill(~seen[:, None, None], 0.0))
+    return o.reshape(n, H, D), lse.permute(2, 0, 1).reshape(n, H)
+
+
+def softmax_attention_ref(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size: int, scale: Optional[float] = None,
+                          window: int = 0, num_sinks: int = 0, prefix_offsets=None, prefix_page_ids=None, prefix_page_indptr=None,
+                          group_offsets=None, dtype: torch.dtype = torch.float32):
+    """``(o [T, H, D] in dtype, lse [T, H])`` of the two attention operators, request by request in ``dtype``."""
+    H, D = q.shape[1], q.shape[2]
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    qo, ko, ip = q_offsets.tolist(), k_offsets.tolist(), page_indptr.tolist()
+    group = None
+    if prefix_offsets is not None:
+        po, pp = prefix_offsets.tolist(), prefix_page_indptr.tolist()
+        go = [0, len(qo) - 1] if group_offsets is None else group_offsets.tolist()
+        group = {b: g for g in range(len(go) - 1) for b in range(go[g], go[g + 1])}
+
+    def fetch(ids, n):
+        c = kv_cache[ids.long()]
+        return [c[:, i].reshape(-1, c.shape[3], D)[:n].to(dtype) for i in (0, 1)]
+
+    out = torch.zeros(q.shape[0], H, D, dtype=dtype, device=q.device)
+    lse = torch.full((q.shape[0], H), -math.inf, dtype=dtype, device=q.device)
+    for b in range(len(qo) - 1):
+        n, m = qo[b + 1] - qo[b], ko[b + 1] - ko[b]
+        if n == 0:
+            continue
+        k, v = fetch(page_ids[ip[b]:ip[b + 1]], m)
+        i = torch.arange(m - n, m, device=q.device)[:, None]
+        j = torch.arange(m, device=q.device)[None, :]
+        sees = j <= i
+        if window > 0:
+            sees = sees & ((j > i - window) | (j < num_sinks))
+        if group is not None and b in group:
+            g = group[b]
+            kp, vp = fetch(prefix_page_ids[pp[g]:pp[g + 1]], po[g + 1] - po[g])
+            k, v = torch.cat([kp, k]), torch.cat([vp, v])
+            sees = torch.cat([torch.ones(n, kp.shape[0], dtype=torch.bool, device=q.device), sees], dim=1)
+        if k.shape[0]:
+            out[qo[b]:qo[b + 1]], lse[qo[b]:qo[b + 1]] = _attention_ref(q[qo[b]:qo[b + 1]].to(dtype), k, v, sees, scale)
+    return out, lse
+
+
+def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks, return_lse, prefix=None):
+    cache = _cache(kv_cache, page_size, _HEAD_DIMS)
+    Hkv, D = cache.shape[3], cache.shape[4]
+    dev = cache.device
+    q = _rows("q", q, None, D, cache)
+    T, H = q.shape[0], q.shape[1]
+    if H == 0 or H % Hkv:
+        raise ValueError("%d query heads cannot share %d key heads" % (H, Hkv))
+    B = q_offsets.numel() - 1
+    if B < 0:
+        raise ValueError("q_offsets must be [requests + 1]")
+    q_offsets, k_offsets = _ints("q_offsets", q_offsets, dev), _ints("k_offsets", k_offsets, dev, B + 1)
+    page_ids, page_indptr = _ints("page_ids", page_ids, dev), _ints("page_indptr", page_indptr, dev, B + 1)
+    if window < 0 or num_sinks < 0:
+        raise ValueError("window and num_sinks must not be negative")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    groups, g_off, p_off, p_ids, p_ptr = 0, None, None, None, None
+    if prefix is not None:
+        g_off, p_off, p_ids, p_ptr = prefix
+        groups = p_off.numel() - 1
+        if groups < 0 or (g_off is None and groups != 1):
+            raise ValueError("prefix_offsets must be [groups + 1], and [2] without group_offsets")
+        p_off, p_ids = _ints("prefix_offsets", p_off, dev), _ints("prefix_page_ids", p_ids, dev)
+        p_ptr = _ints("prefix_page_indptr", p_ptr, dev, groups + 1)
+        if g_off is not None:
+            g_off = _ints("group_offsets", g_off, dev, groups + 1)
+    if not cache.is_cuda:
+        o, lse = softmax_attention_ref(q, cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks,
+                                       p_off, p_ids, p_ptr, g_off)
+        return (o.to(q.dtype), lse) if return_lse else o.to(q.dtype)
+    if page_size % 16:
+        raise ValueError("page_size must be a multiple of 16, got %d" % page_size)
+    with _lib.on_device(dev):
+        out = torch.empty(T, H, D, dtype=q.dtype, device=dev)
+        lse = torch.empty(T, H, dtype=torch.float32, device=dev) if return_lse else None
+        if T and B == 0:
+            raise ValueError("q holds %d tokens but there are no requests" % T)
+        if T:
+            if g_off is None and groups:
+                g_off = _one_group(B, dev)
+            lib, sms = _lib.lib(), _lib.num_sms(dev)
+            nbytes = lib.rb_softmax_attn_workspace(sms, T, H, D, groups)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            rc = lib.rb_softmax_attn_paged(
+                q.data_ptr(), q.stride(0), T, H, Hkv, D, cache.data_ptr(), cache.shape[0], page_size, q_offsets.data_ptr(),
+                k_offsets.data_ptr(), page_ids.data_ptr(), page_indptr.data_ptr(), page_ids.numel(), B, _lib.ptr(g_off),
+                _lib.ptr(p_off), _lib.ptr(p_ids), _lib.ptr(p_ptr), p_ids.numel() if groups else 0, groups,
+                min(int(window), 1 << 30), min(int(num_sinks), 1 << 30), scale, int(q.dtype == torch.bfloat16), out.data_ptr(),
+                out.stride(0), _lib.ptr(lse), ws.data_ptr(), nbytes, sms, _lib.status_tensor(dev).data_ptr(), _lib.stream_ptr(dev))
+            _lib.check(rc, "rb_softmax_attn_paged")
+    return (out, lse) if return_lse else out
+
+
+def _one_group(requests: int, device) -> torch.Tensor:
+    t = torch.zeros(2, dtype=torch.int32, device=device)
+    t[1:].fill_(requests)
+    return t
+
+
+def softmax_attention_paged(q: torch.Tensor, kv_cache: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor,
+                            page_ids: torch.Tensor, page_indptr: torch.Tensor, page_size: int, scale: Optional[float] = None,
+                            window: int = 0, num_sinks: int = 0, return_lse: bool = False):
+    """Causal softmax attention of the new tokens (``q [T, heads, head_dim]``, jagged by ``q_offsets``) over the paged cache.
+
+    Request ``b`` has ``k_offsets[b + 1] - k_offsets[b]`` keys in the pages ``page_ids[page_indptr[b]:page_indptr[b + 1]]``,
+    the last of which are its new tokens' own (already appended); its ``i``-th query sits at the position of the ``i``-th of
+    them.  A query sees the keys up to its position - with ``window > 0`` only the last ``window`` of them (itself
+    included) and the first ``num_sinks`` tokens.  Pages that lie wholly before the window and after the sinks are not
+    read and may be gone.  ``heads`` is a multiple of the cache's ``kv_heads``; query head ``h`` reads key head
+    ``h // (heads / kv_heads)``.  ``scale`` defaults to ``head_dim ** -0.5``.
+
+    Returns ``[T, heads, head_dim]`` (and, ``return_lse``, fp32 ``[T, heads]``: log of the sum of the exponentials).  A
+    query that sees no key gives 0 and ``-inf``; rows of ``q`` behind the last request are undefined in the result.  bf16 or
+    fp16, head_dim 64 or 128, page_size a multiple of 16.  Stale values in slots that a block of queries does not see do no
+    harm; a non-finite VALUE that one query sees can spread to neighbouring queries of the same request that do not.  A
+    missing page reads as zeros and is reported by ``_lib.check_status``."""
+    return _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks, return_lse)
+
+
+def softmax_attention_shared_prefix(q: torch.Tensor, kv_cache: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor,
+                                    page_ids: torch.Tensor, page_indptr: torch.Tensor, prefix_offsets: torch.Tensor,
+                                    prefix_page_ids: torch.Tensor, prefix_page_indptr: torch.Tensor, page_size: int,
+                                    group_offsets: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                                    return_lse: bool = False):
+    """:func:`softmax_attention_paged` for requests that share what stands before their own keys.
+
+    Group ``g`` is the requests ``group_offsets[g]:group_offsets[g + 1]`` (without ``group_offsets``: one group of all);
+    all of its queries see the ``prefix_offsets[g + 1] - prefix_offsets[g]`` keys of the pages
+    ``prefix_page_ids[prefix_page_indptr[g]:prefix_page_indptr[g + 1]]``, then - causally - their request's own keys, which
+    ``k_offsets``, ``page_ids`` and ``page_indptr`` describe without the prefix (a request need not have any).  The result is that of one
+    attention over prefix and own keys together; the prefix is read once for the group instead of once per request."""
+    return _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, 0, 0, return_lse,
+                   (group_offsets, prefix_offsets, prefix_page_ids, prefix_page_indptr))

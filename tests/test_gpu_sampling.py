@@ -1,0 +1,121 @@
+"""``sample_scores`` on the GPU against its row-by-row statement in 64 bits: the items are the same, always."""
+import math
+
+import pytest
+import torch
+
+from recsdk_b200.ops import sampling as S
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+
+def _same(scores, u, offsets=None, **kw):
+    ids, lp = S.sample_scores(scores, u, offsets, **kw)
+    want, want_lp = S.sample_scores_ref(scores, u, offsets, **kw)
+    assert ids.dtype == torch.int64 and lp.dtype == torch.float32
+    assert torch.equal(ids, want), (ids - want).nonzero().flatten().tolist()
+    some = want >= 0
+    assert (lp[~some] == -math.inf).all()
+    # both are fp32 roundings (half a step, 2^-24) of 64-bit values that agree to far more digits
+    assert ((lp - want_lp)[some].abs() <= 2.0 ** -23 * want_lp[some].abs() + 1e-11).all()
+
+
+FILTERS = [dict(), dict(top_k=1), dict(top_k=7), dict(top_k=10 ** 6), dict(top_p=0.3), dict(top_p=0.95), dict(min_p=0.05), dict(min_p=1.0),
+           dict(temperature=0.0), dict(temperature=0.3, top_k=50, top_p=0.9), dict(temperature=2.5, top_k=300, top_p=0.5, min_p=0.01),
+           dict(top_p=1e-6)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("width", [1, 2, 31, 33, 511, 4099, 50021])
+def test_dense(dtype, width):
+    g = torch.Generator(device=DEV).manual_seed(width)
+    rows = 24 if width < 10000 else 6
+    x = (torch.randn(rows, width, generator=g, device=DEV) * 2.5).to(dtype)
+    for kw in FILTERS:
+        _same(x, torch.rand(rows, generator=g, device=DEV), **kw)
+
+
+@pytest.mark.parametrize("off", [torch.int32, torch.int64])
+def test_jagged(off):
+    g = torch.Generator(device=DEV).manual_seed(3)
+    lens = [0, 1, 5, 0, 1000, 33, 4096, 2, 0]
+    x = torch.randn(sum(lens), generator=g, device=DEV)
+    o = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=off, device=DEV)
+    for kw in FILTERS:
+        _same(x, torch.rand(len(lens), generator=g, device=DEV), o, **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_ties(dtype):
+    """Many equal scores: the cut goes through them by index."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randint(-3, 3, (16, 777), generator=g, device=DEV).to(dtype) * 0.5
+    x[1] = 1.0
+    x[2] = -0.0
+    x[2, ::2] = 0.0
+    for kw in FILTERS + [dict(top_k=100, top_p=0.5), dict(top_p=0.5)]:
+        _same(x, torch.rand(16, generator=g, device=DEV), **kw)
+
+
+def test_infinities_and_nan():
+    inf = math.inf
+    rows = [[-inf] * 5, [math.nan] * 5, [inf, 1.0, inf, -inf, math.nan], [-inf, math.nan, 2.0, -inf, -inf], [3e38, -3e38, 3e38, 0, 0],
+            [-3.4e38, -inf, -3.4e38, math.nan, -3.4e38], [0.0, -0.0, 0.0, -0.0, -inf]]
+    x = torch.tensor(rows, device=DEV)
+    for uv in (0.0, 0.4, 0.999999):
+        for kw in (dict(), dict(top_k=2), dict(top_p=0.4), dict(min_p=0.5), dict(temperature=0.0), dict(temperature=1e-30)):
+            _same(x, torch.full((len(rows),), uv, device=DEV), **kw)
+    _same(x.half(), torch.full((len(rows),), 0.7, device=DEV))
+
+
+def test_border_uniforms_and_equal_weights():
+    x = torch.zeros(8, 1000, device=DEV)
+    u = torch.tensor([0.0, 0.001, 0.5, 0.25, 0.75, 1.0 - 2.0 ** -24, 1.0, 0.125], device=DEV)
+    for kw in (dict(), dict(top_k=8), dict(top_k=512, top_p=0.5), dict(top_p=0.25)):
+        _same(x, u, **kw)
+    ids, lp = S.sample_scores(x, u, top_k=8)
+    assert ids.tolist() == [0, 0, 4, 2, 6, 7, 7, 1] and torch.allclose(lp, torch.full_like(lp, -math.log(8)))
+
+
+def test_parameters_per_row():
+    g = torch.Generator(device=DEV).manual_seed(6)
+    x = torch.randn(12, 3001, generator=g, device=DEV)
+    u = torch.rand(12, generator=g, device=DEV)
+    t = torch.tensor([0.0, 1, 0.5, 2, -1, 1, 1, 1, 0.2, 1, 3, 1], device=DEV)
+    k = torch.tensor([0, 1, 5, 0, 3, -4, 10 ** 6, 100, 7, 0, 2, 3000], device=DEV)
+    p = torch.tensor([1, 0.5, 2, 0.9, 0.1, 0.99, 0.7, 1, 0.0, -1, 0.5, 0.3], device=DEV)
+    m = torch.tensor([0, 0, 0, 0.1, 0, 0.5, 0, 1, 2, 0, 0, 0.01], device=DEV)
+    _same(x, u, temperature=t, top_k=k, top_p=p, min_p=m)
+    _same(x, u, temperature=0.7, top_k=k.int(), top_p=0.8, min_p=m)
+
+
+def test_strides_streams_and_graph():
+    g = torch.Generator(device=DEV).manual_seed(7)
+    big = torch.randn(10, 4000, generator=g, device=DEV)
+    u = torch.rand(10, generator=g, device=DEV)
+    for x in (big[:, 3:2000], big[::2, :777], big.t()[:10, ::3][:, :3]):
+        _same(x, u[: x.shape[0]], top_k=20, top_p=0.9)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ids, _ = S.sample_scores(big, u, top_p=0.9)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gids, glp = S.sample_scores(big, u, top_p=0.9)
+    graph.replay()
+    assert torch.equal(gids, ids)
+    u.copy_(torch.rand(10, generator=g, device=DEV))
+    graph.replay()
+    assert torch.equal(gids, S.sample_scores(big, u, top_p=0.9)[0])
+
+
+def test_the_draws_follow_the_distribution():
+    """Evenly spaced uniforms: every item comes exactly as often as its share says, to within one draw at each border."""
+    x = torch.randn(300, generator=torch.Generator().manual_seed(8))
+    n = 20000
+    u = ((torch.arange(n) + 0.5) / n).to(DEV)
+    ids, _ = S.sample_scores(x.to(DEV).expand(n, 300), u, temperature=0.8)
+    want = torch.softmax(x.double() / torch.tensor(0.8, dtype=torch.float32).double(), 0) * n
+    assert ((torch.bincount(ids.cpu(), minlength=300) - want).abs() <= 1.01).all()
