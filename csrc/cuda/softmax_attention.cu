@@ -34,15 +34,6 @@ template <int D> struct Cfg {
   static constexpr int SMEM = RING + 1024 + 2048;
 };
 
-struct Meta { int valid, seq, qt, h, c0, c1, n, pad; long long t0, total; };
-
-struct Outs {
-  void* out; long long ld_o; float* lse;   // final results: 16-bit rows [Tq][ld_o], lse [Tq][H] or null
-  float* part_o; float* part_lse;          // when not null: fp32 [2][Tq][H][D] and log2 [2][Tq][H] instead, by Seq::part
-  float* cut_o; float* cut_lse;            // [CTAs][2][RT][D], [CTAs][2][RT]: items cut by a share's border
-  Meta* meta;                              // [CTAs]
-};
-
 struct Items { int qt, units; };           // row tiles of a sequence, units of keys of each
 
 template <int D>
@@ -62,8 +53,6 @@ __device__ __forceinline__ Items items_of(const Batch& p, const Seq& s) {
   return r;
 }
 
-__device__ __forceinline__ long long share(int c, int n, long long total) { return total * c / n; }
-
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (BF16)
@@ -78,27 +67,6 @@ __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t& a, uint32_t& b, u
 }
 __device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
-}
-
-// one finished row (or a third of it): o normalised, lse in log2
-template <int D, bool BF16, int N>
-__device__ __forceinline__ void write_row(const Batch& p, const Outs& w, const Seq& s, int row, int h, int col, const float (&o)[N],
-                                          float lse2) {
-  const long long t = s.q_begin + row / p.G;
-  const int head = h * p.G + row % p.G;
-  if (w.part_o) {
-    const long long at = (static_cast<long long>(s.part) * p.Tq + t) * p.H + head;
-    float* dst = w.part_o + at * D + col;
-#pragma unroll
-    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-    if (col == 0) w.part_lse[at] = lse2;
-  } else {
-    uint16_t* dst = reinterpret_cast<uint16_t*>(w.out) + t * w.ld_o + static_cast<long long>(head) * D + col;
-#pragma unroll
-    for (int i = 0; i < N; i += 4)
-      *reinterpret_cast<uint2*>(dst + i) = make_uint2(pack16<BF16>(o[i], o[i + 1]), pack16<BF16>(o[i + 2], o[i + 3]));
-    if (col == 0 && w.lse) w.lse[t * p.H + head] = lse2 * LN2;
-  }
 }
 
 template <int D, bool BF16>
@@ -177,7 +145,7 @@ __global__ void __launch_bounds__(NW * 32) attn_rows_kernel(const __grid_constan
       const long long t0 = pos - off;
       if (pos == p0 && off > 0 && share(cta - 1, n_sh, total) <= t0) {
         // the first border inside this item: the second kernel joins its pieces
-        m.valid = 1; m.seq = b; m.qt = qt; m.h = h; m.t0 = t0; m.total = total; m.n = n_sh;
+        m.valid = 1; m.seq = b; m.row0 = qt * RT; m.rows = rows; m.h = h; m.t0 = t0; m.total = total; m.n = n_sh;
         m.c0 = cta - 1;
         m.c1 = static_cast<int>(((t0 + it.units) * n_sh - 1) / total);        // the share that holds the item's last unit
       }
@@ -377,19 +345,18 @@ __global__ void __launch_bounds__(NW * 32) attn_rows_kernel(const __grid_constan
   if (tid == 0) w.meta[cta] = m;
 }
 
-// Joins the pieces of the items that borders cut: CTA c looks after the item whose first border is share c's begin.
+// Joins the pieces of the items that borders cut: block (c, y) looks after 16 rows of the item whose first border is share
+// c's begin.  Items have up to `block_rows` rows.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(128) attn_join_kernel(const Batch p, const Outs w) {
+__global__ void __launch_bounds__(128) attn_join_kernel(const Batch p, const Outs w, int block_rows) {
   const Meta m = w.meta[blockIdx.x];
-  if (!m.valid) return;
-  const Seq s = seq_of(p, m.seq);
-  const int rows = min(s.len_q * p.G - m.qt * RT, RT);
   constexpr int TPR = 128 / RT, N = 4;
-  const int r = threadIdx.x / TPR;
-  if (r >= rows) return;
+  const int r = blockIdx.y * RT + threadIdx.x / TPR;
+  if (!m.valid || r >= m.rows) return;
+  const Seq s = seq_of(p, m.seq);
   auto cut = [&](int c) {
     const long long b = share(c, m.n, m.total);
-    return (static_cast<long long>(c) * 2 + (b >= m.t0 ? 0 : 1)) * RT + r;
+    return (static_cast<long long>(c) * 2 + (b >= m.t0 ? 0 : 1)) * block_rows + r;
   };
   float mm = -INFINITY;
   for (int c = m.c0; c <= m.c1; ++c) mm = fmaxf(mm, w.cut_lse[cut(c)]);
@@ -415,7 +382,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const Batch p, const Out
   for (int k = 0; k < D / (TPR * N); ++k) {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[k][i] *= inv;
-    write_row<D, BF16, N>(p, w, s, m.qt * RT + r, m.h, (threadIdx.x % TPR) * N + k * TPR * N, x[k], lse2);
+    write_row<D, BF16, N>(p, w, s, m.row0 + r, m.h, (threadIdx.x % TPR) * N + k * TPR * N, x[k], lse2);
   }
 }
 
@@ -448,26 +415,74 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const Batch p, const Ou
 
 constexpr long long align256(long long n) { return (n + 255) / 256 * 256; }
 
-struct Space { long long cut_o, cut_lse, meta, part_o, part_lse, total; };
+// Workspace: the pieces of the rows kernel, those of the tiles kernel, the two parts of rows behind a prefix.
+struct Space { long long cut_o[2], cut_lse[2], meta[2], part_o, part_lse, total; };
 
-Space space_of(int n_cta, int D, long long rows, bool parts) {
+Space space_of(int n_cta, int D, long long rows, bool with_rows, bool with_tiles, bool parts) {
   Space s;
-  s.cut_o = 0;
-  s.cut_lse = align256(s.cut_o + static_cast<long long>(n_cta) * 2 * RT * D * 4);
-  s.meta = align256(s.cut_lse + static_cast<long long>(n_cta) * 2 * RT * 4);
-  s.part_o = align256(s.meta + static_cast<long long>(n_cta) * static_cast<long long>(sizeof(Meta)));
-  s.part_lse = align256(s.part_o + (parts ? 2 * rows * D * 4 : 0));
-  s.total = align256(s.part_lse + (parts ? 2 * rows * 4 : 0));
+  long long at = 0;
+  auto take = [&](long long bytes) { const long long was = at; at = align256(at + bytes); return was; };
+  for (int k = 0; k < 2; ++k) {
+    const long long n = (k ? with_tiles : with_rows) ? static_cast<long long>(n_cta) : 0, block = k ? TILE_ROWS : RT;
+    s.cut_o[k] = take(n * 2 * block * D * 4);
+    s.cut_lse[k] = take(n * 2 * block * 4);
+    s.meta[k] = take(n * static_cast<long long>(sizeof(Meta)));
+  }
+  s.part_o = take(parts ? 2 * rows * D * 4 : 0);
+  s.part_lse = take(parts ? 2 * rows * 4 : 0);
+  s.total = at;
   return s;
 }
 
+// Which kernel a list of sequences takes, by the average number of rows that share a key head: the rows kernel reads
+// K and V once for 16 of them, the tiles kernel once for 256 with at least 128 computed.
+bool by_tiles(long long Tq, int G, int sequences, float scale) {
+  return G <= 128 && scale > 0.f && sequences > 0 && Tq * G >= 48LL * sequences;
+}
+
+struct Plan { bool tiles_a, tiles_b; };
+
+Plan plan_of(long long Tq, int G, int B, int groups, float scale) {
+  const bool own = by_tiles(Tq, G, B, scale);
+  Plan r;
+  r.tiles_a = groups > 0 ? by_tiles(Tq, G, groups, scale) : own;
+  r.tiles_b = groups > 0 && own;
+  return r;
+}
+
 template <int D, bool BF16>
-int launch(const CUtensorMap& tm, const Batch& p, Outs w, int n_cta, bool parts, cudaStream_t st) {
-  RB_CUDA_CHECK(cudaFuncSetAttribute(attn_rows_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM));
-  attn_rows_kernel<D, BF16><<<n_cta, NW * 32, Cfg<D>::SMEM, st>>>(tm, p, w);
-  RB_CUDA_CHECK(cudaGetLastError());
-  attn_join_kernel<D, BF16><<<n_cta, 128, 0, st>>>(p, w);
-  RB_CUDA_CHECK(cudaGetLastError());
+int join(const Batch& p, const Outs& w, int n_cta, int block_rows, cudaStream_t st) {
+  attn_join_kernel<D, BF16><<<dim3(n_cta, block_rows / RT), 128, 0, st>>>(p, w, block_rows);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <int D, bool BF16>
+int launch(const Batch& p, Outs w, const Plan& plan, const Space& sp, char* ws, const void* cache, int n_cta, cudaStream_t st) {
+  const bool parts = p.b.B > 0;
+  for (int tiles = 0; tiles < 2; ++tiles) {
+    Batch q = p;
+    if (plan.tiles_a != (tiles != 0)) q.a.B = 0;
+    if (plan.tiles_b != (tiles != 0)) q.b.B = 0;
+    if (q.a.B + q.b.B == 0) continue;
+    w.cut_o = reinterpret_cast<float*>(ws + sp.cut_o[tiles]);
+    w.cut_lse = reinterpret_cast<float*>(ws + sp.cut_lse[tiles]);
+    w.meta = reinterpret_cast<Meta*>(ws + sp.meta[tiles]);
+    if (tiles) {
+      const int rc = launch_tiles(q, w, cache, D, BF16, n_cta, st);
+      if (rc) return rc;
+    } else {
+      CUtensorMap tm;
+      q.box_rows = p.page_size % KT == 0 ? KT : 16;
+      const int rc = rb_host::make_map_2d(&tm, cache, p.total_rows, static_cast<long long>(p.Hkv) * D, static_cast<long long>(p.Hkv) * D,
+                                          64, q.box_rows, BF16);
+      if (rc) return rc;
+      RB_CUDA_CHECK(cudaFuncSetAttribute(attn_rows_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM));
+      attn_rows_kernel<D, BF16><<<n_cta, NW * 32, Cfg<D>::SMEM, st>>>(tm, q, w);
+      RB_CUDA_CHECK(cudaGetLastError());
+    }
+    const int rc = join<D, BF16>(q, w, n_cta, tiles ? TILE_ROWS : RT, st);
+    if (rc) return rc;
+  }
   if (parts) {
     const long long rows = static_cast<long long>(p.Tq) * p.H;
     const int per = 256 / (D / 4);
@@ -480,8 +495,11 @@ int launch(const CUtensorMap& tm, const Batch& p, Outs w, int n_cta, bool parts,
 }  // namespace
 
 // Bytes of workspace that rb_softmax_attn_paged needs.
-RB_API long long rb_softmax_attn_workspace(int num_sms, long long Tq, int H, int D, int prefix) {
-  return space_of(num_sms > 0 ? num_sms : 148, D, Tq * H, prefix != 0).total;
+RB_API long long rb_softmax_attn_workspace(int num_sms, long long Tq, int H, int Hkv, int D, int B, int groups, float scale) {
+  if (Hkv <= 0 || H % Hkv) return 0;
+  const Plan plan = plan_of(Tq, H / Hkv, B, groups, scale);
+  return space_of(num_sms > 0 ? num_sms : 148, D, Tq * H, !plan.tiles_a || (groups > 0 && !plan.tiles_b), plan.tiles_a || plan.tiles_b,
+                  groups > 0).total;
 }
 
 // q [Tq][H][D] (token stride ld_q), cache [num_pages][2][page_size][Hkv][D], bf16 or fp16; int32 offsets and page tables on
@@ -503,7 +521,8 @@ RB_API int rb_softmax_attn_paged(const void* q, long long ld_q, long long Tq, in
   const long long rows = num_pages * 2 * page_size;
   if (Tq * H > 0x7fffffffLL || rows + page_size > 0x7fffffffLL) return -4;
   const int n_cta = num_sms > 0 ? num_sms : 148;
-  const Space sp = space_of(n_cta, D, Tq * H, groups > 0);
+  const Plan plan = plan_of(Tq, H / Hkv, B, groups, scale);
+  const Space sp = space_of(n_cta, D, Tq * H, !plan.tiles_a || (groups > 0 && !plan.tiles_b), plan.tiles_a || plan.tiles_b, groups > 0);
   if (workspace_bytes < sp.total) return -5;
   Batch p;
   const Seqs own = {q_offsets, nullptr, k_offsets, page_ids, page_indptr, num_page_ids, B, B, 1};
@@ -512,20 +531,13 @@ RB_API int rb_softmax_attn_paged(const void* q, long long ld_q, long long Tq, in
   p.a = groups > 0 ? pre : own;
   p.b = groups > 0 ? own : none;
   p.q = q; p.ld_q = ld_q; p.Tq = static_cast<int>(Tq); p.H = H; p.Hkv = Hkv; p.G = H / Hkv; p.page_size = page_size;
-  p.box_rows = page_size % KT == 0 ? KT : 16; p.total_rows = static_cast<int>(rows); p.window = window; p.sinks = sinks;
+  p.box_rows = 16; p.total_rows = static_cast<int>(rows); p.window = window; p.sinks = sinks;
   p.scale_log2 = scale * LOG2E; p.status = status;
   char* ws = static_cast<char*>(workspace);
   Outs w;
   w.out = out; w.ld_o = ld_o; w.lse = lse;
   w.part_o = groups > 0 ? reinterpret_cast<float*>(ws + sp.part_o) : nullptr;
   w.part_lse = reinterpret_cast<float*>(ws + sp.part_lse);
-  w.cut_o = reinterpret_cast<float*>(ws + sp.cut_o);
-  w.cut_lse = reinterpret_cast<float*>(ws + sp.cut_lse);
-  w.meta = reinterpret_cast<Meta*>(ws + sp.meta);
-  CUtensorMap tm;
-  const int rc = rb_host::make_map_2d(&tm, cache, rows, static_cast<long long>(Hkv) * D, static_cast<long long>(Hkv) * D, 64,
-                                      p.box_rows, is_bf16 != 0);
-  if (rc) return rc;
-  if (D == 64) return is_bf16 ? launch<64, true>(tm, p, w, n_cta, groups > 0, st) : launch<64, false>(tm, p, w, n_cta, groups > 0, st);
-  return is_bf16 ? launch<128, true>(tm, p, w, n_cta, groups > 0, st) : launch<128, false>(tm, p, w, n_cta, groups > 0, st);
+  if (D == 64) return is_bf16 ? launch<64, true>(p, w, plan, sp, ws, cache, n_cta, st) : launch<64, false>(p, w, plan, sp, ws, cache, n_cta, st);
+  return is_bf16 ? launch<128, true>(p, w, plan, sp, ws, cache, n_cta, st) : launch<128, false>(p, w, plan, sp, ws, cache, n_cta, st);
 }

@@ -67,7 +67,7 @@ struct Span {
   int hi;                     // keys at or past it are seen by no row of the block
   int lo;                     // keys before it are seen by no row, unless they are sinks
   int sinks;
-  int sink_tiles, first, tiles;   // tile v is v < sink_tiles ? v : first + v - sink_tiles
+  int sink_tiles, first, end, tiles;   // tile v is v < sink_tiles ? v : first + v - sink_tiles
   __device__ __forceinline__ int tile(int v) const { return v < sink_tiles ? v : first + v - sink_tiles; }
 };
 
@@ -81,10 +81,10 @@ __device__ __forceinline__ Span span_of(const Batch& p, const Seq& s, int t_lo, 
   const bool win = s.causal && p.window > 0;
   r.lo = win ? max(r.p_min - p.window + 1, 0) : 0;
   r.sinks = win ? min(p.sinks, r.hi) : 0;
-  const int end = (r.hi + T - 1) / T;
+  r.end = (r.hi + T - 1) / T;
   r.first = r.lo / T;
   r.sink_tiles = min((r.sinks + T - 1) / T, r.first);
-  r.tiles = r.sink_tiles + max(end - r.first, 0);
+  r.tiles = r.sink_tiles + max(r.end - r.first, 0);
   return r;
 }
 
@@ -115,5 +115,53 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// The keys of all items (sequence, block of rows, key head) are laid end to end in units and cut into as many equal shares as
+// there are CTAs; none is empty.  Share c begins at share(c).
+__device__ __forceinline__ long long share(int c, int n, long long total) { return total * c / n; }
+
+// Rows [row0, row0 + rows) of a sequence (packed: token * G + head of the group) whose units shares c0..c1 hold; left by
+// the share c0 + 1 for the kernel that joins the pieces.
+struct Meta { int valid, seq, row0, rows, h, c0, c1, n; long long t0, total; };
+
+struct Outs {
+  void* out; long long ld_o; float* lse;   // final results: 16-bit rows [Tq][ld_o], lse [Tq][H] or null
+  float* part_o; float* part_lse;          // when not null: fp32 [2][Tq][H][D] and log2 [2][Tq][H] instead, by Seq::part
+  float* cut_o; float* cut_lse;            // [shares][2][rows of a block][D], [shares][2][rows]: pieces of items cut by a border
+  Meta* meta;                              // [shares]
+};
+
+// N consecutive elements of one finished row: o normalised, lse in log2
+template <int D, bool BF16, int N>
+__device__ __forceinline__ void write_row(const Batch& p, const Outs& w, const Seq& s, int row, int h, int col, const float (&o)[N],
+                                          float lse2) {
+  const long long t = s.q_begin + row / p.G;
+  const int head = h * p.G + row % p.G;
+  if (w.part_o) {
+    const long long at = (static_cast<long long>(s.part) * p.Tq + t) * p.H + head;
+    float* dst = w.part_o + at * D + col;
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+    if (col == 0) w.part_lse[at] = lse2;
+  } else {
+    uint16_t* dst = reinterpret_cast<uint16_t*>(w.out) + t * w.ld_o + static_cast<long long>(head) * D + col;
+    if (N % 8 == 0) {
+#pragma unroll
+      for (int i = 0; i + 8 <= N; i += 8)
+        *reinterpret_cast<uint4*>(dst + i) = make_uint4(pack16<BF16>(o[i], o[i + 1]), pack16<BF16>(o[i + 2], o[i + 3]),
+                                                        pack16<BF16>(o[i + 4], o[i + 5]), pack16<BF16>(o[i + 6], o[i + 7]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i += 4)
+        *reinterpret_cast<uint2*>(dst + i) = make_uint2(pack16<BF16>(o[i], o[i + 1]), pack16<BF16>(o[i + 2], o[i + 3]));
+    }
+    if (col == 0 && w.lse) w.lse[t * p.H + head] = lse2 * LN2;
+  }
+}
+
+// softmax_attention_tiles.cu: the kernel for many rows per sequence; fills out / part and the cut pieces (blocks of
+// TILE_ROWS rows) of all sequences of p
+constexpr int TILE_ROWS = 256;
+int launch_tiles(const Batch& p, const Outs& w, const void* cache, int D, bool is_bf16, int n_cta, cudaStream_t st);
 
 }  // namespace rb_attn

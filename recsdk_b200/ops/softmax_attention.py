@@ -239,7 +239,7 @@ def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size,
             if g_off is None and groups:
                 g_off = _one_group(B, dev)
             lib, sms = _lib.lib(), _lib.num_sms(dev)
-            nbytes = lib.rb_softmax_attn_workspace(sms, T, H, D, groups)
+            nbytes = lib.rb_softmax_attn_workspace(sms, T, H, Hkv, D, B, groups, scale)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             rc = lib.rb_softmax_attn_paged(
                 q.data_ptr(), q.stride(0), T, H, Hkv, D, cache.data_ptr(), cache.shape[0], page_size, q_offsets.data_ptr(),
