@@ -8,8 +8,9 @@
 //   * 256 rows (two row tiles of 128: 128 / G tokens x the G query heads that share a key head) walk the same key tiles, or
 //   * where a block has 128 rows or fewer, one row tile takes even key tiles with one set of warps and odd ones with
 //     the other; the two results are joined from TMEM at the end.
-// Roles: one thread issues TMA loads (Q once per block, then K and V tiles of 128 keys through a ring, box by box through the page
-// table), one issues tcgen05.mma, one warp clears V of keys that nobody sees (0 x NaN), eight warps do the softmax, a
+// Roles: one warp issues TMA loads (Q once per block, then K and V tiles of 128 keys through a ring, box by box through the page
+// table), two warps issue tcgen05.mma, one for each row tile, and clear V of keys that nobody sees (0 x NaN), one thread
+// works the pieces of the share out ahead, eight warps do the softmax, a
 // thread per row: S from TMEM, maximum, exponentials, P back to TMEM over S as the A operand of O += P V.  O stays in TMEM
 // and is rescaled only when a row's maximum has grown by more than 2^8 since the value its weights refer to, which fp32
 // sums and 16-bit weights (a floating-point type: no precision lost) bear and which is rare after the first tiles.
@@ -22,24 +23,27 @@ namespace {
 
 using namespace rb_attn;
 
-constexpr int KT = 128;                 // keys per tile
+constexpr int KT = 64;                  // keys per tile
 constexpr int MT = 128;                 // rows per row tile
+// An item costs as much as FIXED units before its first key tile (measured: 4.4 us to finish one block and begin the next, 1.1
+// us a unit): without them the shares with many short items would run half as long again as the others.
+constexpr int FIXED = 4;
 constexpr int THREADS = 384;            // 4 service warps, 2 x 4 softmax warps
-constexpr int WAIT = 1 << 22;
+constexpr uint32_t WAIT = 1u << 24;     // tries of a wait: some tenths of a second
 
 template <int D> struct Cfg {
   static constexpr int CH = D / 64;
-  static constexpr int TILE = KT * D * 2;                       // bytes of a Q, K or V tile
-  static constexpr int STAGES = D == 64 ? 10 : 5;
+  static constexpr int TILE = KT * D * 2, Q_TILE = MT * D * 2;  // bytes of a K or V tile, of a Q tile
+  static constexpr int STAGES = D == 64 ? 8 : 5;                // a K and a V tile each
   static constexpr int TAIL = 3072;               // shared memory is full to the last byte for D = 128
-  static constexpr int SMEM = (2 + STAGES) * TILE + TAIL;
+  static constexpr int SMEM = 2 * Q_TILE + STAGES * 2 * TILE + TAIL;
 };
 
 // One block of query tokens of a sequence: [t_lo, t_lo + tokens)
 struct Block {
   int t_lo, tokens, two;                // two: a row tile each for the first and the rest of the tokens
   Span span;
-  int units;
+  int units;                            // FIXED for the block itself, then one or two key tiles each
 };
 
 __device__ __forceinline__ int blocks_of(const Seq& s, int tpt) { return (s.len_q + 2 * tpt - 1) / (2 * tpt); }
@@ -50,7 +54,7 @@ __device__ __forceinline__ Block block_of(const Batch& p, const Seq& s, int i, i
   b.tokens = min(s.len_q - b.t_lo, 2 * tpt);
   b.two = b.tokens > tpt;
   b.span = span_of<KT>(p, s, b.t_lo, b.t_lo + b.tokens - 1);
-  b.units = max(b.two ? b.span.tiles : (b.span.tiles + 1) / 2, 1);
+  b.units = max(b.two ? b.span.tiles : (b.span.tiles + 1) / 2, 1) + FIXED;
   return b;
 }
 
@@ -70,60 +74,47 @@ struct Walk {
       b = block_of(p, s, block, tpt);
       const long long all = static_cast<long long>(b.units) * p.Hkv;
       if (pos >= base + all) { base += all; ++block; continue; }
-      h = static_cast<int>((pos - base) / b.units);
-      u0 = static_cast<int>((pos - base) % b.units);
+      const uint32_t at = static_cast<uint32_t>(pos - base);                  // below units * Hkv: both are small numbers
+      h = static_cast<int>(at / b.units);
+      u0 = static_cast<int>(at - h * b.units);
       u1 = static_cast<int>(min(static_cast<long long>(b.units), u0 + (p1 - pos)));
+      if (u1 <= FIXED) { done(); continue; }                                  // the next share begins the item
       return true;
     }
     return false;
   }
   __device__ __forceinline__ void done() { pos += u1 - u0; }
   // virtual key tiles of the piece
-  __device__ __forceinline__ int v0() const { return b.two ? u0 : 2 * u0; }
-  __device__ __forceinline__ int v1() const { return min(b.two ? u1 : 2 * u1, b.span.tiles); }
+  __device__ __forceinline__ int v0() const { const int u = max(u0 - FIXED, 0); return b.two ? u : 2 * u; }
+  __device__ __forceinline__ int v1() const { return min((b.two ? 1 : 2) * (u1 - FIXED), b.span.tiles); }
 };
 
-// Where the tiles of a piece with n key tiles stand in the order of loads, which is the order of first use:
-// K0 V0 K1 V1 ... when both row tiles use every key tile, K0 K1 V0 K2 V1 ... when they take turns.
-__device__ __forceinline__ int k_index(bool two, int m) { return two ? 2 * m : m + max(m - 1, 0); }
-__device__ __forceinline__ int v_index(bool two, int m, int n) { return two ? 2 * m + 1 : m + min(n, m + 2); }
-
-// which key tiles row tile w of a block sees (the other's extra tiles at the ends are left out)
-struct Active {
-  int sink_end, first, end;
-  __device__ __forceinline__ bool operator()(int tile) const { return tile < sink_end || (tile >= first && tile < end); }
-};
-__device__ __forceinline__ Active active_of(const Batch& p, const Seq& s, const Block& b, int w, int tpt) {
-  Active a;
-  const int lo = b.two ? b.t_lo + w * tpt : b.t_lo;
-  const int hi = b.two ? min(lo + tpt, b.t_lo + b.tokens) - 1 : b.t_lo + b.tokens - 1;
-  const Span sp = span_of<KT>(p, s, lo, hi);
-  a.sink_end = (sp.sinks + KT - 1) / KT;
-  a.first = sp.first;
-  a.end = sp.end;
-  return a;
-}
-
-// A piece of the share as the roles need it; one thread works ahead and leaves it in shared memory.
+// A piece of the share as the roles need it; one thread works ahead and leaves it in shared memory.  Its key tiles are
+// m = 0 .. n - 1 (tile v0 + m of the span).  Step e of the piece brings K of tile e and V of tile e - ahead through one slot
+// of the ring (n + ahead steps): every row tile's S is computed two tiles ahead of its P.
 struct Piece {
   Seq s;
   Span span;
-  Active act[2];
-  int n;                                // key tiles v0 .. v0 + n; -1: there are no more pieces
+  int n;                                // -1: there are no more pieces
   int v0, two, h, t_lo, tokens;
-  int has[2];                           // whether a row tile (set of warps) sees any of them
+  int sink_end[2], first[2], end[2];    // row tile x sees the tiles m < sink_end[x] and first[x] <= m < end[x]
+  int tiles[2];                         // how many of the piece's that are
+  int clean_sinks, clean_lo, clean_hi;  // key tiles (by number) that some row sees to the last key
+  int full_sinks, full_lo, full_hi;     // key tiles that every row sees to the last key
   int whole;                            // the piece is the whole item
   int cut;                              // else: where its results go
 };
 
 struct Bars {
-  uint64_t full[10], empty[10];         // ring
-  uint64_t q_full, q_empty, dirty, fixed, drain, swap[2];
-  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t full[8], empty[8];           // ring
+  uint64_t q_full, q_empty, fixed, drain[2], swap[2];
+  uint64_t s_full[2][2], p_full[2][2];  // of row tile x, buffer b
+  uint64_t o_done[2];                   // every product with V
+  uint64_t o_full[2], o_empty[2];       // the piece's result is there, has been read
   uint64_t piece_full[2], piece_empty[2];
 };
-static_assert(sizeof(Bars) <= 512 && sizeof(Piece) <= 160, "the tail's layout");
-constexpr int READERS = 2 + 1 + 8;      // of a piece: loads, tensor core, clearing warp, softmax warps
+static_assert(sizeof(Bars) <= 512 && sizeof(Piece) <= 216, "the tail's layout");
+constexpr int READERS = 1 + 2 + 8;      // warps that read a piece: loads, tensor core, softmax
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -142,37 +133,52 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+__device__ __forceinline__ bool elect() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+  return ok != 0;
+}
+// rb::mbar_wait without the sleep between tries: the waits here are on the critical path and short
+__device__ __forceinline__ bool spin_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status) {
+  for (uint32_t it = 0; it < WAIT; ++it) {
+    if (rb::mbar_try_wait(bar, parity)) return true;
+    if ((it & 1023) == 1023 && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  if (status) atomicCAS(status, 0, RB_ERR_MBAR_TIMEOUT);
+  return false;
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const Batch p, const Outs w) {
   using C = Cfg<D>;
   extern __shared__ __align__(1024) uint8_t smem[];                           // the swizzle wants it; nothing is left to align by hand
-  uint8_t* q_s = smem;                                                        // [2][TILE]
-  uint8_t* ring = smem + 2 * C::TILE;                                         // [STAGES][TILE]
-  uint8_t* tail = ring + C::STAGES * C::TILE;
+  uint8_t* q_s = smem;                                                        // [2][Q_TILE]
+  uint8_t* ring = smem + 2 * C::Q_TILE;                                       // [STAGES][K, V][TILE]
+  uint8_t* tail = ring + C::STAGES * 2 * C::TILE;
   Bars* bars = reinterpret_cast<Bars*>(tail);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 512);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 516);
   int* found = reinterpret_cast<int*>(tail + 520);                            // sequence, block
   long long* found_base = reinterpret_cast<long long*>(tail + 528);
-  long long* wsum = reinterpret_cast<long long*>(tail + 544);                 // [12]
-  int* wcnt = reinterpret_cast<int*>(tail + 640);                             // [12]
-  float* ml = reinterpret_cast<float*>(tail + 704);                           // [2][MT][2]
-  Piece* pieces = reinterpret_cast<Piece*>(tail + 2752);                      // [2]
+  long long* wsum = reinterpret_cast<long long*>(ring + 4 * THREADS);         // [12], before the first load like first_item
+  int* wcnt = reinterpret_cast<int*>(ring + 4 * THREADS + 128);               // [12]
+  float* ml = reinterpret_cast<float*>(tail + 592);                           // [2][MT][2]
+  Piece* pieces = reinterpret_cast<Piece*>(tail + 2640);                      // [2]
   int* first_item = reinterpret_cast<int*>(ring);                             // [THREADS], before the first load
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tpt = MT / p.G;                                                   // tokens per row tile
   const int nb = p.a.B + p.b.B;
 
   if (tid == 0) {
-    for (int i = 0; i < C::STAGES; ++i) { rb::mbar_init(&bars->full[i], 1); rb::mbar_init(&bars->empty[i], 1); }
-    rb::mbar_init(&bars->q_full, 1); rb::mbar_init(&bars->q_empty, 1);
-    rb::mbar_init(&bars->dirty, 1);
-    rb::mbar_init(&bars->fixed, 32); rb::mbar_init(&bars->drain, 1);
+    for (int i = 0; i < C::STAGES; ++i) { rb::mbar_init(&bars->full[i], 1); rb::mbar_init(&bars->empty[i], 2); }
+    rb::mbar_init(&bars->q_full, 1); rb::mbar_init(&bars->q_empty, 2);
+    rb::mbar_init(&bars->fixed, 2);
     for (int i = 0; i < 2; ++i) {
-      rb::mbar_init(&bars->s_full[i], 1); rb::mbar_init(&bars->p_full[i], MT);
-      rb::mbar_init(&bars->o_full[i], 1); rb::mbar_init(&bars->o_empty[i], MT);
-      rb::mbar_init(&bars->swap[i], 2 * MT);
+      for (int j = 0; j < 2; ++j) { rb::mbar_init(&bars->s_full[i][j], 1); rb::mbar_init(&bars->p_full[i][j], MT / 32); }
+      rb::mbar_init(&bars->o_done[i], 1); rb::mbar_init(&bars->o_full[i], 1); rb::mbar_init(&bars->o_empty[i], MT / 32);
+      rb::mbar_init(&bars->swap[i], 2 * MT / 32); rb::mbar_init(&bars->drain[i], 1);
       rb::mbar_init(&bars->piece_full[i], 1); rb::mbar_init(&bars->piece_empty[i], READERS);
     }
     *abort_flag = 0;
@@ -263,15 +269,25 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const uint32_t tmem = *tmem_slot;                                           // S / P of row tile w at w * 128, O at 256 + w * 128
   bool gave_up = false;
   int n_piece = 0;
-  // the next piece, or null when there are no more (or a wait ran out; warps that work as one give up as one)
-  auto next_piece = [&](bool as_warp) -> const Piece* {
-    bool ok = !gave_up && rb::mbar_wait(&bars->piece_full[n_piece & 1], (n_piece >> 1) & 1, abort_flag, p.status, WAIT);
-    if (as_warp) ok = __all_sync(0xffffffffu, ok);
-    if (!ok) { gave_up = true; return nullptr; }
+  // A warp waits and arrives as one: lane 0 does it.  (Every thread's own arrival and polling on the same word is served
+  // one after another: with 128 of each per step that was most of a step's time.)
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    int ok = 0;
+    ok = !gave_up && spin_wait(bar, parity, abort_flag, p.status);
+    if (!__all_sync(0xffffffffu, ok)) gave_up = true;
+    return !gave_up;
+  };
+  auto arrive = [&](uint64_t* bar) {
+    __syncwarp();
+    if (lane == 0) rb::mbar_arrive(bar);
+  };
+  // the next piece, or null when there are no more (or a wait ran out); a warp gives up as one
+  auto next_piece = [&]() -> const Piece* {
+    if (!wait(&bars->piece_full[n_piece & 1], (n_piece >> 1) & 1)) return nullptr;
     const Piece* q = pieces + (n_piece & 1);
     return q->n < 0 ? nullptr : q;
   };
-  auto done_piece = [&]() { rb::mbar_arrive(&bars->piece_empty[n_piece & 1]); ++n_piece; };
+  auto done_piece = [&]() { arrive(&bars->piece_empty[n_piece & 1]); ++n_piece; };
 
   if (warp == 3) {
     // ------------------------------------------------------------------ pieces
@@ -282,25 +298,35 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mt.valid = 0;
       for (;; ++n_piece) {
         const bool more = walk.next(p, tpt);
-        if (!rb::mbar_wait(&bars->piece_empty[n_piece & 1], ((n_piece >> 1) & 1) ^ 1, abort_flag, p.status, WAIT)) break;
+        if (!spin_wait(&bars->piece_empty[n_piece & 1], ((n_piece >> 1) & 1) ^ 1, abort_flag, p.status)) break;
         Piece& q = pieces[n_piece & 1];
         q.n = -1;
         if (more) {
           const Block& b = walk.b;
           q.s = walk.s; q.span = b.span; q.v0 = walk.v0(); q.n = max(walk.v1() - walk.v0(), 0); q.two = b.two; q.h = walk.h;
           q.t_lo = b.t_lo; q.tokens = b.tokens;
+          const int skip = b.span.first - b.span.sink_tiles + q.v0;            // tile number - m, past the sinks
           for (int x = 0; x < 2; ++x) {
-            const Active act = active_of(p, walk.s, b, x, tpt);
-            q.act[x] = act;
-            int has = !b.two && q.n > x;
-            if (b.two) for (int j = 0; j < q.n && !has; ++j) has = act(b.span.tile(q.v0 + j));
-            q.has[x] = has;
+            const int lo = b.t_lo + x * tpt;
+            const Span sx = span_of<KT>(p, walk.s, lo, min(lo + tpt, b.t_lo + b.tokens) - 1);
+            q.sink_end[x] = (sx.sinks + KT - 1) / KT - q.v0;               // (past sink_tiles nothing is skipped)
+            q.first[x] = sx.first - skip;
+            q.end[x] = sx.end - skip;
+            // sinks first, then the range, without what both count
+            const int se = min(max(q.sink_end[x], 0), q.n), fi = min(max(q.first[x], se), q.n), en = min(max(q.end[x], fi), q.n);
+            q.tiles[x] = b.two ? se + en - fi : (q.n + 1 - x) / 2;
           }
-          q.whole = walk.u0 == 0 && walk.u1 == b.units;
+          const bool win = walk.s.causal && p.window > 0;
+          q.clean_sinks = b.span.sinks / KT; q.clean_lo = (b.span.lo + KT - 1) / KT; q.clean_hi = b.span.hi / KT;
+          const int upto = max(walk.s.causal ? b.span.p_min + 1 : b.span.hi, 0);
+          q.full_sinks = win ? min(p.sinks, upto) / KT : 0;
+          q.full_lo = win ? (max(b.span.p_max - p.window + 1, 0) + KT - 1) / KT : 0;
+          q.full_hi = upto / KT;
+          q.whole = walk.u0 <= FIXED && walk.u1 == b.units;
           q.cut = cta * 2 + (walk.pos == walk.p0 ? 0 : 1);
           const long long t0 = walk.pos - walk.u0;
-          if (walk.pos == walk.p0 && walk.u0 > 0 && share(cta - 1, n_sh, total) <= t0) {
-            // the first border inside this item: another kernel joins its pieces
+          if (walk.pos == walk.p0 && walk.u0 > FIXED && share(cta - 1, n_sh, total) <= t0 + FIXED) {
+            // the first border between this item's tiles: another kernel joins its pieces
             mt.valid = 1; mt.seq = walk.seq; mt.row0 = b.t_lo * p.G; mt.rows = b.tokens * p.G; mt.h = walk.h;
             mt.t0 = t0; mt.total = total; mt.n = n_sh; mt.c0 = cta - 1;
             mt.c1 = static_cast<int>(((t0 + b.units) * n_sh - 1) / total);
@@ -313,187 +339,160 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       w.meta[cta] = mt;
     }
   } else if (warp == 0) {
-    // ------------------------------------------------------------------ loads
-    if (lane == 0) {
-      int r = 0, n_q = 0;
-      while (const Piece* q = next_piece(false)) {
-        const bool two = q->two;
-        const int v0 = q->v0, n = q->n, h = q->h;
-        const Seq s = q->s;
-        const Span sp = q->span;
-        const int q_row = s.q_begin + q->t_lo;
-        done_piece();
-        if (n == 0) continue;
-        auto load_kv = [&](int kind, int m) {                                 // kind 0: K, 1: V
-          const int st = r % C::STAGES;
-          if (gave_up || !rb::mbar_wait(&bars->empty[st], ((r / C::STAGES) & 1) ^ 1, abort_flag, p.status, WAIT)) { gave_up = true; return; }
-          uint8_t* dst = ring + st * C::TILE;
-          rb::mbar_expect_tx(&bars->full[st], C::TILE);
-          const int k0 = sp.tile(v0 + m) * KT;
-          for (int x = 0; x < KT; x += p.box_rows) {
-            const int row = box_row(p, s, sp, k0 + x) + kind * p.page_size;
-#pragma unroll
-            for (int c = 0; c < C::CH; ++c)
-              rb::tma_load_2d(dst + c * (KT * 128) + x * 128, &tm_kv, &bars->full[st], h * D + c * 64, row);
-          }
-          ++r;
-        };
-        if (!rb::mbar_wait(&bars->q_empty, (n_q & 1) ^ 1, abort_flag, p.status, WAIT)) { gave_up = true; break; }
-        ++n_q;
-        const int tiles_q = two ? 2 : 1;
-        rb::mbar_expect_tx(&bars->q_full, tiles_q * C::CH * p.G * tpt * 128);
-        for (int t = 0; t < tiles_q; ++t)
-#pragma unroll
-          for (int c = 0; c < C::CH; ++c)
-            rb::tma_load_3d(q_s + t * C::TILE + c * (MT * 128), &tm_q, &bars->q_full, c * 64, h * p.G, q_row + t * tpt);
-        // the order of k_index and v_index
-        load_kv(0, 0);
-        if (!two && n > 1) load_kv(0, 1);
-        for (int m = 0; m < n; ++m) {
-          load_kv(1, m);
-          const int k = two ? m + 1 : m + 2;
-          if (k < n) load_kv(0, k);
-        }
-      }
-      if (gave_up)                                                            // copies in flight end before the kernel does
-        for (int i = max(r - C::STAGES, 0); i < r; ++i)
-          for (int k = 0; k < (1 << 16) && !rb::mbar_try_wait(&bars->full[i % C::STAGES], (i / C::STAGES) & 1); ++k) {}
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ tensor core
-    if (lane == 0) {
-      const uint32_t idesc_s = rb::umma_idesc(MT, KT, 0, 0, BF16), idesc_o = rb::umma_idesc(MT, D, 0, 1, BF16);
-      const uint32_t q_addr = rb::smem_u32(q_s), ring_addr = rb::smem_u32(ring);
-      int r0 = 0, n_q = 0, n_fix = 0;                                         // ring loads before this piece, blocks, cleared tiles
-      uint32_t par_p = 0, par_o = 0;                                          // bit x: parity of row tile x's next P, next O
-      while (const Piece* q = next_piece(false)) {
-        const bool two = q->two;
-        const int v0 = q->v0, n = q->n;
-        const Span sp = q->span;
-        const Active act0 = q->act[0], act1 = q->act[1];
-        done_piece();
-        if (n == 0) continue;
-        const int slots = two ? n : (n + 1) / 2;
-        int k_seen = -1, v_seen = -1;
-        uint32_t started = 0;
-        auto tile_at = [&](int slot, int x) { return two ? slot : 2 * slot + x; };
-        auto valid = [&](int slot, int x) {
-          const int m = tile_at(slot, x);
-          if (slot >= slots || m >= n) return false;
-          if (!two) return true;
-          const int t = sp.tile(v0 + m);
-          return x == 0 ? act0(t) : act1(t);
-        };
-        auto wait_full = [&](int idx) {
-          if (!gave_up && !rb::mbar_wait(&bars->full[idx % C::STAGES], (idx / C::STAGES) & 1, abort_flag, p.status, WAIT)) gave_up = true;
-          return !gave_up;
-        };
-        // a K or V tile is given back once its last user has been issued
-        auto release = [&](int idx) { rb::umma_commit(&bars->empty[idx % C::STAGES]); };
-        auto see_k = [&](int m) {
-          if (m <= k_seen) return !gave_up;
-          k_seen = m;
-          return wait_full(r0 + k_index(two, m));
-        };
-        auto issue_s = [&](int slot, int x) {                                 // S_x = Q_x K^T
-          const int m = tile_at(slot, x);
-          if (!see_k(m)) return;
-          rb::tc_fence_after();
-          const uint32_t qa = q_addr + (two ? x : 0) * C::TILE, ka = ring_addr + ((r0 + k_index(two, m)) % C::STAGES) * C::TILE;
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk / 4) * (KT * 128) + (kk % 4) * 32;
-            rb::umma_f16_ss(tmem + x * 128, rb::umma_smem_desc(qa + off, 16, 1024), rb::umma_smem_desc(ka + off, 16, 1024), idesc_s,
-                            kk > 0 ? 1u : 0u);
-          }
-          rb::umma_commit(&bars->s_full[x]);
-        };
-        auto end_k = [&](int slot) {                                          // all of a slot's S are issued
-          if (slot >= slots) return;
-          for (int x = 0; x < (two ? 1 : 2); ++x) {
-            const int m = tile_at(slot, x);
-            if (m < n && see_k(m)) release(r0 + k_index(two, m));             // (a tile nobody needs has been loaded all the same)
-          }
-          if (slot == slots - 1) rb::umma_commit(&bars->q_empty);
-        };
-        if (!rb::mbar_wait(&bars->q_full, n_q & 1, abort_flag, p.status, WAIT)) { gave_up = true; break; }
-        ++n_q;
-        for (int x = 0; x < 2; ++x) if (valid(0, x)) issue_s(0, x);
-        end_k(0);
-        for (int j = 0; j < slots && !gave_up; ++j) {
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int m = tile_at(j, x);
-            if (m < n && m > v_seen) {                                        // V of this tile, cleared where no row sees it
-              v_seen = m;
-              if (!wait_full(r0 + v_index(two, m, n))) break;
-              const int k0 = sp.tile(v0 + m) * KT;
-              if (!(k0 + KT <= sp.hi && (k0 >= sp.lo || k0 + KT <= sp.sinks))) {
-                rb::mbar_arrive(&bars->dirty);
-                if (!rb::mbar_wait(&bars->fixed, n_fix & 1, abort_flag, p.status, WAIT)) { gave_up = true; break; }
-                ++n_fix;
-              }
-            }
-            if (valid(j, x)) {
-              const uint32_t bit = 1u << x;
-              if (!(started & bit)) {
-                if (!rb::mbar_wait(&bars->o_empty[x], ((par_o >> x) & 1) ^ 1, abort_flag, p.status, WAIT)) { gave_up = true; break; }
-                par_o ^= bit;
-              }
-              if (!rb::mbar_wait(&bars->p_full[x], (par_p >> x) & 1, abort_flag, p.status, WAIT)) { gave_up = true; break; }
-              par_p ^= bit;
-              rb::tc_fence_after();
-              const uint32_t va = ring_addr + ((r0 + v_index(two, m, n)) % C::STAGES) * C::TILE;
-#pragma unroll
-              for (int kk = 0; kk < KT / 16; ++kk)
-                rb::umma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, rb::umma_smem_desc(va + kk * 2048, KT * 128, 1024), idesc_o,
-                                ((started & bit) || kk > 0) ? 1u : 0u);
-              started |= bit;
-            }
-            if (m < n && (!two || x == 1)) release(r0 + v_index(two, m, n));
-            if (valid(j + 1, x)) issue_s(j + 1, x);
-          }
-          if (!gave_up) end_k(j + 1);
-        }
-        if (gave_up) break;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) if (started & (1u << x)) rb::umma_commit(&bars->o_full[x]);
-        r0 += 2 * n;
-      }
-      if (gave_up) {                                                          // nothing of ours still runs when TMEM is freed
-        rb::umma_commit(&bars->drain);
-        for (int k = 0; k < (1 << 16) && !rb::mbar_try_wait(&bars->drain, 0); ++k) {}
-      }
-    }
-  } else if (warp == 2) {
-    // ------------------------------------------------------------------ V rows that nobody sees
-    int r0 = 0, n_fix = 0;
-    while (const Piece* q = next_piece(true)) {
-      const int v0 = q->v0, n = q->n;
+    // ------------------------------------------------------------------ loads: a lane per box of K, a lane per box of V
+    int st = 0, n_q = 0, last = 0;
+    uint32_t par = 1;                                                         // of `empty`
+    const int boxes = KT / p.box_rows;
+    const int my_kind = lane / (boxes * C::CH);                               // 0: K, 1: V
+    const int my_box = lane / C::CH % boxes, my_chunk = lane % C::CH;
+    while (const Piece* q = next_piece()) {
       const bool two = q->two;
+      const int v0 = q->v0, n = q->n, col = q->h * D + my_chunk * 64, q_head = q->h * p.G;
+      const Seq s = q->s;
       const Span sp = q->span;
-      __syncwarp();
-      if (lane == 0) done_piece(); else ++n_piece;
-      for (int m = 0; m < n && !gave_up; ++m) {
-        const int k0 = sp.tile(v0 + m) * KT;
-        if (k0 + KT <= sp.hi && (k0 >= sp.lo || k0 + KT <= sp.sinks)) continue;
-        const bool ok = rb::mbar_wait(&bars->dirty, n_fix & 1, abort_flag, p.status, WAIT);      // it is there and still untouched
-        if (!__all_sync(0xffffffffu, ok)) { gave_up = true; break; }
-        ++n_fix;
-        uint8_t* tile = ring + ((r0 + v_index(two, m, n)) % C::STAGES) * C::TILE;
-        for (int i = lane; i < KT; i += 32) {
-          const int j = k0 + i;
-          if (j < sp.hi && (j >= sp.lo || j < sp.sinks)) continue;
-          uint4* row = reinterpret_cast<uint4*>(tile + i * 128);
+      const int q_row = s.q_begin + q->t_lo;
+      done_piece();
+      if (n == 0) continue;
+      // Rows of the boxes, looked up for 32 / boxes tiles at a time (a division, a page id: slow one by one): lane l holds
+      // box l % boxes of tile l / boxes of a batch; V lags K by less than a batch.
+      const int batch = 32 / boxes;
+      int rows_now = 0, rows_before = 0, begin = 0;                           // begin: first tile of rows_now
+      auto look_up = [&](int m0) {
+        const int m = m0 + lane / boxes, v = v0 + m;
+        const int k0 = (v < sp.sink_tiles ? v : sp.first + v - sp.sink_tiles) * KT;
+        rows_before = rows_now;
+        rows_now = m < n && lane < batch * boxes ? box_row(p, s, sp, k0 + (lane % boxes) * p.box_rows) : p.total_rows;
+        begin = m0;
+      };
+      look_up(0);
+      if (!wait(&bars->q_empty, (n_q & 1) ^ 1)) break;
+      ++n_q;
+      if (lane == 0) {
+        rb::mbar_expect_tx(&bars->q_full, (two ? 2 : 1) * C::CH * p.G * tpt * 128);
+        for (int t = 0; t < (two ? 2 : 1); ++t)
 #pragma unroll
           for (int c = 0; c < C::CH; ++c)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) row[c * (KT * 8) + e] = make_uint4(0, 0, 0, 0);
-        }
-        rb::fence_proxy_async_smem();
-        rb::mbar_arrive(&bars->fixed);
+            rb::tma_load_3d(q_s + t * C::Q_TILE + c * (MT * 128), &tm_q, &bars->q_full, c * 64, q_head, q_row + t * tpt);
       }
-      r0 += 2 * n;
+      const int ahead = two ? 2 : 4;
+      for (int e = 0; e < n + ahead; ++e) {
+        if (e == begin + batch) look_up(e);
+        const int m = my_kind ? e - ahead : e;                                // this lane's tile
+        const int src = (m - begin) * boxes + my_box;
+        const int now = __shfl_sync(0xffffffffu, rows_now, src & 31), old = __shfl_sync(0xffffffffu, rows_before, (src + batch * boxes) & 31);
+        const int row = (m >= begin ? now : old) + my_kind * p.page_size;
+        if (!wait(&bars->empty[st], par)) break;
+        if (lane == 0) rb::mbar_expect_tx(&bars->full[st], ((e < n ? 1 : 0) + (e >= ahead ? 1 : 0)) * C::TILE);
+        __syncwarp();
+        if (my_kind < 2 && m >= 0 && m < n)
+          rb::tma_load_2d(ring + (st * 2 + my_kind) * C::TILE + my_chunk * (KT * 128) + my_box * p.box_rows * 128, &tm_kv, &bars->full[st], col, row);
+        ++last;
+        if (++st == C::STAGES) { st = 0; par ^= 1; }
+      }
+    }
+    if (gave_up && lane == 0)                                                 // copies in flight end before the kernel does
+      for (int i = max(last - C::STAGES, 0); i < last; ++i)
+        for (int k = 0; k < (1 << 16) && !rb::mbar_try_wait(&bars->full[i % C::STAGES], (i / C::STAGES) & 1); ++k) {}
+  } else if (warp < 3) {
+    // ------------------------------------------------------------------ tensor core: warp 1 + x for row tile x
+    // Each of the two walks the whole ring and gives every tile back, used or not, so both keep its order.
+    const int x = warp - 1;
+    const uint32_t idesc_s = rb::umma_idesc(MT, KT, 0, 0, BF16), idesc_o = rb::umma_idesc(MT, D, 0, 1, BF16);
+    const uint32_t t_s = tmem + x * 128, t_o = tmem + 256 + x * 128;          // S and P: two buffers of KT columns
+    // descriptors of a tile at offset 0; an address is added to the low word in units of 16 bytes
+    const uint32_t ring_at = rb::smem_u32(ring) >> 4;
+    const uint64_t d_k = rb::umma_smem_desc(0, 16, 1024) + ring_at, d_v = rb::umma_smem_desc(0, KT * 128, 1024) + ring_at + (C::TILE >> 4);
+    const uint64_t d_q = rb::umma_smem_desc(0, 16, 1024) + (rb::smem_u32(q_s) >> 4);
+    int st = 0;
+    uint32_t par = 0, par_q = 0, par_o = 1, par_fix = 0, n_s = 0, n_p = 0;   // n_s, n_p: this row tile's S and P so far
+    // the ring's slot goes back once what was issued so far is done
+    auto pass = [&](bool used) {
+      if (elect()) {
+        if (used) rb::umma_commit(&bars->empty[st]); else rb::mbar_arrive(&bars->empty[st]);
+      }
+      if (++st == C::STAGES) { st = 0; par ^= 1; }
+    };
+    auto mma_s = [&](int q_tile) {                                            // S = Q K^T with the slot's K
+      rb::tc_fence_after();
+      const uint32_t buf = n_s++ & 1;
+      if (elect()) {
+        const uint64_t dq = d_q + static_cast<uint32_t>(q_tile * (C::Q_TILE >> 4)), dk = d_k + static_cast<uint32_t>(st * (C::TILE >> 3));
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          rb::umma_f16_ss(t_s + buf * KT, dq + (((kk / 4) * (MT * 128) + (kk % 4) * 32) >> 4),
+                          dk + (((kk / 4) * (KT * 128) + (kk % 4) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+        rb::umma_commit(&bars->s_full[x][buf]);
+      }
+    };
+    while (const Piece* q = next_piece()) {
+      const bool two = q->two, any = q->tiles[x] > 0;
+      const int n = q->n;
+      const int v0 = q->v0, sink_tiles = q->span.sink_tiles, skip = q->span.first - sink_tiles;
+      const int c_sinks = q->clean_sinks, c_lo = q->clean_lo, c_hi = q->clean_hi;
+      const int hi = q->span.hi, lo = q->span.lo, sinks = q->span.sinks;
+      const int se = q->sink_end[x], fi = q->first[x], en = q->end[x];
+      done_piece();
+      if (n == 0) continue;
+      bool started = false;
+      auto mine = [&](int m) { return two ? m < se || (m >= fi && m < en) : (m & 1) == x; };
+      if (!wait(&bars->q_full, par_q)) break;
+      par_q ^= 1;
+      const int ahead = two ? 2 : 4;
+      for (int e = 0; e < n + ahead; ++e) {
+        const int m = e - ahead;
+        const bool use_k = e < n && mine(e), use_v = m >= 0 && mine(m);
+        if (!wait(&bars->full[st], par)) break;
+        if (m >= 0 && (two || use_v)) {
+          // V of keys that no row of the block sees may be anything: clear it
+          const int v = v0 + m, t = v < sink_tiles ? v : v + skip;
+          if (!(t < c_sinks || (t >= c_lo && t < c_hi))) {
+            uint8_t* tile = ring + (st * 2 + 1) * C::TILE;
+            for (int i = two ? lane * 2 + x : lane; i < KT; i += two ? 64 : 32) {
+              const int j = t * KT + i;
+              if (j < hi && (j >= lo || j < sinks)) continue;
+              uint4* row = reinterpret_cast<uint4*>(tile + i * 128);
+#pragma unroll
+              for (int c = 0; c < C::CH; ++c)
+#pragma unroll
+                for (int u = 0; u < 8; ++u) row[c * (KT * 8) + ((u + lane) & 7)] = make_uint4(0, 0, 0, 0);
+            }
+            rb::fence_proxy_async_smem();
+            __syncwarp();
+            if (two) {                                                        // the other half of the rows is the other warp's
+              arrive(&bars->fixed);
+              if (!wait(&bars->fixed, par_fix)) break;
+              par_fix ^= 1;
+            }
+          }
+        }
+        if (use_v) {                                                          // O (+)= P V
+          if (!started) {
+            if (!wait(&bars->o_empty[x], par_o)) break;
+            par_o ^= 1;
+          }
+          const uint32_t buf = n_p & 1;
+          if (!wait(&bars->p_full[x][buf], (n_p >> 1) & 1)) break;
+          ++n_p;
+          rb::tc_fence_after();
+          if (elect()) {
+            const uint64_t dv = d_v + static_cast<uint32_t>(st * (C::TILE >> 3));
+#pragma unroll
+            for (int kk = 0; kk < KT / 16; ++kk)
+              rb::umma_f16_ts(t_o, t_s + buf * KT + kk * 8, dv + kk * 128, idesc_o, (kk > 0 || started) ? 1u : 0u);
+            rb::umma_commit(&bars->o_done[x]);
+          }
+          started = true;
+        }
+        if (use_k) mma_s(two ? x : 0);
+        pass(use_k || use_v);
+        if (e == n - 1 && elect()) rb::umma_commit(&bars->q_empty);           // the last S is issued: Q may go
+      }
+      if (gave_up) break;
+      if (any && elect()) rb::umma_commit(&bars->o_full[x]);
+    }
+    if (gave_up && lane == 0) {                                               // nothing of ours still runs when TMEM is freed
+      rb::umma_commit(&bars->drain[x]);
+      for (int k = 0; k < (1 << 16) && !rb::mbar_try_wait(&bars->drain[x], 0); ++k) {}
     }
   } else {
     // ------------------------------------------------------------------ softmax: thread = row
@@ -501,57 +500,52 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int row = quarter * 32 + lane;
     const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t t_s = tmem + lane_sel + x * 128, t_o = tmem + lane_sel + 256 + x * 128;
-    const int my_tok = row / p.G;                                              // of the row tile
-    uint32_t par_s = 0, par_o = 0, par_swap = 0;
-    while (const Piece* q = next_piece(true)) {
+    const int my_tok = row / p.G, my_head = row % p.G;                         // of the row tile, of the group
+    uint32_t n_s = 0, par_o = 0, par_swap = 0;                                  // key tiles so far; bit y: of row tile y's o_full
+    while (const Piece* q = next_piece()) {
       const bool two = q->two;
       const int n = q->n;
       float m_ref = -INFINITY, sum = 0.f;                                      // log2 domain
       bool any = false;
       {
-        const int v0 = q->v0, slots = two ? n : (n + 1) / 2;
-        const Active act = q->act[x];
-        const int sink_tiles = q->span.sink_tiles, skip = q->span.first - sink_tiles;
-        const int len_k = q->s.len_k, causal = q->s.causal;
+        const int v0 = q->v0, sink_tiles = q->span.sink_tiles, skip = q->span.first - sink_tiles;
+        const int se = q->sink_end[x], fi = q->first[x], en = q->end[x];
+        const int full_s = q->full_sinks, full_lo = q->full_lo, full_hi = q->full_hi;
         const int pos = q->t_lo + (two ? x * tpt : 0) + my_tok + q->s.delta();
-        // tiles that every row of the block sees in full: ends at or before p_min (hi), begins after p_max - window or is all sinks
-        const int full_hi = causal ? q->span.p_min + 1 : q->span.hi;
-        const int full_lo = causal && p.window > 0 ? q->span.p_max - p.window + 1 : 0;
-        for (int j = 0; j < slots; ++j) {
-          const int m = two ? j : 2 * j + x;
-          if (m >= n) continue;
+        // this row sees the keys below `upto`, of those the ones from `from` on and the sinks
+        const int upto = q->s.causal ? min(pos + 1, q->s.len_k) : q->s.len_k;
+        const bool win = q->s.causal && p.window > 0;
+        const int from = win ? pos - p.window + 1 : 0, sinks = win ? p.sinks : 0;
+        for (int m = two ? 0 : x; m < n; m += two ? 1 : 2) {
+          if (two && !(m < se || (m >= fi && m < en))) continue;
           const int t = v0 + m < sink_tiles ? v0 + m : v0 + m + skip;
-          if (two && !act(t)) continue;
-          const bool ok = rb::mbar_wait(&bars->s_full[x], par_s, abort_flag, p.status, WAIT);
-          if (!__all_sync(0xffffffffu, ok)) { gave_up = true; break; }
-          par_s ^= 1;
+          const uint32_t buf = n_s & 1;
+          if (!wait(&bars->s_full[x][buf], (n_s >> 1) & 1)) break;
           rb::tc_fence_after();
-          uint32_t sr[4][32];
+          uint32_t sr[KT / 32][32];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) rb::tmem_ld_32x32(t_s + c * 32, sr[c]);
+          for (int c = 0; c < KT / 32; ++c) rb::tmem_ld_32x32(t_s + buf * KT + c * 32, sr[c]);
           rb::tmem_ld_wait();
-          const int k0 = t * KT;
-          if (!(k0 + KT <= full_hi && (k0 >= full_lo || k0 + KT <= p.sinks))) {
-            // bit-wise limits of this row: keys below `upto`, of those from `from` on or sinks
-            const int upto = min(causal ? min(pos + 1, len_k) : len_k, k0 + KT) - k0;
-            const int from = causal && p.window > 0 ? pos - p.window + 1 - k0 : -1, sink = p.sinks - k0;
+          if (!(t < full_s || (t >= full_lo && t < full_hi))) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < KT / 32; ++c) {
+              const int k0 = t * KT + c * 32;
+              auto below = [&](int n_keys) { const int d = n_keys - k0; return d >= 32 ? 0xffffffffu : d <= 0 ? 0u : (1u << d) - 1u; };
+              const uint32_t seen = below(upto) & (~below(from) | below(sinks));
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const int i = c * 32 + e;
-                if (i >= upto || (i < from && i >= sink)) sr[c][e] = 0xff800000u;
-              }
-          }
-          float mx = -INFINITY, my = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              mx = fmaxf(mx, __uint_as_float(sr[c][e]));
-              my = fmaxf(my, __uint_as_float(sr[c][e + 1]));
+              for (int e = 0; e < 32; ++e)
+                if (!(seen & (1u << e))) sr[c][e] = 0xff800000u;
             }
-          const float m_new = fmaxf(mx, my) * p.scale_log2;                    // scale > 0 in this kernel
+          }
+          float mx[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t* v = &sr[c >> 1][(c & 1) * 16];
+            mx[c] = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[15]));
+#pragma unroll
+            for (int e = 1; e < 15; e += 2) mx[c] = fmaxf(mx[c], fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+          }
+          const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;   // scale > 0 in this kernel
           // O and the sum refer to m_ref; only a row that outgrows it by 2^8 (or its first weight) moves it
           const bool grow = m_new > m_ref + 8.f || (m_ref == -INFINITY && m_new > -INFINITY);
           if (__any_sync(0xffffffffu, grow)) {
@@ -559,7 +553,9 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             if (grow) m_ref = m_new;
             sum *= f;
             if (any) {
-              // S of this tile was issued after the product with the tile before: O is at rest
+              // once the product with the tile before is done, O is at rest until this tile's P is there
+              if (!wait(&bars->o_done[x], (n_s - 1) & 1)) break;
+              rb::tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < D / 16; ++c) {
                 uint32_t o[16];
@@ -576,7 +572,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           const float2 sc = make_float2(p.scale_log2, p.scale_log2), nb2 = make_float2(-base, -base);
           float2 acc0 = make_float2(sum, 0.f), acc1 = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < KT / 32; ++c) {
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
@@ -588,24 +584,25 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               pk[e >> 1] = pack16<BF16>(a.x, a.y);
               pk[(e >> 1) + 1] = pack16<BF16>(b.x, b.y);
             }
-            rb::tmem_st_32x16(t_s + c * 16, pk);
+            rb::tmem_st_32x16(t_s + buf * KT + c * 16, pk);
           }
           sum = (acc0.x + acc0.y) + (acc1.x + acc1.y);
           rb::tmem_st_wait();
           rb::tc_fence_before();
-          rb::mbar_arrive(&bars->p_full[x]);
+          arrive(&bars->p_full[x][buf]);
+          ++n_s;
           any = true;
         }
       }
       // ---- the piece's result: columns [c_lo, c_hi) of the row are this thread's to write
       int c_lo = 0, c_hi = D;
       float f0 = x == 0 ? 1.f : 0.f, f1 = 1.f - f0, l = sum, m_all = m_ref;
-      const bool mine = q->has[x] != 0, theirs = q->has[x ^ 1] != 0;
-      bool ok = !gave_up;
+      const bool mine = q->tiles[x] > 0;
+      const uint32_t had = (q->tiles[0] > 0 ? 1u : 0u) | (q->tiles[1] > 0 ? 2u : 0u);
       if (!two) {
         ml[(x * MT + row) * 2] = m_ref; ml[(x * MT + row) * 2 + 1] = sum;
-        rb::mbar_arrive(&bars->swap[0]);
-        ok = rb::mbar_wait(&bars->swap[0], par_swap, abort_flag, p.status, WAIT) && ok;
+        arrive(&bars->swap[0]);
+        wait(&bars->swap[0], par_swap);
         const float m0 = ml[row * 2], l0 = ml[row * 2 + 1], m1 = ml[(MT + row) * 2], l1 = ml[(MT + row) * 2 + 1];
         m_all = fmaxf(m0, m1);
         const float bm = m_all == -INFINITY ? 0.f : m_all;
@@ -613,61 +610,74 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         l = f0 * l0 + f1 * l1;
         c_lo = x * (D / 2); c_hi = c_lo + D / 2;
       }
-      const bool read0 = two ? x == 0 && mine : q->has[0] != 0, read1 = two ? x == 1 && mine : q->has[1] != 0;
-      if (ok && read0) ok = rb::mbar_wait(&bars->o_full[0], par_o & 1, abort_flag, p.status, WAIT);
-      if (ok && read1) ok = rb::mbar_wait(&bars->o_full[1], (par_o >> 1) & 1, abort_flag, p.status, WAIT);
-      if (!__all_sync(0xffffffffu, ok)) gave_up = true;
+      const bool read0 = two ? x == 0 && mine : q->tiles[0] > 0, read1 = two ? x == 1 && mine : q->tiles[1] > 0;
+      if (read0) wait(&bars->o_full[0], par_o & 1);
+      if (read1) wait(&bars->o_full[1], par_o >> 1);
+      par_o ^= had;
       rb::tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const float lse2 = l == 0.f ? -INFINITY : m_all + log2f(l);
       f0 *= inv; f1 *= inv;
       if (!gave_up) {
         const int r_cut = two ? x * tpt * p.G + row : row;                      // row of the block
-        const bool live = row < tpt * p.G && (two ? x * tpt : 0) + my_tok < q->tokens;
-        const int row0 = q->t_lo * p.G, h = q->h;
-        const bool whole = q->whole != 0;
-        const long long cut = static_cast<long long>(q->cut) * TILE_ROWS + r_cut;
+        const int tok = (two ? x * tpt : 0) + my_tok;
+        const bool live = row < tpt * p.G && tok < q->tokens;
+        const long long t = q->s.q_begin + q->t_lo + tok;
+        const int head = q->h * p.G + my_head;
+        // where this row goes: a 16-bit row of the result, or an fp32 row of a part or of a cut item's piece
+        float* dst32 = nullptr;
+        float* dst_lse;
+        uint16_t* dst16 = nullptr;
+        float lse_out = lse2;
+        if (!q->whole) {
+          const long long cut = static_cast<long long>(q->cut) * TILE_ROWS + r_cut;
+          dst32 = w.cut_o + cut * D;
+          dst_lse = w.cut_lse + cut;
+        } else if (w.part_o) {
+          const long long at = (static_cast<long long>(q->s.part) * p.Tq + t) * p.H + head;
+          dst32 = w.part_o + at * D;
+          dst_lse = w.part_lse + at;
+        } else {
+          dst16 = reinterpret_cast<uint16_t*>(w.out) + t * w.ld_o + static_cast<long long>(head) * D;
+          dst_lse = w.lse ? w.lse + t * p.H + head : nullptr;
+          lse_out = lse2 * LN2;
+        }
+        if (live && c_lo == 0 && dst_lse) *dst_lse = lse_out;
 #pragma unroll 1
-        for (int c = c_lo; c < c_hi; c += 16) {
-          uint32_t a[16];
-          float o[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = 0.f;
+        for (int c = c_lo; c < c_hi; c += 32) {
+          uint32_t a[32];
+          float o[32];
           if (read0) {
-            rb::tmem_ld_32x16(tmem + lane_sel + 256 + c, a);
+            rb::tmem_ld_32x32(tmem + lane_sel + 256 + c, a);
             rb::tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = f0 * __uint_as_float(a[e]);
           }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = read0 ? f0 * __uint_as_float(a[e]) : 0.f;
           if (read1) {
-            rb::tmem_ld_32x16(tmem + lane_sel + 384 + c, a);
+            rb::tmem_ld_32x32(tmem + lane_sel + 384 + c, a);
             rb::tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = fmaf(f1, __uint_as_float(a[e]), o[e]);
+            for (int e = 0; e < 32; ++e) o[e] = fmaf(f1, __uint_as_float(a[e]), o[e]);
           }
-          if (live) {
-            if (whole) {
-              write_row<D, BF16, 16>(p, w, q->s, row0 + r_cut, h, c, o, lse2);
-            } else {
-              float4* dst = reinterpret_cast<float4*>(w.cut_o + cut * D + c);
+          if (live && dst16) {
 #pragma unroll
-              for (int e = 0; e < 16; e += 4) dst[e >> 2] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-              if (c == 0) w.cut_lse[cut] = lse2;
-            }
+            for (int e = 0; e < 32; e += 8)
+              *reinterpret_cast<uint4*>(dst16 + c + e) = make_uint4(pack16<BF16>(o[e], o[e + 1]), pack16<BF16>(o[e + 2], o[e + 3]),
+                                                                    pack16<BF16>(o[e + 4], o[e + 5]), pack16<BF16>(o[e + 6], o[e + 7]));
+          } else if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(dst32 + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
       }
       rb::tc_fence_before();
       if (!two) {                                                               // both sets of warps read both results
-        rb::mbar_arrive(&bars->swap[1]);
-        const bool both = rb::mbar_wait(&bars->swap[1], par_swap, abort_flag, p.status, WAIT);
-        if (!__all_sync(0xffffffffu, both)) gave_up = true;
+        arrive(&bars->swap[1]);
+        wait(&bars->swap[1], par_swap);
         par_swap ^= 1;
       }
-      if (mine) { rb::mbar_arrive(&bars->o_empty[x]); par_o ^= 1u << x; }
-      if (theirs) par_o ^= 1u << (x ^ 1);
-      __syncwarp();
-      if (lane == 0) done_piece(); else ++n_piece;
+      if (mine) arrive(&bars->o_empty[x]);
+      done_piece();
     }
   }
   __syncwarp();
