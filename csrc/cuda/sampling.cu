@@ -4,23 +4,38 @@
 //     the first k;  of those, up to the first whose running sum reaches p times their sum;  of those, w_i >= min_p
 //   -> the smallest index i whose running sum over the kept items, in index order, exceeds u times their sum.
 //
-// Every filter keeps a beginning of the same order, so no sort is needed: a radix descent over the 32 ordered bits of the
-// score finds the last kept value (by count for k, by weight for p) and how many of the items that share it are kept.
+// Every filter keeps a beginning of the same order, so no sort is needed: a histogram over 1/64 octaves of the weight and a
+// radix descent inside the bin that the cut falls into find the last kept value (by count for k, by weight for p) and how
+// many of the items that share it are kept.  Where at most LIST items can be kept (short rows, small k), one CTA sorts
+// those instead.
 //
-// Weights are summed in 64 bits: with 10^5 items of similar score the borders lie 1e-5 apart, and 32-bit exponentials
-// (relative error 1e-7 each) would draw a neighbour every few thousand rows.  Sums inside the descent are whole numbers
-// (2^-44 of the largest weight for rows up to 2^18 items, coarser beyond), so atomics in any order give the same bits.
+// Weights are computed and summed in 64 bits: with N kept items each of the N borders can go either way with the sums'
+// relative error as its chance, and 32-bit exponentials (1e-7 each) would draw a neighbour in every hundredth row of 10^5
+// items.  The exponential is table-driven (Tang, ACM TOMS 15, 1989): 2^(n/64) from a table, 2^(f/64) as a polynomial of
+// degree 4 (relative error below 4e-14).  Sums inside the histograms are whole numbers (2^-44 of the largest weight for
+// rows up to 2^18 items, coarser beyond), so atomics in any order give the same bits.
+//
+// Bound: the row is read from memory once, into the shared memory of a cluster of CTAs (1 to 8 by its size and by how many
+// rows there are), which then exchange histograms and sums through distributed shared memory; what remains is the 64-bit
+// arithmetic, about ten operations per item and pass.  Rows that do not fit are read again from L2.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int NT = 512, NWARP = NT / 32;
-constexpr int BINS = 2048;
+constexpr int BINS = 2048, PB = BINS / NT;
+constexpr int MAX_CLUSTER = 8;
+constexpr int LIST = 1024;                      // items that are sorted, or kept aside for a descent
 
 struct SampleArgs {
   const void* scores; long long ld;             // dense: rows of `width`, `ld` elements apart
   const void* offsets; int offsets64;           // jagged: [rows + 1] into scores (then `width` is its length), or null
   long long width; int rows;
+  int cap;                                      // elements of a slice that shared memory holds
   const float* uniform;
   const float* temperature; const int* top_k; const float* top_p; const float* min_p;   // per row, or null: the values below
   float temperature_v; int top_k_v; float top_p_v, min_p_v;
@@ -41,34 +56,88 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 constexpr uint32_t KEY_NONE = 0x007fffffu;                         // -inf: never drawn
 
+// What the CTAs of a cluster read of one another
 struct Shared {
-  unsigned int cnt[BINS];
-  unsigned long long mass[BINS];
+  unsigned int lo[BINS], hi[BINS];              // 64-bit sums (or counts, in lo) by bin
+  double table[64];                             // 2^(j / 64)
+  unsigned int best, first;                     // largest key of the slice; its first index (where that is all that is asked)
+  unsigned long long list[LIST];                // (key, ~index) of the items that can be kept, or keys in the cut's bin
+  unsigned int listed;
+  unsigned int key_min, key_max;                // of the slice's items in the cut's bin
+  double sum; unsigned int ties;                // of the slice's kept items; of those that equal the cut
+  // within the CTA
   double wsum[NWARP];
   unsigned int wcnt[NWARP];
   unsigned long long wmass[NWARP];
-  double d0, d1;
-  unsigned long long m0;
+  unsigned int queue[NWARP][64];
   unsigned int u0, u1, u2;
+  unsigned long long m0, m1;
 };
 
-// weight of a score
+// exp((x - top) / T), 64 bits
 struct Weigher {
-  double top, inv_t;
+  const double* table;
+  double top, scale;                            // scale = 64 log2(e) / T
   uint32_t top_key;
-  __device__ __forceinline__ double operator()(uint32_t k) const {
-    return k == top_key ? 1.0 : exp((static_cast<double>(value_of(k)) - top) * inv_t);
+  // with its binary exponent raised by `up`
+  __device__ __forceinline__ double operator()(uint32_t k, int up = 0) const {
+    const double t = k == top_key ? 0.0 : (static_cast<double>(value_of(k)) - top) * scale;
+    if (!(t > -65000.0)) return 0.0;
+    const double magic = 6755399441055744.0;                       // 1.5 * 2^52: the sum's low word is the nearest whole number
+    const double nd = t + magic;
+    const int n = __double2loint(nd);
+    const double f = t - (nd - magic);
+    constexpr double c1 = 0.6931471805599453 / 64, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4;
+    const double q = fma(fma(fma(fma(c4, f, c3), f, c2), f, c1), f, 1.0) * table[n & 63];
+    return __hiloint2double(__double2hiint(q) + (((n >> 6) + up) << 20), __double2loint(q));
+  }
+  // the weight in units of 2^-shift, rounded (shift <= 44)
+  __device__ __forceinline__ unsigned long long fixed(uint32_t k, int shift) const {
+    const double w = (*this)(k, shift) + 4503599627370496.0;       // + 2^52
+    return static_cast<unsigned long long>(__double_as_longlong(w)) & 0xfffffffffffffULL;
   }
 };
 
 // Where the order is cut: everything above `key` is kept and the first `ties` items (in index order) that equal it.
 struct Cut { uint32_t key; unsigned int ties; };
 
+__device__ __forceinline__ void add64(Shared& s, int bin, unsigned long long v) {
+  const unsigned int lo = static_cast<unsigned int>(v);
+  const unsigned int old = atomicAdd(&s.lo[bin], lo);
+  const unsigned int hi = static_cast<unsigned int>(v >> 32) + (old + lo < old ? 1u : 0u);
+  if (hi) atomicAdd(&s.hi[bin], hi);
+}
+
+// f(key, index in the slice) for all of a slice, 16 bytes at a time where its address allows
+template <typename T, typename F>
+__device__ __forceinline__ void for_each(const T* x, int n, F&& f) {
+  constexpr int V = 16 / sizeof(T);
+  const int head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T)));
+  for (int i = threadIdx.x; i < head; i += NT) f(key_of(to_f<T>(x[i])), i);
+  const int nv = (n - head) / V;
+  const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+  for (int i = threadIdx.x; i < nv; i += NT) {
+    const uint4 u = xv[i];
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int j = 0; j < V; ++j) f(key_of(to_f<T>(e[j])), head + i * V + j);
+  }
+  for (int i = head + nv * V + threadIdx.x; i < n; i += NT) f(key_of(to_f<T>(x[i])), i);
+}
+
 template <typename T>
-__global__ void __launch_bounds__(NT) sample_kernel(const SampleArgs p) {
-  __shared__ Shared s;
+__global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  Shared& s = *reinterpret_cast<Shared*>(smem);
+  T* store = reinterpret_cast<T*>(smem + (sizeof(Shared) + 15) / 16 * 16);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int c = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
+  if (tid < 64) s.table[tid] = exp2(tid / 64.0);
+  auto sync = [&]() { if (c > 1) cluster.sync(); else __syncthreads(); };
+  auto peer = [&](int r) -> Shared& { return c > 1 ? *cluster.map_shared_rank(&s, r) : s; };
+
+  for (int row = blockIdx.x / c; row < p.rows; row += gridDim.x / c) {
     long long lo = 0, hi = p.width;
     const T* x = reinterpret_cast<const T*>(p.scores);
     if (p.offsets) {
@@ -80,212 +149,454 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleArgs p) {
     } else {
       x += row * p.ld;
     }
-    const int n = static_cast<int>(hi - lo);
+    const int n_row = static_cast<int>(hi - lo);
+    // this CTA's slice [s_lo, s_lo + n)
+    const int part = ((n_row + c - 1) / c + 31) / 32 * 32;
+    const int s_lo = min(rank * part, n_row), n = min(part, n_row - s_lo);
+    x += s_lo;
     const float temp = p.temperature ? p.temperature[row] : p.temperature_v;
     const int top_k = p.top_k ? p.top_k[row] : p.top_k_v;
     const float top_p = p.top_p ? p.top_p[row] : p.top_p_v;
     const float min_p = p.min_p ? p.min_p[row] : p.min_p_v;
-    float uf = p.uniform[row];
+    const float uf = p.uniform[row];
     const double u = uf > 0.f ? static_cast<double>(uf) : 0.0;
-    // ---- the largest score and its first index
-    unsigned long long best = 0;                                   // key, then index from the back
-    for (int i = tid; i < n; i += NT) {
-      const unsigned long long v = (static_cast<unsigned long long>(key_of(to_f<T>(x[i]))) << 32) | (0xffffffffu - i);
-      best = v > best ? v : best;
-    }
+
+    // ---- bring the slice in; its largest score (fmaxf passes over NaN)
+    float most = -INFINITY;
+    if (n <= p.cap) {
+      // at the same offset from a 16-byte border, so that both sides move in vectors
+      T* y = store + (reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T);
+      constexpr int V = 16 / sizeof(T);
+      const int head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T)));
+      const int nv = (n - head) / V;
+      for (int i = tid; i < head; i += NT) { y[i] = x[i]; most = fmaxf(most, to_f<T>(x[i])); }
+      const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+      uint4* yv = reinterpret_cast<uint4*>(y + head);
+#pragma unroll 4
+      for (int i = tid; i < nv; i += NT) {
+        const uint4 v = __ldg(xv + i);
+        yv[i] = v;
+        const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long v = __shfl_xor_sync(0xffffffffu, best, o);
-      best = v > best ? v : best;
+        for (int j = 0; j < V; ++j) most = fmaxf(most, to_f<T>(e[j]));
+      }
+      for (int i = head + nv * V + tid; i < n; i += NT) { y[i] = x[i]; most = fmaxf(most, to_f<T>(x[i])); }
+      x = y;
+    } else {
+      for_each<T>(x, n, [&](uint32_t k, int) { most = fmaxf(most, value_of(k)); });
     }
-    __syncthreads();                                               // the row before is done with the shared words
-    if (lane == 0) s.wmass[warp] = best;
+    uint32_t top_key = __reduce_max_sync(0xffffffffu, key_of(most));
+    if (lane == 0) s.wcnt[warp] = top_key;
+    if (tid == 0) { s.listed = 0; s.first = 0xffffffffu; }
     __syncthreads();
-    for (int i = 0; i < NWARP; ++i) best = s.wmass[i] > best ? s.wmass[i] : best;
-    const uint32_t top_key = static_cast<uint32_t>(best >> 32);
-    if (n == 0 || top_key <= KEY_NONE) {
-      if (tid == 0) { p.ids[row] = -1; p.logprobs[row] = -INFINITY; }
+    if (tid == 0) {
+      for (int i = 0; i < NWARP; ++i) top_key = max(top_key, s.wcnt[i]);
+      s.best = top_key;
+    }
+    sync();
+    for (int r = 0; r < c; ++r) top_key = max(top_key, peer(r).best);
+    if (n_row == 0 || top_key <= KEY_NONE) {
+      if (rank == 0 && tid == 0) { p.ids[row] = -1; p.logprobs[row] = -INFINITY; }
+      sync();                                                      // nobody's words are still being read
       continue;
     }
     if (!(temp > 0.f)) {
-      if (tid == 0) { p.ids[row] = 0xffffffffu - static_cast<uint32_t>(best); p.logprobs[row] = 0.f; }
+      unsigned int at = 0xffffffffu;
+      for_each<T>(x, n, [&](uint32_t k, int i) { if (k == top_key) at = min(at, static_cast<unsigned int>(s_lo + i)); });
+      at = __reduce_min_sync(0xffffffffu, at);
+      if (lane == 0 && at != 0xffffffffu) atomicMin(&peer(0).first, at);
+      sync();
+      if (rank == 0 && tid == 0) { p.ids[row] = s.first; p.logprobs[row] = 0.f; }
+      sync();
       continue;
     }
     Weigher wt;
-    wt.top = static_cast<double>(value_of(top_key)); wt.inv_t = 1.0 / static_cast<double>(temp); wt.top_key = top_key;
+    wt.table = s.table; wt.top = static_cast<double>(value_of(top_key)); wt.top_key = top_key;
+    wt.scale = 64.0 * 1.4426950408889634 / static_cast<double>(temp);
     Cut cut = {KEY_NONE, 0};
-    // ---- radix descent: by count, then by weight
-    const int shift_fx = 62 - max(18, 32 - __clz(n));
-    const double fx = static_cast<double>(1ULL << shift_fx);
-    for (int by_mass = 0; by_mass < 2; ++by_mass) {
-      if (by_mass ? !(top_p < 1.f) : !(top_k > 0 && top_k < n)) continue;
-      uint32_t prefix = 0;
-      int bits = 0;
-      unsigned int c_before = 0;
-      unsigned long long m_before = 0, target = 0;
-      bool none = false;
-      for (int level = 0; level < 3 && !none; ++level) {
-        const int width = level < 2 ? 11 : 10, down = 32 - bits - width;
-        for (int i = tid; i < BINS; i += NT) { s.cnt[i] = 0; s.mass[i] = 0; }
+    // bins of 1/64 octave of the weight, the last one open: monotone in the score, in 32 bits
+    const float top_f = value_of(top_key), bin_scale = 64.f * 1.44269504f / temp;
+    auto bin_of = [&](uint32_t k) { return static_cast<int>(fminf((top_f - value_of(k)) * bin_scale, BINS - 1.f)); };   // (NaN: inf - inf -> last)
+    const int shift_fx = 62 - max(18, 32 - __clz(n_row));
+    const double mp = static_cast<double>(min_p);
+
+    // ---- the first CTA's list holds everything that can be kept: sort, cut, draw
+    auto draw_listed = [&]() {
+      const int m = static_cast<int>(s.listed);
+      int size = 2;
+      while (size < m) size *= 2;
+      for (int i = m + tid; i < size; i += NT) s.list[i] = 0;
+      auto sort = [&](bool descending) {
+        for (int k = 2; k <= size; k *= 2)
+          for (int j = k / 2; j > 0; j /= 2) {
+            __syncthreads();
+            for (int t = tid; t < size / 2; t += NT) {
+              const int i = 2 * t - (t & (j - 1)), l = i + j;
+              const unsigned long long a = s.list[i], b = s.list[l];
+              if (((a < b) == descending) == ((i & k) == 0) && a != b) { s.list[i] = b; s.list[l] = a; }
+            }
+          }
         __syncthreads();
-        for (int i = tid; i < n; i += NT) {
-          const uint32_t k = key_of(to_f<T>(x[i]));
-          if (k <= cut.key || (bits && (k >> (32 - bits)) != prefix)) continue;
-          const int bin = (k >> down) & ((1 << width) - 1);
-          if (by_mass) atomicAdd(&s.mass[bin], static_cast<unsigned long long>(wt(k) * fx + 0.5));
-          else atomicAdd(&s.cnt[bin], 1u);
-        }
-        if (by_mass && tid == 0 && cut.ties && (!bits || (cut.key >> (32 - bits)) == prefix))
-          atomicAdd(&s.mass[(cut.key >> down) & ((1 << width) - 1)], cut.ties * static_cast<unsigned long long>(wt(cut.key) * fx + 0.5));
-        __syncthreads();
-        // the bin where the running sum from above reaches the target: 4 bins per thread, from the highest down
-        constexpr int PB = BINS / NT;
-        unsigned int c4 = 0;
-        unsigned long long m4 = 0;
-        for (int i = 0; i < PB; ++i) {
-          const int b = BINS - 1 - (tid * PB + i);
-          c4 += s.cnt[b];
-          m4 += s.mass[b];
-        }
-        unsigned int ci = c4;
-        unsigned long long mi = m4;
+      };
+      // running sums of two items per thread, in order -> sum before the first of them
+      auto scan = [&](double w0, double w1, double& all) {
+        double incl = w0 + w1;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const unsigned int a = __shfl_up_sync(0xffffffffu, ci, o);
-          const unsigned long long b = __shfl_up_sync(0xffffffffu, mi, o);
-          if (lane >= o) { ci += a; mi += b; }
+          const double y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
         }
-        if (lane == 31) { s.wcnt[warp] = ci; s.wmass[warp] = mi; }
+        __syncthreads();
+        if (lane == 31) s.wsum[warp] = incl;
+        __syncthreads();
+        double before = __shfl_up_sync(0xffffffffu, incl, 1);
+        if (lane == 0) before = 0.0;
+        all = 0.0;
+        for (int i = 0; i < NWARP; ++i) {
+          if (i < warp) before += s.wsum[i];
+          all += s.wsum[i];
+        }
+        return before;
+      };
+      sort(true);
+      double* weights = reinterpret_cast<double*>(s.lo);           // by place in the sorted list
+      const int i0 = 2 * tid, i1 = i0 + 1;
+      auto item = [&](int i) { return i < m && (top_k <= 0 || i < top_k) ? wt(static_cast<uint32_t>(s.list[i] >> 32)) : 0.0; };
+      const double w0 = item(i0), w1 = item(i1);
+      double all, kept_all;
+      const double before = scan(w0, w1, all);
+      const double limit = top_p < 1.f ? static_cast<double>(top_p) * all : INFINITY;
+      auto kept = [&](int i, double w, double b) {
+        return i < m && (top_k <= 0 || i < top_k) && (i == 0 || b < limit) && (w >= mp || static_cast<uint32_t>(s.list[i] >> 32) == top_key);
+      };
+      const bool k0 = kept(i0, w0, before), k1 = kept(i1, w1, before + w0);
+      const unsigned int at0 = k0 ? 0xffffffffu - static_cast<unsigned int>(s.list[i0]) : 0xffffffffu;
+      const unsigned int at1 = k1 ? 0xffffffffu - static_cast<unsigned int>(s.list[i1]) : 0xffffffffu;
+      __syncthreads();
+      if (i0 < size) {
+        weights[i0] = k0 ? w0 : 0.0;
+        weights[i1] = k1 ? w1 : 0.0;
+        s.list[i0] = (static_cast<unsigned long long>(at0) << 32) | i0;        // by index; what is not kept comes last
+        s.list[i1] = (static_cast<unsigned long long>(at1) << 32) | i1;
+      }
+      sort(false);
+      const double v0 = i0 < size ? weights[static_cast<uint32_t>(s.list[i0])] : 0.0, v1 = i0 < size ? weights[static_cast<uint32_t>(s.list[i1])] : 0.0;
+      const double run = scan(v0, v1, kept_all);
+      const double target = u * kept_all;
+      if (tid == 0) { s.u0 = 0xffffffffu; s.u1 = 0; }
+      __syncthreads();
+      if (v0 > 0.0) { if (run + v0 > target) atomicMin(&s.u0, i0); atomicMax(&s.u1, i0); }
+      if (v1 > 0.0) { if (run + v0 + v1 > target) atomicMin(&s.u0, i1); atomicMax(&s.u1, i1); }
+      __syncthreads();
+      if (tid == 0) {
+        const unsigned int pick = s.u0 != 0xffffffffu ? s.u0 : s.u1;
+        p.ids[row] = static_cast<long long>(s.list[pick] >> 32);
+        p.logprobs[row] = static_cast<float>(log(weights[static_cast<uint32_t>(s.list[pick])] / kept_all));
+      }
+    };
+    auto list_item = [&](uint32_t k, int i) {
+      Shared& first = peer(0);
+      const unsigned int at = atomicAdd(&first.listed, 1u);
+      if (at < LIST) first.list[at] = (static_cast<unsigned long long>(k) << 32) | (0xffffffffu - static_cast<unsigned int>(s_lo + i));
+    };
+    if (n_row <= LIST) {
+      for_each<T>(x, n, [&](uint32_t k, int i) { if (k > KEY_NONE) list_item(k, i); });
+      sync();
+      if (rank == 0) draw_listed();
+      sync();
+      continue;
+    }
+    bool drawn = false;
+
+    for (int by_mass = 0; by_mass < 2 && !drawn; ++by_mass) {
+      if (by_mass ? !(top_p < 1.f) : !(top_k > 0 && top_k < n_row)) continue;
+      // Finds, from the top, the bin where the running sum reaches the target.  -> u2: found, u0: the bin, u1 / m0: what is above it
+      unsigned long long target = 0, above = 0, in_bin = 0, all = 0;
+      auto find_bin = [&](bool upwards) {
+        // the cluster's histogram, PB bins per thread in order from the highest score down
+        unsigned long long v[PB], mine = 0;
+#pragma unroll
+        for (int i = 0; i < PB; ++i) {
+          const int b = upwards ? tid * PB + i : BINS - 1 - (tid * PB + i);
+          v[i] = 0;
+          for (int r = 0; r < c; ++r) {
+            const Shared& o = peer(r);
+            v[i] += (static_cast<unsigned long long>(o.hi[b]) << 32) + o.lo[b];
+          }
+          mine += v[i];
+        }
+        unsigned long long incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        if (lane == 31) s.wmass[warp] = incl;
         if (tid == 0) s.u2 = 0;
         __syncthreads();
-        unsigned int cb = ci - c4, call = 0;
-        unsigned long long mb = mi - m4, mall = 0;
+        unsigned long long before = above + incl - mine;
+        all = 0;
         for (int i = 0; i < NWARP; ++i) {
-          if (i < warp) { cb += s.wcnt[i]; mb += s.wmass[i]; }
-          call += s.wcnt[i];
-          mall += s.wmass[i];
+          if (i < warp) before += s.wmass[i];
+          all += s.wmass[i];
         }
-        if (level == 0) {
+        if (!target) {
           if (by_mass) {
-            const double t = ceil(static_cast<double>(top_p) * static_cast<double>(mall));
+            const double t = ceil(static_cast<double>(top_p) * static_cast<double>(all));
             target = t > 1.0 ? static_cast<unsigned long long>(t) : 1ULL;     // at least the first item
           } else {
-            none = call <= static_cast<unsigned int>(top_k);                  // fewer items than k: all are kept
+            target = all <= static_cast<unsigned int>(top_k) ? ~0ULL : static_cast<unsigned long long>(top_k);
           }
         }
-        cb += c_before;
-        mb += m_before;
+#pragma unroll
         for (int i = 0; i < PB; ++i) {
-          const int b = BINS - 1 - (tid * PB + i);
-          const bool here = by_mass ? (mb < target && mb + s.mass[b] >= target)
-                                    : (cb < static_cast<unsigned int>(top_k) && cb + s.cnt[b] >= static_cast<unsigned int>(top_k));
-          if (here) { s.u0 = b; s.u1 = cb; s.m0 = mb; s.u2 = 1; }
-          cb += s.cnt[b];
-          mb += s.mass[b];
+          if (before < target && before + v[i] >= target) { s.u0 = upwards ? tid * PB + i : BINS - 1 - (tid * PB + i); s.m0 = before; s.m1 = v[i]; s.u2 = 1; }
+          before += v[i];
         }
         __syncthreads();
-        if (!s.u2) none = true;
-        if (!none) {
-          prefix = (prefix << width) | s.u0;
-          bits += width;
-          c_before = s.u1;
-          m_before = s.m0;
-        }
+        if (s.u2) { above = s.m0; in_bin = s.m1; }
+        return s.u2 ? static_cast<int>(s.u0) : -1;
+      };
+      auto clear = [&]() {
+        for (int i = tid; i < BINS; i += NT) { s.lo[i] = 0; s.hi[i] = 0; }
+        if (tid == 0) { s.key_min = 0xffffffffu; s.key_max = 0; }
         __syncthreads();
+      };
+      auto add = [&](int bin, uint32_t k) {
+        if (by_mass) add64(s, bin, wt.fixed(k, shift_fx)); else atomicAdd(&s.lo[bin], 1u);
+      };
+      // items equal to an earlier cut count as many times as they are kept: one thread adds them
+      const bool lump = by_mass && cut.ties && rank == 0 && tid == 0;
+      sync();                                                      // earlier histograms have been read
+      clear();
+      for_each<T>(x, n, [&](uint32_t k, int) { if (k > cut.key) add(bin_of(k), k); });
+      if (lump) add64(s, bin_of(cut.key), cut.ties * wt.fixed(cut.key, shift_fx));
+      sync();
+      const int bin = find_bin(true);
+      if (bin < 0) continue;                                       // fewer items than k
+      if (!by_mass && above + in_bin <= LIST) {                    // all that can be kept fits the list
+        for_each<T>(x, n, [&](uint32_t k, int i) { if (k > KEY_NONE && bin_of(k) <= bin) list_item(k, i); });
+        sync();
+        if (rank == 0) draw_listed();
+        drawn = true;
+        break;
       }
-      if (none) continue;
+      // the keys in that bin (set aside while they are few), then a descent over their range
+      uint32_t k_min = 0xffffffffu, k_max = 0;
+      if (tid == 0) s.listed = 0;
+      __syncthreads();
+      for_each<T>(x, n, [&](uint32_t k, int) {
+        if (k > cut.key && bin_of(k) == bin) {
+          k_min = min(k_min, k);
+          k_max = max(k_max, k);
+          const unsigned int at = atomicAdd(&s.listed, 1u);
+          if (at < LIST) s.list[at] = k;
+        }
+      });
+      if (lump && bin_of(cut.key) == bin) { k_min = min(k_min, cut.key); k_max = max(k_max, cut.key); }
+      k_min = __reduce_min_sync(0xffffffffu, k_min);
+      k_max = __reduce_max_sync(0xffffffffu, k_max);
+      if (lane == 0 && k_min <= k_max) { atomicMin(&s.key_min, k_min); atomicMax(&s.key_max, k_max); }
+      sync();
+      const int aside = static_cast<int>(s.listed);
+      for (int r = 0; r < c; ++r) { k_min = min(k_min, peer(r).key_min); k_max = max(k_max, peer(r).key_max); }
+      while (k_min < k_max) {
+        const int down = max(0, 32 - __clz(k_max - k_min) - 11);   // (k_max - k_min) >> down < 2^11
+        sync();
+        clear();
+        if (aside <= LIST) {
+          for (int i = tid; i < aside; i += NT) {
+            const uint32_t k = static_cast<uint32_t>(s.list[i]);
+            if (k >= k_min && k <= k_max) add((k - k_min) >> down, k);
+          }
+        } else {
+          for_each<T>(x, n, [&](uint32_t k, int) {
+            if (k > cut.key && k >= k_min && k <= k_max && bin_of(k) == bin) add((k - k_min) >> down, k);
+          });
+        }
+        if (lump && cut.key >= k_min && cut.key <= k_max && bin_of(cut.key) == bin)
+          add64(s, (cut.key - k_min) >> down, cut.ties * wt.fixed(cut.key, shift_fx));
+        sync();
+        const int b = find_bin(false);
+        if (b < 0) break;                                          // (cannot be: the sum is reached in this range)
+        k_min += static_cast<uint32_t>(b) << down;
+        k_max = min(k_max, k_min + ((1u << down) - 1u));
+      }
       if (by_mass) {
-        const unsigned long long w = static_cast<unsigned long long>(wt(prefix) * fx + 0.5);
-        const unsigned long long r = w ? (target - m_before + w - 1) / w : 0xffffffffULL;
-        const unsigned int most = prefix == cut.key ? cut.ties : 0xffffffffu;
+        const unsigned long long w = wt.fixed(k_min, shift_fx);
+        const unsigned long long r = w ? (target - above + w - 1) / w : 0xffffffffULL;
+        const unsigned int most = k_min == cut.key ? cut.ties : 0xffffffffu;
         cut.ties = static_cast<unsigned int>(min(r, static_cast<unsigned long long>(most)));
       } else {
-        cut.ties = static_cast<unsigned int>(top_k) - c_before;
+        cut.ties = static_cast<unsigned int>(target - above);
       }
-      cut.key = prefix;
+      cut.key = k_min;
     }
-    // ---- draw: split the range among the warps, find the one where the running sum passes u * total, repeat inside it
-    const double mp = static_cast<double>(min_p);
+
+    if (drawn) {
+      sync();
+      continue;
+    }
+    // ---- draw: which CTA, which warp, ... holds the item where the running sum passes u * total
+    // min-p as a key: the smallest one with enough weight, by 32 tries at a time
+    uint32_t lim = cut.key;                                        // kept: keys above it, and the cut's ties
+    if (mp > 0.0) {
+      uint32_t below = KEY_NONE, enough = top_key;                 // w(below) < mp <= w(enough)
+      while (enough - below > 1) {
+        const uint32_t step = (enough - below - 1) / 32 + 1, k = below + step * (lane + 1);
+        const unsigned int yes = __ballot_sync(0xffffffffu, k < enough && k > below && wt(k) >= mp);
+        const uint32_t tried = (enough - below - 1) / step;        // tries below `enough`; from the f-th on they have enough weight
+        const uint32_t f = yes ? __ffs(yes) - 1 : tried;
+        if (yes) enough = below + step * (f + 1);
+        below += step * f;
+      }
+      lim = max(lim, enough - 1);
+    }
     const double w_tie = cut.ties ? wt(cut.key) : 0.0;
-    const bool tie_ok = w_tie >= mp || cut.key == top_key;
-    auto weight = [&](uint32_t k) -> double {
-      if (k <= cut.key) return 0.0;
-      const double w = wt(k);
-      return w >= mp || k == top_key ? w : 0.0;
-    };
-    int a = 0, len = n;
-    unsigned int ties_left = tie_ok ? cut.ties : 0u;
-    double target = 0.0, total = 0.0;
-    bool first = true;
-    while (first || len > 32) {
-      const int seg = ((len + NWARP - 1) / NWARP + 31) / 32 * 32;
+    const unsigned int ties_kept = cut.ties && (w_tie >= mp || cut.key == top_key) ? cut.ties : 0u;
+    // sums of the warps' segments of [a, a + len): kept keys are queued so that every lane of the 64-bit arithmetic has one
+    auto segments = [&](int a, int len, int seg) {
       double sum = 0.0;
-      unsigned int ties = 0;
+      unsigned int ties = 0, queued = 0;
+      unsigned int* q = s.queue[warp];
       const int b0 = a + warp * seg, b1 = min(b0 + seg, a + len);
-      for (int i = b0 + lane; i < b1; i += 32) {
-        const uint32_t k = key_of(to_f<T>(x[i]));
-        sum += weight(k);
-        ties += k == cut.key;
+      for (int i = b0; i < b1; i += 32) {
+        const uint32_t k = i + lane < b1 ? key_of(to_f<T>(x[i + lane])) : 0u;
+        ties += k == cut.key && i + lane < b1;
+        const bool keep = k > lim;
+        const unsigned int keeps = __ballot_sync(0xffffffffu, keep);
+        if (keep) q[queued + __popc(keeps & ((1u << lane) - 1))] = k;
+        queued += __popc(keeps);
+        if (queued >= 32) {
+          __syncwarp();
+          sum += wt(q[lane]);
+          const unsigned int rest = lane + 32 < queued ? q[lane + 32] : 0u;
+          queued -= 32;
+          __syncwarp();
+          if (lane < queued) q[lane] = rest;
+        }
       }
+      __syncwarp();
+      if (lane < queued) sum += wt(q[lane]);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        ties += __shfl_xor_sync(0xffffffffu, ties, o);
-      }
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      ties = __reduce_add_sync(0xffffffffu, ties);
       __syncthreads();
       if (lane == 0) { s.wsum[warp] = sum; s.wcnt[warp] = ties; }
       __syncthreads();
-      // every thread walks the 16 sums alike
-      if (first) {
-        unsigned int left = ties_left;
-        for (int i = 0; i < NWARP; ++i) {
-          const unsigned int t = min(s.wcnt[i], left);
-          total += s.wsum[i] + t * w_tie;
-          left -= t;
-        }
-        target = u * total;
-        first = false;
+    };
+    int a = 0, len = n, seg = ((n + NWARP - 1) / NWARP + 31) / 32 * 32;
+    segments(a, len, seg);
+    if (tid == 0) {
+      double sum = 0.0;
+      unsigned int ties = 0;
+      for (int i = 0; i < NWARP; ++i) { sum += s.wsum[i]; ties += s.wcnt[i]; }
+      s.sum = sum;
+      s.ties = ties;
+    }
+    sync();
+    double total = 0.0, before = 0.0, target;
+    unsigned int ties_left = ties_kept;
+    int owner = -1;
+    {
+      unsigned int left = ties_kept;
+      for (int r = 0; r < c; ++r) {
+        const unsigned int t = min(peer(r).ties, left);
+        total += peer(r).sum + t * w_tie;
+        left -= t;
       }
-      double run = 0.0, pick_run = 0.0;
-      unsigned int left = ties_left, pick_left = 0;
-      int pick = -1;
-      for (int i = 0; i < NWARP; ++i) {
-        const unsigned int t = min(s.wcnt[i], left);
-        const double m = s.wsum[i] + t * w_tie;
+      target = u * total;
+      double run = 0.0;
+      left = ties_kept;
+      for (int r = 0; r < c; ++r) {
+        const unsigned int t = min(peer(r).ties, left);
+        const double m = peer(r).sum + t * w_tie;
         if (m > 0.0) {                                             // the last one with any weight, if rounding leaves none
-          pick = i; pick_run = run; pick_left = left;
+          owner = r; before = run; ties_left = left;
           if (run + m > target) break;
         }
         run += m;
         left -= t;
       }
-      if (pick < 0) pick = 0;
-      target -= pick_run;
-      ties_left = pick_left;
-      len = min(seg, a + len - (a + pick * seg));
-      a += pick * seg;
     }
-    if (warp == 0) {
-      const int i = a + lane;
-      const uint32_t k = lane < len ? key_of(to_f<T>(x[i])) : 0u;
-      const bool tie = lane < len && k == cut.key;
-      const unsigned int tied = __ballot_sync(0xffffffffu, tie);
-      double w = lane < len ? weight(k) : 0.0;
-      if (tie && __popc(tied & ((1u << lane) - 1)) < static_cast<int>(min(ties_left, 32u))) w = w_tie;
-      double run = w;
+    if (rank == owner) {
+      target -= before;
+      for (;;) {
+        // every thread walks the 16 sums alike
+        double run = 0.0, pick_run = 0.0;
+        unsigned int left = ties_left, pick_left = 0;
+        int pick = 0;
+        for (int i = 0; i < NWARP; ++i) {
+          const unsigned int t = min(s.wcnt[i], left);
+          const double m = s.wsum[i] + t * w_tie;
+          if (m > 0.0) {
+            pick = i; pick_run = run; pick_left = left;
+            if (run + m > target) break;
+          }
+          run += m;
+          left -= t;
+        }
+        target -= pick_run;
+        ties_left = pick_left;
+        len = min(seg, len - pick * seg);
+        a += pick * seg;
+        if (len <= 32) break;
+        seg = ((len + NWARP - 1) / NWARP + 31) / 32 * 32;
+        segments(a, len, seg);
+      }
+      if (warp == 0) {
+        const uint32_t k = lane < len ? key_of(to_f<T>(x[a + lane])) : 0u;
+        const bool tie = lane < len && k == cut.key;
+        const unsigned int tied = __ballot_sync(0xffffffffu, tie);
+        double w = lane < len && k > lim ? wt(k) : 0.0;
+        if (tie && __popc(tied & ((1u << lane) - 1)) < static_cast<int>(min(ties_left, 32u))) w = w_tie;
+        double run = w;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double v = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += v;
-      }
-      const unsigned int over = __ballot_sync(0xffffffffu, w > 0.0 && run > target), any = __ballot_sync(0xffffffffu, w > 0.0);
-      const int pick = over ? __ffs(over) - 1 : 31 - __clz(any);
-      if (lane == pick) {
-        p.ids[row] = i;
-        p.logprobs[row] = static_cast<float>(log(w / total));
+        for (int o = 1; o < 32; o <<= 1) {
+          const double v = __shfl_up_sync(0xffffffffu, run, o);
+          if (lane >= o) run += v;
+        }
+        const unsigned int over = __ballot_sync(0xffffffffu, w > 0.0 && run > target), any = __ballot_sync(0xffffffffu, w > 0.0);
+        const int pick = over ? __ffs(over) - 1 : 31 - __clz(any);
+        if (lane == pick) {
+          p.ids[row] = s_lo + a + lane;
+          p.logprobs[row] = static_cast<float>(log(w / total));
+        }
       }
     }
+    sync();                                                        // nobody's words are still being read
   }
+}
+
+template <typename T>
+int launch(SampleArgs p, int num_sms, cudaStream_t st) {
+  constexpr int fixed_bytes = (sizeof(Shared) + 15) / 16 * 16 + 16;
+  constexpr int max_bytes = 227 * 1024;
+  constexpr int half_bytes = 113 * 1024;                           // two CTAs per SM
+  // The most a row can have (of jagged rows: all but never, so assume twice the average).
+  long long longest = p.width;
+  if (p.offsets) longest = min(p.width, 2 * p.width / p.rows + 1024);
+  // CTAs per row: enough to hold it in shared memory at two CTAs per SM, and more while SMs would stay idle and a CTA keeps
+  // some thousand items
+  int c = 1;
+  while (c < MAX_CLUSTER && (longest + c - 1) / c * static_cast<long long>(sizeof(T)) + fixed_bytes > half_bytes) c *= 2;
+  while (c < MAX_CLUSTER && 2LL * c * p.rows <= num_sms && longest / c > 4096) c *= 2;
+  const long long slice = (((longest + c - 1) / c + 31) / 32 * 32) * static_cast<long long>(sizeof(T));
+  const long long room = slice + fixed_bytes <= half_bytes ? slice : min(slice, static_cast<long long>(max_bytes - fixed_bytes));
+  p.cap = static_cast<int>(room / sizeof(T));
+  const int bytes = fixed_bytes + static_cast<int>(room);
+  RB_CUDA_CHECK(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(c) * static_cast<unsigned>(min(p.rows, 65536)));
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = c; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, sample_kernel<T>, p));
 }
 
 }  // namespace
@@ -298,18 +609,17 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleArgs p) {
 RB_API int rb_sample_scores(const void* scores, long long ld, const void* offsets, int offsets64, long long width, int rows,
                             const float* uniform, const float* temperature, const int* top_k, const float* top_p,
                             const float* min_p, float temperature_v, int top_k_v, float top_p_v, float min_p_v, long long* ids,
-                            float* logprobs, int dtype, cudaStream_t st) {
+                            float* logprobs, int dtype, int num_sms, cudaStream_t st) {
   if (rows == 0) return 0;
-  if (width > 0x7fffffffLL) return -1;
+  if (width > 0x7fffffffLL - 64) return -1;
   SampleArgs p;
-  p.scores = scores; p.ld = ld; p.offsets = offsets; p.offsets64 = offsets64; p.width = width; p.rows = rows;
+  p.scores = scores; p.ld = ld; p.offsets = offsets; p.offsets64 = offsets64; p.width = width; p.rows = rows; p.cap = 0;
   p.uniform = uniform; p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
   p.temperature_v = temperature_v; p.top_k_v = top_k_v; p.top_p_v = top_p_v; p.min_p_v = min_p_v;
   p.ids = ids; p.logprobs = logprobs;
-  const int grid = rows < 65536 ? rows : 65536;
-  if (dtype == 0) sample_kernel<float><<<grid, NT, 0, st>>>(p);
-  else if (dtype == 1) sample_kernel<__half><<<grid, NT, 0, st>>>(p);
-  else if (dtype == 2) sample_kernel<__nv_bfloat16><<<grid, NT, 0, st>>>(p);
-  else return -2;
-  return static_cast<int>(cudaGetLastError());
+  const int sms = num_sms > 0 ? num_sms : 148;
+  if (dtype == 0) return launch<float>(p, sms, st);
+  if (dtype == 1) return launch<__half>(p, sms, st);
+  if (dtype == 2) return launch<__nv_bfloat16>(p, sms, st);
+  return -2;
 }

@@ -59,8 +59,8 @@ def sample_scores(scores: torch.Tensor, uniform: torch.Tensor, offsets: Optional
         raise ValueError("uniform must be [%d] fp32 on %s" % (rows, dev))
     if scores.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise ValueError("scores must be fp32, fp16 or bf16, got %s" % (scores.dtype,))
-    if width >= 1 << 31:
-        raise ValueError("rows of 2^31 and more scores are not supported")
+    if width > (1 << 31) - 65:
+        raise ValueError("2^31 - 64 and more scores in a row (or in all jagged rows) are not supported")
     big = torch.finfo(torch.float32).max
     t_t, t_v = _param("temperature", temperature, rows, torch.float32, dev, 0.0, big)
     k_t, k_v = _param("top_k", top_k, rows, torch.int32, dev, 0, (1 << 31) - 1)
@@ -80,7 +80,7 @@ def sample_scores(scores: torch.Tensor, uniform: torch.Tensor, offsets: Optional
                                          int(offsets is not None and offsets.dtype == torch.int64), width, rows,
                                          uniform.data_ptr(), _lib.ptr(t_t), _lib.ptr(k_t), _lib.ptr(p_t), _lib.ptr(m_t),
                                          float(t_v), int(k_v), float(p_v), float(m_v), ids.data_ptr(), logprobs.data_ptr(),
-                                         _lib.dtype_code(scores.dtype), _lib.stream_ptr(dev))
+                                         _lib.dtype_code(scores.dtype), _lib.num_sms(dev), _lib.stream_ptr(dev))
         _lib.check(rc, "rb_sample_scores")
     return ids, logprobs
 
