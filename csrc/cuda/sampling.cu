@@ -11,8 +11,8 @@
 //
 // Weights are computed and summed in 64 bits: with N kept items each of the N borders can go either way with the sums'
 // relative error as its chance, and 32-bit exponentials (1e-7 each) would draw a neighbour in every hundredth row of 10^5
-// items.  The exponential is table-driven (Tang, ACM TOMS 15, 1989): 2^(n/64) from a table, 2^(f/64) as a polynomial of
-// degree 4 (relative error below 4e-14).  Sums inside the histograms are whole numbers (2^-44 of the largest weight for
+// items.  The exponential is table-driven (Tang, ACM TOMS 15, 1989): 2^(n/256) from a table, 2^(f/256), |f| <= 1/2, as a
+// polynomial of degree 3 (relative error (ln2/512)^4 / 24 = 1.4e-13).  Sums inside the histograms are whole numbers (2^-44 of the largest weight for
 // rows up to 2^18 items, coarser beyond), so atomics in any order give the same bits.
 //
 // Bound: the row is read from memory once, into the shared memory of a cluster of CTAs (1 to 8 by its size and by how many
@@ -29,6 +29,7 @@ namespace cg = cooperative_groups;
 constexpr int NT = 512, NWARP = NT / 32;
 constexpr int BINS = 2048, PB = BINS / NT;
 constexpr int MAX_CLUSTER = 8;
+constexpr int TABLE = 256;
 constexpr int LIST = 1024;                      // items that are sorted, or kept aside for a descent
 
 struct SampleArgs {
@@ -57,9 +58,9 @@ __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k
 constexpr uint32_t KEY_NONE = 0x007fffffu;                         // -inf: never drawn
 
 // What the CTAs of a cluster read of one another
-struct Shared {
+struct __align__(16) Shared {
   unsigned int lo[BINS], hi[BINS];              // 64-bit sums (or counts, in lo) by bin
-  double table[64];                             // 2^(j / 64)
+  double table[TABLE];                          // 2^(j / TABLE)
   unsigned int best, first;                     // largest key of the slice; its first index (where that is all that is asked)
   unsigned long long list[LIST];                // (key, ~index) of the items that can be kept, or keys in the cut's bin
   unsigned int listed;
@@ -69,7 +70,7 @@ struct Shared {
   double wsum[NWARP];
   unsigned int wcnt[NWARP];
   unsigned long long wmass[NWARP];
-  unsigned int queue[NWARP][64];
+  float queue[NWARP][64];
   unsigned int u0, u1, u2;
   unsigned long long m0, m1;
 };
@@ -77,23 +78,23 @@ struct Shared {
 // exp((x - top) / T), 64 bits
 struct Weigher {
   const double* table;
-  double top, scale;                            // scale = 64 log2(e) / T
-  uint32_t top_key;
-  // with its binary exponent raised by `up`
-  __device__ __forceinline__ double operator()(uint32_t k, int up = 0) const {
-    const double t = k == top_key ? 0.0 : (static_cast<double>(value_of(k)) - top) * scale;
-    if (!(t > -65000.0)) return 0.0;
+  double scale;                                 // 1/256 octaves per unit of score
+  float top;
+  // with its binary exponent raised by `up`; x is not NaN and at most top
+  __device__ __forceinline__ double operator()(float x, int up = 0) const {
+    const double t = x == top ? 0.0 : (static_cast<double>(x) - static_cast<double>(top)) * scale;
     const double magic = 6755399441055744.0;                       // 1.5 * 2^52: the sum's low word is the nearest whole number
     const double nd = t + magic;
     const int n = __double2loint(nd);
     const double f = t - (nd - magic);
-    constexpr double c1 = 0.6931471805599453 / 64, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4;
-    const double q = fma(fma(fma(fma(c4, f, c3), f, c2), f, c1), f, 1.0) * table[n & 63];
-    return __hiloint2double(__double2hiint(q) + (((n >> 6) + up) << 20), __double2loint(q));
+    constexpr double c1 = 0.6931471805599453 / TABLE, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3;
+    const double q = fma(fma(fma(c3, f, c2), f, c1), f, 1.0) * table[n & (TABLE - 1)];
+    const double w = __hiloint2double(__double2hiint(q) + (((n >> 8) + up) << 20), __double2loint(q));
+    return t > -260000.0 ? w : 0.0;                                // (2^-1015; also for -inf)
   }
-  // the weight in units of 2^-shift, rounded (shift <= 44)
-  __device__ __forceinline__ unsigned long long fixed(uint32_t k, int shift) const {
-    const double w = (*this)(k, shift) + 4503599627370496.0;       // + 2^52
+  // the weight in units of 2^-shift, rounded (up <= 44)
+  __device__ __forceinline__ unsigned long long fixed(float x, int up) const {
+    const double w = (*this)(x, up) + 4503599627370496.0;          // + 2^52
     return static_cast<unsigned long long>(__double_as_longlong(w)) & 0xfffffffffffffULL;
   }
 };
@@ -108,21 +109,28 @@ __device__ __forceinline__ void add64(Shared& s, int bin, unsigned long long v) 
   if (hi) atomicAdd(&s.hi[bin], hi);
 }
 
-// f(key, index in the slice) for all of a slice, 16 bytes at a time where its address allows
+// f(scores, how many, index of the first in the slice) for all of a slice, 16 bytes at a time where its address allows
 template <typename T, typename F>
 __device__ __forceinline__ void for_each(const T* x, int n, F&& f) {
   constexpr int V = 16 / sizeof(T);
   const int head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T)));
-  for (int i = threadIdx.x; i < head; i += NT) f(key_of(to_f<T>(x[i])), i);
   const int nv = (n - head) / V;
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   for (int i = threadIdx.x; i < nv; i += NT) {
     const uint4 u = xv[i];
     const T* e = reinterpret_cast<const T*>(&u);
+    float v[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) f(key_of(to_f<T>(e[j])), head + i * V + j);
+    for (int j = 0; j < V; ++j) v[j] = to_f<T>(e[j]);
+    f(v, head + i * V);
   }
-  for (int i = head + nv * V + threadIdx.x; i < n; i += NT) f(key_of(to_f<T>(x[i])), i);
+  // the ends, one by one
+  const int ends = n - nv * V;
+  if (static_cast<int>(threadIdx.x) < ends) {
+    const int i = static_cast<int>(threadIdx.x) < head ? threadIdx.x : nv * V + threadIdx.x;
+    float v[1] = {to_f<T>(x[i])};
+    f(v, i);
+  }
 }
 
 template <typename T>
@@ -133,7 +141,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   cg::cluster_group cluster = cg::this_cluster();
   const int c = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid < 64) s.table[tid] = exp2(tid / 64.0);
+  for (int i = tid; i < TABLE; i += NT) s.table[i] = exp2(i / static_cast<double>(TABLE));
   auto sync = [&]() { if (c > 1) cluster.sync(); else __syncthreads(); };
   auto peer = [&](int r) -> Shared& { return c > 1 ? *cluster.map_shared_rank(&s, r) : s; };
 
@@ -183,7 +191,9 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       for (int i = head + nv * V + tid; i < n; i += NT) { y[i] = x[i]; most = fmaxf(most, to_f<T>(x[i])); }
       x = y;
     } else {
-      for_each<T>(x, n, [&](uint32_t k, int) { most = fmaxf(most, value_of(k)); });
+      for_each<T>(x, n, [&](auto& v, int) {
+        for (float e : v) most = fmaxf(most, e);
+      });
     }
     uint32_t top_key = __reduce_max_sync(0xffffffffu, key_of(most));
     if (lane == 0) s.wcnt[warp] = top_key;
@@ -202,7 +212,13 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     }
     if (!(temp > 0.f)) {
       unsigned int at = 0xffffffffu;
-      for_each<T>(x, n, [&](uint32_t k, int i) { if (k == top_key) at = min(at, static_cast<unsigned int>(s_lo + i)); });
+      const float top_f = value_of(top_key);
+      for_each<T>(x, n, [&](auto& v, int i) {
+        for (float e : v) {
+          if (e == top_f) at = min(at, static_cast<unsigned int>(s_lo + i));
+          ++i;
+        }
+      });
       at = __reduce_min_sync(0xffffffffu, at);
       if (lane == 0 && at != 0xffffffffu) atomicMin(&peer(0).first, at);
       sync();
@@ -210,13 +226,17 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       sync();
       continue;
     }
+    const float top_f = value_of(top_key);
     Weigher wt;
-    wt.table = s.table; wt.top = static_cast<double>(value_of(top_key)); wt.top_key = top_key;
-    wt.scale = 64.0 * 1.4426950408889634 / static_cast<double>(temp);
+    wt.table = s.table; wt.top = top_f;
+    wt.scale = TABLE * 1.4426950408889634 / static_cast<double>(temp);
+    auto wk = [&](uint32_t k) { return wt(value_of(k)); };
     Cut cut = {KEY_NONE, 0};
-    // bins of 1/64 octave of the weight, the last one open: monotone in the score, in 32 bits
-    const float top_f = value_of(top_key), bin_scale = 64.f * 1.44269504f / temp;
-    auto bin_of = [&](uint32_t k) { return static_cast<int>(fminf((top_f - value_of(k)) * bin_scale, BINS - 1.f)); };   // (NaN: inf - inf -> last)
+    float cut_f = -INFINITY;                                       // its value
+    // bins of 1/64 octave of the weight, the last one open: all that matters is that they are monotone in the score
+    const float bin_scale = 64.f * 1.44269504f / temp, bin_shift = top_f * bin_scale;
+    auto place_of = [&](float x) { return fmaxf(fminf(fmaf(x, -bin_scale, bin_shift), BINS - 1.f), 0.f); };
+    auto bin_of = [&](float x) { return static_cast<int>(place_of(x)); };
     const int shift_fx = 62 - max(18, 32 - __clz(n_row));
     const double mp = static_cast<double>(min_p);
 
@@ -261,7 +281,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       sort(true);
       double* weights = reinterpret_cast<double*>(s.lo);           // by place in the sorted list
       const int i0 = 2 * tid, i1 = i0 + 1;
-      auto item = [&](int i) { return i < m && (top_k <= 0 || i < top_k) ? wt(static_cast<uint32_t>(s.list[i] >> 32)) : 0.0; };
+      auto item = [&](int i) { return i < m && (top_k <= 0 || i < top_k) ? wk(static_cast<uint32_t>(s.list[i] >> 32)) : 0.0; };
       const double w0 = item(i0), w1 = item(i1);
       double all, kept_all;
       const double before = scan(w0, w1, all);
@@ -300,7 +320,12 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       if (at < LIST) first.list[at] = (static_cast<unsigned long long>(k) << 32) | (0xffffffffu - static_cast<unsigned int>(s_lo + i));
     };
     if (n_row <= LIST) {
-      for_each<T>(x, n, [&](uint32_t k, int i) { if (k > KEY_NONE) list_item(k, i); });
+      for_each<T>(x, n, [&](auto& v, int i) {
+        for (float e : v) {
+          if (e > -INFINITY) list_item(key_of(e), i);
+          ++i;
+        }
+      });
       sync();
       if (rank == 0) draw_listed();
       sync();
@@ -314,17 +339,27 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       unsigned long long target = 0, above = 0, in_bin = 0, all = 0;
       auto find_bin = [&](bool upwards) {
         // the cluster's histogram, PB bins per thread in order from the highest score down
-        unsigned long long v[PB], mine = 0;
+        static_assert(PB == 4, "a thread's bins are one vector");
+        unsigned long long v[PB] = {0, 0, 0, 0}, mine = 0;
+        const int at = upwards ? tid : BINS / PB - 1 - tid;
+        auto add4 = [&](const uint4& l, const uint4& h) {
+          const uint32_t ls[4] = {l.x, l.y, l.z, l.w}, hs[4] = {h.x, h.y, h.z, h.w};
 #pragma unroll
-        for (int i = 0; i < PB; ++i) {
-          const int b = upwards ? tid * PB + i : BINS - 1 - (tid * PB + i);
-          v[i] = 0;
-          for (int r = 0; r < c; ++r) {
-            const Shared& o = peer(r);
-            v[i] += (static_cast<unsigned long long>(o.hi[b]) << 32) + o.lo[b];
-          }
-          mine += v[i];
+          for (int i = 0; i < 4; ++i) v[i] += (static_cast<unsigned long long>(hs[i]) << 32) + ls[i];
+        };
+        for (int r = 0; r < c; r += 2) {                           // two peers' loads in flight
+          const Shared& a = peer(r);
+          const Shared& b = peer(min(r + 1, c - 1));
+          const uint4 la = reinterpret_cast<const uint4*>(a.lo)[at], ha = reinterpret_cast<const uint4*>(a.hi)[at];
+          const uint4 lb = reinterpret_cast<const uint4*>(b.lo)[at], hb = reinterpret_cast<const uint4*>(b.hi)[at];
+          add4(la, ha);
+          if (r + 1 < c) add4(lb, hb);
         }
+        if (!upwards) {
+          unsigned long long y = v[0]; v[0] = v[3]; v[3] = y;
+          y = v[1]; v[1] = v[2]; v[2] = y;
+        }
+        mine = v[0] + v[1] + v[2] + v[3];
         unsigned long long incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -362,20 +397,38 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
         if (tid == 0) { s.key_min = 0xffffffffu; s.key_max = 0; }
         __syncthreads();
       };
-      auto add = [&](int bin, uint32_t k) {
-        if (by_mass) add64(s, bin, wt.fixed(k, shift_fx)); else atomicAdd(&s.lo[bin], 1u);
+      auto add = [&](int bin, float e) {
+        if (by_mass) add64(s, bin, wt.fixed(e, shift_fx)); else atomicAdd(&s.lo[bin], 1u);
       };
       // items equal to an earlier cut count as many times as they are kept: one thread adds them
       const bool lump = by_mass && cut.ties && rank == 0 && tid == 0;
       sync();                                                      // earlier histograms have been read
       clear();
-      for_each<T>(x, n, [&](uint32_t k, int) { if (k > cut.key) add(bin_of(k), k); });
-      if (lump) add64(s, bin_of(cut.key), cut.ties * wt.fixed(cut.key, shift_fx));
+      if (by_mass) {
+        for_each<T>(x, n, [&](auto& v, int) {
+          constexpr int N = sizeof(v) / sizeof(float);
+          unsigned long long w[N];                                 // all the arithmetic before the first atomic
+#pragma unroll
+          for (int j = 0; j < N; ++j) w[j] = wt.fixed(v[j], shift_fx);
+#pragma unroll
+          for (int j = 0; j < N; ++j) if (v[j] > cut_f) add64(s, bin_of(v[j]), w[j]);
+        });
+      } else {
+        for_each<T>(x, n, [&](auto& v, int) {
+          for (float e : v) if (e > cut_f) atomicAdd(&s.lo[bin_of(e)], 1u);
+        });
+      }
+      if (lump) add64(s, bin_of(cut_f), cut.ties * wt.fixed(cut_f, shift_fx));
       sync();
       const int bin = find_bin(true);
       if (bin < 0) continue;                                       // fewer items than k
       if (!by_mass && above + in_bin <= LIST) {                    // all that can be kept fits the list
-        for_each<T>(x, n, [&](uint32_t k, int i) { if (k > KEY_NONE && bin_of(k) <= bin) list_item(k, i); });
+        for_each<T>(x, n, [&](auto& v, int i) {
+          for (float e : v) {
+            if (e > -INFINITY && bin_of(e) <= bin) list_item(key_of(e), i);
+            ++i;
+          }
+        });
         sync();
         if (rank == 0) draw_listed();
         drawn = true;
@@ -383,39 +436,50 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       }
       // the keys in that bin (set aside while they are few), then a descent over their range
       uint32_t k_min = 0xffffffffu, k_max = 0;
+      uint32_t* aside = reinterpret_cast<uint32_t*>(s.list);
       if (tid == 0) s.listed = 0;
       __syncthreads();
-      for_each<T>(x, n, [&](uint32_t k, int) {
-        if (k > cut.key && bin_of(k) == bin) {
-          k_min = min(k_min, k);
-          k_max = max(k_max, k);
-          const unsigned int at = atomicAdd(&s.listed, 1u);
-          if (at < LIST) s.list[at] = k;
-        }
+      auto in_this = [&](float e) {
+        const float at = place_of(e);
+        return e > cut_f && at >= bin && (at < bin + 1.f || bin == BINS - 1);
+      };
+      for_each<T>(x, n, [&](auto& v, int) {
+        for (float e : v)
+          if (in_this(e)) {
+            const uint32_t k = key_of(e);
+            k_min = min(k_min, k);
+            k_max = max(k_max, k);
+            const unsigned int at = atomicAdd(&s.listed, 1u);
+            if (at < 2 * LIST) aside[at] = k;
+          }
       });
-      if (lump && bin_of(cut.key) == bin) { k_min = min(k_min, cut.key); k_max = max(k_max, cut.key); }
+      if (lump && bin_of(cut_f) == bin) { k_min = min(k_min, cut.key); k_max = max(k_max, cut.key); }
       k_min = __reduce_min_sync(0xffffffffu, k_min);
       k_max = __reduce_max_sync(0xffffffffu, k_max);
       if (lane == 0 && k_min <= k_max) { atomicMin(&s.key_min, k_min); atomicMax(&s.key_max, k_max); }
       sync();
-      const int aside = static_cast<int>(s.listed);
+      const int n_aside = static_cast<int>(s.listed);
       for (int r = 0; r < c; ++r) { k_min = min(k_min, peer(r).key_min); k_max = max(k_max, peer(r).key_max); }
       while (k_min < k_max) {
         const int down = max(0, 32 - __clz(k_max - k_min) - 11);   // (k_max - k_min) >> down < 2^11
         sync();
         clear();
-        if (aside <= LIST) {
-          for (int i = tid; i < aside; i += NT) {
-            const uint32_t k = static_cast<uint32_t>(s.list[i]);
-            if (k >= k_min && k <= k_max) add((k - k_min) >> down, k);
+        if (n_aside <= 2 * LIST) {
+          for (int i = tid; i < n_aside; i += NT) {
+            const uint32_t k = aside[i];
+            if (k >= k_min && k <= k_max) add((k - k_min) >> down, value_of(k));
           }
         } else {
-          for_each<T>(x, n, [&](uint32_t k, int) {
-            if (k > cut.key && k >= k_min && k <= k_max && bin_of(k) == bin) add((k - k_min) >> down, k);
+          for_each<T>(x, n, [&](auto& v, int) {
+            for (float e : v) {
+              if (!in_this(e)) continue;
+              const uint32_t k = key_of(e);
+              if (k >= k_min && k <= k_max) add((k - k_min) >> down, e);
+            }
           });
         }
-        if (lump && cut.key >= k_min && cut.key <= k_max && bin_of(cut.key) == bin)
-          add64(s, (cut.key - k_min) >> down, cut.ties * wt.fixed(cut.key, shift_fx));
+        if (lump && cut.key >= k_min && cut.key <= k_max && bin_of(cut_f) == bin)
+          add64(s, (cut.key - k_min) >> down, cut.ties * wt.fixed(cut_f, shift_fx));
         sync();
         const int b = find_bin(false);
         if (b < 0) break;                                          // (cannot be: the sum is reached in this range)
@@ -423,7 +487,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
         k_max = min(k_max, k_min + ((1u << down) - 1u));
       }
       if (by_mass) {
-        const unsigned long long w = wt.fixed(k_min, shift_fx);
+        const unsigned long long w = wt.fixed(value_of(k_min), shift_fx);
         const unsigned long long r = w ? (target - above + w - 1) / w : 0xffffffffULL;
         const unsigned int most = k_min == cut.key ? cut.ties : 0xffffffffu;
         cut.ties = static_cast<unsigned int>(min(r, static_cast<unsigned long long>(most)));
@@ -431,6 +495,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
         cut.ties = static_cast<unsigned int>(target - above);
       }
       cut.key = k_min;
+      cut_f = value_of(k_min);
     }
 
     if (drawn) {
@@ -442,9 +507,15 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     uint32_t lim = cut.key;                                        // kept: keys above it, and the cut's ties
     if (mp > 0.0) {
       uint32_t below = KEY_NONE, enough = top_key;                 // w(below) < mp <= w(enough)
+      if (mp < 1.0 && !isinf(top_f)) {
+        // where it should be, give or take: a bracket that is checked before it is used
+        const float guess = top_f + temp * __logf(min_p), slack = 1e-3f * (fabsf(temp) + 1e-3f * fabsf(guess));
+        const float g0 = guess - slack, g1 = fminf(guess + slack, top_f);
+        if (g0 > -INFINITY && g0 < g1 && wt(g0) < mp && wt(g1) >= mp) { below = key_of(g0); enough = key_of(g1); }
+      }
       while (enough - below > 1) {
         const uint32_t step = (enough - below - 1) / 32 + 1, k = below + step * (lane + 1);
-        const unsigned int yes = __ballot_sync(0xffffffffu, k < enough && k > below && wt(k) >= mp);
+        const unsigned int yes = __ballot_sync(0xffffffffu, k < enough && k > below && wk(k) >= mp);
         const uint32_t tried = (enough - below - 1) / step;        // tries below `enough`; from the f-th on they have enough weight
         const uint32_t f = yes ? __ffs(yes) - 1 : tried;
         if (yes) enough = below + step * (f + 1);
@@ -452,29 +523,44 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       }
       lim = max(lim, enough - 1);
     }
-    const double w_tie = cut.ties ? wt(cut.key) : 0.0;
+    const double w_tie = cut.ties ? wt(cut_f) : 0.0;
     const unsigned int ties_kept = cut.ties && (w_tie >= mp || cut.key == top_key) ? cut.ties : 0u;
     // sums of the warps' segments of [a, a + len): kept keys are queued so that every lane of the 64-bit arithmetic has one
     auto segments = [&](int a, int len, int seg) {
       double sum = 0.0;
       unsigned int ties = 0, queued = 0;
-      unsigned int* q = s.queue[warp];
+      float* q = s.queue[warp];
       const int b0 = a + warp * seg, b1 = min(b0 + seg, a + len);
-      for (int i = b0; i < b1; i += 32) {
-        const uint32_t k = i + lane < b1 ? key_of(to_f<T>(x[i + lane])) : 0u;
-        ties += k == cut.key && i + lane < b1;
-        const bool keep = k > lim;
+      const float lim_f = value_of(lim);
+      auto take = [&](float e) {                                   // NaN for lanes without an item
+        ties += e == cut_f;
+        const bool keep = e > lim_f;
         const unsigned int keeps = __ballot_sync(0xffffffffu, keep);
-        if (keep) q[queued + __popc(keeps & ((1u << lane) - 1))] = k;
+        if (keep) q[queued + __popc(keeps & ((1u << lane) - 1))] = e;
         queued += __popc(keeps);
         if (queued >= 32) {
           __syncwarp();
           sum += wt(q[lane]);
-          const unsigned int rest = lane + 32 < queued ? q[lane + 32] : 0u;
+          const float rest = lane + 32 < queued ? q[lane + 32] : 0.f;
           queued -= 32;
           __syncwarp();
           if (lane < queued) q[lane] = rest;
         }
+      };
+      // any order does for a sum: lanes read vectors where the segment is aligned
+      constexpr int V = 16 / sizeof(T);
+      const int head = min(b1 - b0, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x + b0) & 15)) & 15) / static_cast<int>(sizeof(T)));
+      const int nv = b1 > b0 ? (b1 - b0 - head) / V : 0, tail = b0 + max(head, 0) + nv * V;
+      if (b1 > b0) {
+        take(lane < head ? to_f<T>(x[b0 + lane]) : NAN);
+        for (int i = 0; i < nv; i += 32) {
+          uint4 u = make_uint4(0, 0, 0, 0);
+          if (i + lane < nv) u = reinterpret_cast<const uint4*>(x + b0 + head)[i + lane];
+          const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+          for (int j = 0; j < V; ++j) take(i + lane < nv ? to_f<T>(e[j]) : NAN);
+        }
+        take(tail + lane < b1 ? to_f<T>(x[tail + lane]) : NAN);
       }
       __syncwarp();
       if (lane < queued) sum += wt(q[lane]);
@@ -548,7 +634,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
         const uint32_t k = lane < len ? key_of(to_f<T>(x[a + lane])) : 0u;
         const bool tie = lane < len && k == cut.key;
         const unsigned int tied = __ballot_sync(0xffffffffu, tie);
-        double w = lane < len && k > lim ? wt(k) : 0.0;
+        double w = lane < len && k > lim ? wk(k) : 0.0;
         if (tie && __popc(tied & ((1u << lane) - 1)) < static_cast<int>(min(ties_left, 32u))) w = w_tie;
         double run = w;
 #pragma unroll
