@@ -245,17 +245,31 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       const int m = static_cast<int>(s.listed);
       int size = 2;
       while (size < m) size *= 2;
-      for (int i = m + tid; i < size; i += NT) s.list[i] = 0;
-      auto sort = [&](bool descending) {
-        for (int k = 2; k <= size; k *= 2)
-          for (int j = k / 2; j > 0; j /= 2) {
-            __syncthreads();
-            for (int t = tid; t < size / 2; t += NT) {
-              const int i = 2 * t - (t & (j - 1)), l = i + j;
-              const unsigned long long a = s.list[i], b = s.list[l];
-              if (((a < b) == descending) == ((i & k) == 0) && a != b) { s.list[i] = b; s.list[l] = a; }
+      const int i0 = 2 * tid, i1 = i0 + 1;
+      // bitonic, two neighbouring items per thread: partners up to 32 apart are in the warp, others are met in the list
+      auto sort = [&](unsigned long long& v0, unsigned long long& v1, bool descending) {
+        for (int k = 2; k <= size; k *= 2) {
+          const bool down = ((i0 & k) == 0) == descending;         // the larger of a pair comes first
+          for (int j = k / 2; j > 1; j /= 2) {
+            unsigned long long q0, q1;
+            if (j >= 64) {
+              __syncthreads();
+              if (i0 < size) { s.list[i0] = v0; s.list[i1] = v1; }
+              __syncthreads();
+              q0 = s.list[(i0 ^ j) & (LIST - 1)];
+              q1 = s.list[(i1 ^ j) & (LIST - 1)];
+            } else {
+              q0 = __shfl_xor_sync(0xffffffffu, v0, j / 2);
+              q1 = __shfl_xor_sync(0xffffffffu, v1, j / 2);
             }
+            const bool larger = ((i0 & j) == 0) == down;
+            if ((q0 > v0) == larger) v0 = q0;
+            if ((q1 > v1) == larger) v1 = q1;
           }
+          if ((v1 > v0) == down) { const unsigned long long y = v0; v0 = v1; v1 = y; }
+        }
+        __syncthreads();
+        if (i0 < size) { s.list[i0] = v0; s.list[i1] = v1; }
         __syncthreads();
       };
       // running sums of two items per thread, in order -> sum before the first of them
@@ -278,9 +292,9 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
         }
         return before;
       };
-      sort(true);
+      unsigned long long e0 = i0 < m ? s.list[i0] : 0, e1 = i1 < m ? s.list[i1] : 0;
+      sort(e0, e1, true);
       double* weights = reinterpret_cast<double*>(s.lo);           // by place in the sorted list
-      const int i0 = 2 * tid, i1 = i0 + 1;
       auto item = [&](int i) { return i < m && (top_k <= 0 || i < top_k) ? wk(static_cast<uint32_t>(s.list[i] >> 32)) : 0.0; };
       const double w0 = item(i0), w1 = item(i1);
       double all, kept_all;
@@ -293,13 +307,10 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       const unsigned int at0 = k0 ? 0xffffffffu - static_cast<unsigned int>(s.list[i0]) : 0xffffffffu;
       const unsigned int at1 = k1 ? 0xffffffffu - static_cast<unsigned int>(s.list[i1]) : 0xffffffffu;
       __syncthreads();
-      if (i0 < size) {
-        weights[i0] = k0 ? w0 : 0.0;
-        weights[i1] = k1 ? w1 : 0.0;
-        s.list[i0] = (static_cast<unsigned long long>(at0) << 32) | i0;        // by index; what is not kept comes last
-        s.list[i1] = (static_cast<unsigned long long>(at1) << 32) | i1;
-      }
-      sort(false);
+      if (i0 < size) { weights[i0] = k0 ? w0 : 0.0; weights[i1] = k1 ? w1 : 0.0; }
+      e0 = (static_cast<unsigned long long>(at0) << 32) | i0;      // by index; what is not kept comes last
+      e1 = (static_cast<unsigned long long>(at1) << 32) | i1;
+      sort(e0, e1, false);
       const double v0 = i0 < size ? weights[static_cast<uint32_t>(s.list[i0])] : 0.0, v1 = i0 < size ? weights[static_cast<uint32_t>(s.list[i1])] : 0.0;
       const double run = scan(v0, v1, kept_all);
       const double target = u * kept_all;
