@@ -397,7 +397,8 @@ __global__ void __launch_bounds__(256) attn_merge_kernel(const Batch p, const Ou
   // tokens of requests in no group have no first part, tokens of no request neither
   const int t = static_cast<int>(row / p.H);
   const int* go = p.a.group_offsets;
-  const bool has_a = t >= p.a.q_offsets[min(max(go[0], 0), p.a.num_requests)] && t < p.a.q_offsets[min(max(go[p.a.B], 0), p.a.num_requests)];
+  const bool has_a = t >= p.a.q_offsets[go ? min(max(go[0], 0), p.a.num_requests) : 0] &&
+                     t < p.a.q_offsets[go ? min(max(go[p.a.B], 0), p.a.num_requests) : p.a.num_requests];
   const bool has_b = t >= p.b.q_offsets[0] && t < p.b.q_offsets[p.b.B];
   const float a = has_a ? w.part_lse[row] : -INFINITY, b = has_b ? w.part_lse[rows + row] : -INFINITY;
   const float mm = fmaxf(a, b), bm = mm == -INFINITY ? 0.f : mm;
@@ -517,7 +518,7 @@ RB_API int rb_softmax_attn_paged(const void* q, long long ld_q, long long Tq, in
   if (Tq == 0 || B == 0) return 0;
   if ((D != 64 && D != 128) || Hkv <= 0 || H % Hkv) return -1;
   if (ld_q % 8 || ld_o % 8) return -2;
-  if (page_size % 16 || page_size <= 0 || (groups > 0 && window > 0)) return -3;
+  if (page_size % 16 || page_size <= 0 || (groups > 0 && window > 0) || (groups > 1 && !group_offsets)) return -3;
   const long long rows = num_pages * 2 * page_size;
   if (Tq * H > 0x7fffffffLL || rows + page_size > 0x7fffffffLL) return -4;
   const int n_cta = num_sms > 0 ? num_sms : 148;
@@ -525,9 +526,10 @@ RB_API int rb_softmax_attn_paged(const void* q, long long ld_q, long long Tq, in
   const Space sp = space_of(n_cta, D, Tq * H, !plan.tiles_a || (groups > 0 && !plan.tiles_b), plan.tiles_a || plan.tiles_b, groups > 0);
   if (workspace_bytes < sp.total) return -5;
   Batch p;
-  const Seqs own = {q_offsets, nullptr, k_offsets, page_ids, page_indptr, num_page_ids, B, B, 1};
-  const Seqs none = {nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0, 0, 0};
-  const Seqs pre = {q_offsets, group_offsets, prefix_offsets, prefix_page_ids, prefix_page_indptr, num_prefix_page_ids, groups, B, 0};
+  const Seqs own = {q_offsets, nullptr, 0, k_offsets, page_ids, page_indptr, num_page_ids, B, B, 1};
+  const Seqs none = {nullptr, nullptr, 0, nullptr, nullptr, nullptr, 0, 0, 0, 0};
+  const Seqs pre = {q_offsets, group_offsets, group_offsets == nullptr, prefix_offsets, prefix_page_ids, prefix_page_indptr, num_prefix_page_ids,
+                    groups, B, 0};
   p.a = groups > 0 ? pre : own;
   p.b = groups > 0 ? own : none;
   p.q = q; p.ld_q = ld_q; p.Tq = static_cast<int>(Tq); p.H = H; p.Hkv = Hkv; p.G = H / Hkv; p.page_size = page_size;

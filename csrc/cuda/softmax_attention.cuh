@@ -13,6 +13,7 @@ constexpr float LN2 = 0.6931471805599453f;
 struct Seqs {
   const int* q_offsets;       // [B+1] rows of q per sequence ...
   const int* group_offsets;   // ... or null; [B+1] into q_offsets: sequence g holds the queries of requests go[g]..go[g+1]-1
+  int one_group;              // B is 1 and holds the queries of all requests
   const int* k_offsets;       // [B+1] keys per sequence (differences are used)
   const int* page_ids;
   const int* page_indptr;     // [B+1]
@@ -43,7 +44,7 @@ __device__ __forceinline__ Seq seq_of(const Batch& p, int i) {
   const Seqs& s = second ? p.b : p.a;
   const int j = second ? i - p.a.B : i;
   Seq r;
-  int q0 = j, q1 = j + 1;
+  int q0 = j, q1 = s.one_group ? s.num_requests : j + 1;
   if (s.group_offsets) {
     q0 = min(max(s.group_offsets[j], 0), s.num_requests);
     q1 = min(max(s.group_offsets[j + 1], q0), s.num_requests);

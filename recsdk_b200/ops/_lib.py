@@ -104,23 +104,14 @@ def stream_ptr(device: Optional[torch.device] = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-class on_device:
-    """Makes the tensors' device current for a launch (a stream only takes launches of its own device)."""
+def is_current(index: int) -> bool:
+    """Whether the device is the current one (a stream only takes launches of its own device)."""
+    return torch._C._cuda_getDevice() == index
 
-    __slots__ = ("index", "before")
 
-    def __init__(self, device: torch.device) -> None:
-        self.index, self.before = device.index, None
-
-    def __enter__(self) -> None:
-        now = torch.cuda.current_device()
-        if self.index is not None and now != self.index:
-            self.before = now
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc) -> None:
-        if self.before is not None:
-            torch.cuda.set_device(self.before)
+def raw_stream(index: int) -> int:
+    """``stream_ptr`` of a device by its index, without the stream object around it."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -68,20 +68,24 @@ def sample_scores(scores: torch.Tensor, uniform: torch.Tensor, offsets: Optional
     m_t, m_v = _param("min_p", min_p, rows, torch.float32, dev, 0.0, 1.0)
     if not scores.is_cuda:
         return sample_scores_ref(scores, uniform, offsets, temperature, top_k, top_p, min_p)
-    with _lib.on_device(dev):
-        if scores.stride(-1) != 1 and width > 1:
-            scores = scores.contiguous()
-        uniform = uniform.contiguous()
-        if offsets is not None:
-            offsets = offsets.contiguous()
-        ids = torch.empty(rows, dtype=torch.int64, device=dev)
-        logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
-        rc = _lib.lib().rb_sample_scores(scores.data_ptr(), scores.stride(0) if offsets is None else 0, _lib.ptr(offsets),
-                                         int(offsets is not None and offsets.dtype == torch.int64), width, rows,
-                                         uniform.data_ptr(), _lib.ptr(t_t), _lib.ptr(k_t), _lib.ptr(p_t), _lib.ptr(m_t),
-                                         float(t_v), int(k_v), float(p_v), float(m_v), ids.data_ptr(), logprobs.data_ptr(),
-                                         _lib.dtype_code(scores.dtype), _lib.num_sms(dev), _lib.stream_ptr(dev))
-        _lib.check(rc, "rb_sample_scores")
+    index = scores.get_device()
+    if not _lib.is_current(index):
+        with torch.cuda.device(index):
+            return sample_scores(scores, uniform, offsets, temperature, top_k, top_p, min_p)
+    if width > 1 and scores.stride(-1) != 1:
+        scores = scores.contiguous()
+    uniform = uniform.contiguous()
+    off_ptr, off_64 = None, False
+    if offsets is not None:
+        offsets = offsets.contiguous()
+        off_ptr, off_64 = offsets.data_ptr(), offsets.dtype is torch.int64
+    ids = torch.empty(rows, dtype=torch.int64, device=dev)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
+    rc = _lib.lib().rb_sample_scores(scores.data_ptr(), scores.stride(0) if offsets is None else 0, off_ptr, off_64, width, rows,
+                                     uniform.data_ptr(), _lib.ptr(t_t), _lib.ptr(k_t), _lib.ptr(p_t), _lib.ptr(m_t), float(t_v),
+                                     int(k_v), float(p_v), float(m_v), ids.data_ptr(), logprobs.data_ptr(),
+                                     _lib.dtype_code(scores.dtype), _lib.num_sms(dev), _lib.raw_stream(index))
+    _lib.check(rc, "rb_sample_scores")
     return ids, logprobs
 
 

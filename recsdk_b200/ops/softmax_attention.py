@@ -13,6 +13,7 @@ those of :class:`~recsdk_b200.inference.KVCacheMetadata`.  There is no gradient.
 (``*_ref``), which are also what the tests compare with."""
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional
 
@@ -37,36 +38,41 @@ def rotary_table(max_positions: int, rotary_dim: int, base: float = 10000.0, dev
 # ----------------------------------------------------------------------------- checks
 def _rows(name: str, x: torch.Tensor, heads: Optional[int], dim: int, like: torch.Tensor) -> torch.Tensor:
     """[T, heads, dim] with adjacent heads and 16-byte aligned rows (others are copied)."""
-    if x.dim() != 3 or (heads is not None and x.shape[1] != heads) or x.shape[2] != dim:
-        raise ValueError("%s must be [tokens, %s, %d], got %s" % (name, "heads" if heads is None else heads, dim, tuple(x.shape)))
-    if x.dtype != like.dtype or x.device != like.device:
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
+        raise ValueError("%s must be [tokens, %s, %d], got %s" % (name, "heads" if heads is None else heads, dim, tuple(shape)))
+    if x.dtype is not like.dtype or x.get_device() != like.get_device():
         raise ValueError("%s must be %s on %s like the cache, got %s on %s" % (name, like.dtype, like.device, x.dtype, x.device))
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s requires a gradient, which this operator does not have (use torch.no_grad())" % name)
-    if x.is_cuda and x.numel() and (x.stride(2) != 1 or x.stride(1) != dim or x.stride(0) % 8 or x.stride(0) < 0 or x.data_ptr() % 16):
-        x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
+    if x.is_cuda:
+        st = x.stride()
+        if (st[2] != 1 or st[1] != dim or st[0] & 7 or st[0] < 0 or x.data_ptr() & 15) and x.numel():
+            x = x.contiguous()
+            if x.data_ptr() & 15:
+                x = x.clone()
     return x
 
 
-def _ints(name: str, x: torch.Tensor, device, n: Optional[int] = None) -> torch.Tensor:
-    if x.dim() != 1 or (n is not None and x.numel() != n):
-        raise ValueError("%s must be a vector%s, got %s" % (name, "" if n is None else " of %d" % n, tuple(x.shape)))
-    if x.dtype not in (torch.int32, torch.int64) or x.device != device:
-        raise ValueError("%s must be int32 or int64 on %s, got %s on %s" % (name, device, x.dtype, x.device))
-    return x if x.dtype == torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+def _ints(name: str, x: torch.Tensor, like: torch.Tensor, n: Optional[int] = None) -> torch.Tensor:
+    shape = x.shape
+    if len(shape) != 1 or (n is not None and shape[0] != n):
+        raise ValueError("%s must be a vector%s, got %s" % (name, "" if n is None else " of %d" % n, tuple(shape)))
+    if x.get_device() != like.get_device() or x.dtype not in (torch.int32, torch.int64):
+        raise ValueError("%s must be int32 or int64 on %s, got %s on %s" % (name, like.device, x.dtype, x.device))
+    return x if x.dtype is torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
 
 
 def _cache(kv_cache: torch.Tensor, page_size: int, dims=None) -> torch.Tensor:
-    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2 or kv_cache.shape[2] != page_size or not kv_cache.is_contiguous():
-        raise ValueError("kv_cache must be a contiguous [pages, 2, %d, kv_heads, head_dim], got %s" % (page_size, tuple(kv_cache.shape)))
+    shape = kv_cache.shape
+    if len(shape) != 5 or shape[1] != 2 or shape[2] != page_size or not kv_cache.is_contiguous():
+        raise ValueError("kv_cache must be a contiguous [pages, 2, %d, kv_heads, head_dim], got %s" % (page_size, tuple(shape)))
     if kv_cache.is_cuda:
-        if kv_cache.dtype not in (torch.bfloat16, torch.float16):
+        if kv_cache.dtype is not torch.bfloat16 and kv_cache.dtype is not torch.float16:
             raise ValueError("kv_cache must be bf16 or fp16, got %s" % (kv_cache.dtype,))
-        if dims is not None and kv_cache.shape[4] not in dims:
-            raise ValueError("head_dim must be one of %s, got %d" % (dims, kv_cache.shape[4]))
-        if kv_cache.data_ptr() % 16:
+        if dims is not None and shape[4] not in dims:
+            raise ValueError("head_dim must be one of %s, got %d" % (dims, shape[4]))
+        if kv_cache.data_ptr() & 15:
             raise ValueError("kv_cache must be 16-byte aligned")
     return kv_cache
 
@@ -99,28 +105,28 @@ def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache
     queries go (may be ``q``).  A token whose position or page does not exist is left out and reported by
     ``_lib.check_status``."""
     cache = _cache(kv_cache, page_size)
-    Hkv, D = cache.shape[3], cache.shape[4]
-    dev, n = cache.device, q.shape[0]
+    pages, _, _, Hkv, D = cache.shape
     if D % 16:
         raise ValueError("head_dim must be a multiple of 16, got %d" % D)
     q, k, v = _rows("q", q, None, D, cache), _rows("k", k, Hkv, D, cache), _rows("v", v, Hkv, D, cache)
+    n, H, _ = q.shape
     if k.shape[0] != n or v.shape[0] != n:
         raise ValueError("q, k and v must hold the same tokens, got %d, %d and %d" % (n, k.shape[0], v.shape[0]))
-    if table.dim() != 2 or table.dtype != torch.float32 or table.device != dev or not table.is_contiguous() \
-            or table.shape[1] % 16 or not 0 < table.shape[1] <= D or (table.is_cuda and table.data_ptr() % 16):
+    if table.dim() != 2 or table.dtype is not torch.float32 or table.get_device() != cache.get_device() or not table.is_contiguous() \
+            or table.shape[1] % 16 or not 0 < table.shape[1] <= D or (table.is_cuda and table.data_ptr() & 15):
         raise ValueError("table must be a contiguous fp32 [max_positions, rotary_dim] on %s with rotary_dim a multiple of 16 and "
-                         "at most %d, got %s %s on %s" % (dev, D, table.dtype, tuple(table.shape), table.device))
-    batch_indices, positions = _ints("batch_indices", batch_indices, dev, n), _ints("positions", positions, dev, n)
-    page_ids, page_indptr = _ints("page_ids", page_ids, dev), _ints("page_indptr", page_indptr, dev)
+                         "at most %d, got %s %s on %s" % (cache.device, D, table.dtype, tuple(table.shape), table.device))
+    batch_indices, positions = _ints("batch_indices", batch_indices, cache, n), _ints("positions", positions, cache, n)
+    page_ids, page_indptr = _ints("page_ids", page_ids, cache), _ints("page_indptr", page_indptr, cache)
     if num_tokens is not None:
-        num_tokens = _ints("num_tokens", num_tokens, dev, 1)
-    if page_indptr.numel() < 1:
+        num_tokens = _ints("num_tokens", num_tokens, cache, 1)
+    if page_indptr.shape[0] < 1:
         raise ValueError("page_indptr must be [requests + 1]")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or (out.numel() and (
-            out.stride(2) != 1 or out.stride(1) != D or out.stride(0) % 8 or out.stride(0) < out.shape[1] * D or out.data_ptr() % 16)):
-        raise ValueError("out must be %s %s on %s with adjacent heads and 16-byte aligned rows" % (tuple(q.shape), q.dtype, dev))
+        out = torch.empty((n, H, D), dtype=q.dtype, device=cache.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != cache.device or (out.numel() and (
+            out.stride(2) != 1 or out.stride(1) != D or out.stride(0) % 8 or out.stride(0) < H * D or out.data_ptr() % 16)):
+        raise ValueError("out must be %s %s on %s with adjacent heads and 16-byte aligned rows" % (tuple(q.shape), q.dtype, cache.device))
     if n == 0:
         return out
     if not cache.is_cuda:
@@ -132,14 +138,18 @@ def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache
         cache[at, 0, pos % page_size] = _rotate_ref(k[:m], cos, sin, interleaved)
         cache[at, 1, pos % page_size] = v[:m]
         return out
-    with _lib.on_device(dev):
-        rc = _lib.lib().rb_kv_append_rotary(
-            q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0),
-            cache.data_ptr(), batch_indices.data_ptr(), positions.data_ptr(), page_ids.data_ptr(), page_indptr.data_ptr(),
-            _lib.ptr(num_tokens), n, q.shape[1], Hkv, D, page_indptr.numel() - 1, page_size, page_ids.numel(), cache.shape[0],
-            table.data_ptr(), table.shape[0], table.shape[1], int(interleaved), int(q.dtype == torch.bfloat16), _lib.num_sms(dev),
-            _lib.status_tensor(dev).data_ptr(), _lib.stream_ptr(dev))
-        _lib.check(rc, "rb_kv_append_rotary")
+    index = cache.get_device()
+    if not _lib.is_current(index):
+        with torch.cuda.device(index):
+            return append_kv_rotary(q, k, v, cache, batch_indices, positions, page_ids, page_indptr, page_size, table, interleaved,
+                                    num_tokens, out)
+    rc = _lib.lib().rb_kv_append_rotary(
+        q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0),
+        cache.data_ptr(), batch_indices.data_ptr(), positions.data_ptr(), page_ids.data_ptr(), page_indptr.data_ptr(),
+        _lib.ptr(num_tokens), n, H, Hkv, D, page_indptr.shape[0] - 1, page_size, page_ids.shape[0], pages,
+        table.data_ptr(), table.shape[0], table.shape[1], interleaved, q.dtype is torch.bfloat16, _lib.num_sms(cache.device),
+        _lib.status_tensor(cache.device).data_ptr(), _lib.raw_stream(index))
+    _lib.check(rc, "rb_kv_append_rotary")
     return out
 
 
@@ -196,22 +206,26 @@ def softmax_attention_ref(q, kv_cache, q_offsets, k_offsets, page_ids, page_indp
     return out, lse
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*sizes) -> int:
+    return _lib.lib().rb_softmax_attn_workspace(*sizes)
+
+
 def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks, return_lse, prefix=None):
     cache = _cache(kv_cache, page_size, _HEAD_DIMS)
-    Hkv, D = cache.shape[3], cache.shape[4]
-    dev = cache.device
+    pages, _, _, Hkv, D = cache.shape
     q = _rows("q", q, None, D, cache)
-    T, H = q.shape[0], q.shape[1]
+    T, H, _ = q.shape
     if H == 0 or H % Hkv:
         raise ValueError("%d query heads cannot share %d key heads" % (H, Hkv))
     B = q_offsets.numel() - 1
     if B < 0:
         raise ValueError("q_offsets must be [requests + 1]")
-    q_offsets, k_offsets = _ints("q_offsets", q_offsets, dev), _ints("k_offsets", k_offsets, dev, B + 1)
-    page_ids, page_indptr = _ints("page_ids", page_ids, dev), _ints("page_indptr", page_indptr, dev, B + 1)
+    q_offsets, k_offsets = _ints("q_offsets", q_offsets, cache), _ints("k_offsets", k_offsets, cache, B + 1)
+    page_ids, page_indptr = _ints("page_ids", page_ids, cache), _ints("page_indptr", page_indptr, cache, B + 1)
     if window < 0 or num_sinks < 0:
         raise ValueError("window and num_sinks must not be negative")
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    scale = D ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
     groups, g_off, p_off, p_ids, p_ptr = 0, None, None, None, None
@@ -220,41 +234,36 @@ def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size,
         groups = p_off.numel() - 1
         if groups < 0 or (g_off is None and groups != 1):
             raise ValueError("prefix_offsets must be [groups + 1], and [2] without group_offsets")
-        p_off, p_ids = _ints("prefix_offsets", p_off, dev), _ints("prefix_page_ids", p_ids, dev)
-        p_ptr = _ints("prefix_page_indptr", p_ptr, dev, groups + 1)
+        p_off, p_ids = _ints("prefix_offsets", p_off, cache), _ints("prefix_page_ids", p_ids, cache)
+        p_ptr = _ints("prefix_page_indptr", p_ptr, cache, groups + 1)
         if g_off is not None:
-            g_off = _ints("group_offsets", g_off, dev, groups + 1)
+            g_off = _ints("group_offsets", g_off, cache, groups + 1)
     if not cache.is_cuda:
         o, lse = softmax_attention_ref(q, cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks,
                                        p_off, p_ids, p_ptr, g_off)
         return (o.to(q.dtype), lse) if return_lse else o.to(q.dtype)
     if page_size % 16:
         raise ValueError("page_size must be a multiple of 16, got %d" % page_size)
-    with _lib.on_device(dev):
-        out = torch.empty(T, H, D, dtype=q.dtype, device=dev)
-        lse = torch.empty(T, H, dtype=torch.float32, device=dev) if return_lse else None
-        if T and B == 0:
-            raise ValueError("q holds %d tokens but there are no requests" % T)
-        if T:
-            if g_off is None and groups:
-                g_off = _one_group(B, dev)
-            lib, sms = _lib.lib(), _lib.num_sms(dev)
-            nbytes = lib.rb_softmax_attn_workspace(sms, T, H, Hkv, D, B, groups, scale)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            rc = lib.rb_softmax_attn_paged(
-                q.data_ptr(), q.stride(0), T, H, Hkv, D, cache.data_ptr(), cache.shape[0], page_size, q_offsets.data_ptr(),
-                k_offsets.data_ptr(), page_ids.data_ptr(), page_indptr.data_ptr(), page_ids.numel(), B, _lib.ptr(g_off),
-                _lib.ptr(p_off), _lib.ptr(p_ids), _lib.ptr(p_ptr), p_ids.numel() if groups else 0, groups,
-                min(int(window), 1 << 30), min(int(num_sinks), 1 << 30), scale, int(q.dtype == torch.bfloat16), out.data_ptr(),
-                out.stride(0), _lib.ptr(lse), ws.data_ptr(), nbytes, sms, _lib.status_tensor(dev).data_ptr(), _lib.stream_ptr(dev))
-            _lib.check(rc, "rb_softmax_attn_paged")
+    if T and B == 0:
+        raise ValueError("q holds %d tokens but there are no requests" % T)
+    index, dev = cache.get_device(), cache.device
+    if not _lib.is_current(index):
+        with torch.cuda.device(index):
+            return _attend(q, cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks, return_lse, prefix)
+    out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
+    if T:
+        lib, sms = _lib.lib(), _lib.num_sms(dev)
+        nbytes = _workspace_bytes(sms, T, H, Hkv, D, B, groups, scale)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        rc = lib.rb_softmax_attn_paged(
+            q.data_ptr(), q.stride(0), T, H, Hkv, D, cache.data_ptr(), pages, page_size, q_offsets.data_ptr(),
+            k_offsets.data_ptr(), page_ids.data_ptr(), page_indptr.data_ptr(), page_ids.shape[0], B, _lib.ptr(g_off),
+            _lib.ptr(p_off), _lib.ptr(p_ids), _lib.ptr(p_ptr), p_ids.shape[0] if groups else 0, groups,
+            min(window, 1 << 30), min(num_sinks, 1 << 30), scale, q.dtype is torch.bfloat16, out.data_ptr(), H * D,
+            _lib.ptr(lse), ws.data_ptr(), nbytes, sms, _lib.status_tensor(dev).data_ptr(), _lib.raw_stream(index))
+        _lib.check(rc, "rb_softmax_attn_paged")
     return (out, lse) if return_lse else out
-
-
-def _one_group(requests: int, device) -> torch.Tensor:
-    t = torch.zeros(2, dtype=torch.int32, device=device)
-    t[1:].fill_(requests)
-    return t
 
 
 def softmax_attention_paged(q: torch.Tensor, kv_cache: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor,
