@@ -9,34 +9,37 @@
 //
 // Bound: the bytes of K and V.  The G query heads that share a key head are the rows of one 16-row mma.sync tile (a
 // 128-row tcgen05 tile would be mostly padding here and the matrix rate does not matter), so K and V are read once for all
-// of them.  The keys of all (sequence, row tile, key head) items are laid end to end in units of NW tiles of 32 keys and every
-// CTA takes an equal, contiguous share, found from the offsets on the device: uneven histories cost nothing, no length is
-// needed on the host and a captured graph stays right for other lengths.  An item cut by a share's border leaves partial
-// results (normalised o and its lse) that a second kernel joins.
+// of them.  The keys of all (sequence, row tile, key head) items are laid end to end and every worker takes an equal,
+// contiguous share, found from the offsets on the device: uneven histories cost nothing, no length is needed on the host and
+// a captured graph stays right for other lengths.  An item cut by a share's border leaves partial results (normalised o
+// and its lse) that a second kernel joins.
 //
-// Inside a CTA every warp streams its own tiles through its own TMA ring (128-byte swizzle, read with ldmatrix), with no
-// CTA-wide synchronisation until the warps' results are joined at the end of an item.
+// A worker is one warp where there are enough items to go round - every warp streams its own keys and nothing waits for
+// anything else - and a CTA of eight otherwise, whose warps take turns at the tiles of an item and are joined in shared
+// memory.  Every warp feeds its own ring by TMA (128-byte swizzle, read with ldmatrix), the page rows of 32 boxes looked up
+// at a time.
 #include "softmax_attention.cuh"
 
 namespace {
 
 using namespace rb_attn;
 
-constexpr int KT = 32;      // keys per tile
 constexpr int RT = 16;      // rows per tile
-constexpr int NW = 4;       // warps per CTA
+constexpr int NW = 8;       // warps per CTA
 
 template <int D> struct Cfg {
   static constexpr int CH = D / 64;
+  static constexpr int KT = 2048 / D;                           // keys per tile
   static constexpr int TILE = KT * D * 2;                       // bytes of a K or a V tile
-  static constexpr int STAGES = D == 64 ? 4 : 3;
-  static constexpr int RING = NW * STAGES * 2 * TILE;
+  static constexpr int STAGES = 3;
+  static constexpr int WARP_RING = STAGES * 2 * TILE;
+  static constexpr int RING = NW * WARP_RING;
   static constexpr int SMEM = RING + 1024 + 2048;
 };
 
-struct Items { int qt, units; };           // row tiles of a sequence, units of keys of each
+struct Items { int qt, units; };           // row tiles of a sequence, units of W key tiles of each
 
-template <int D>
+template <int KT, int W>
 __device__ __forceinline__ Items items_of(const Batch& p, const Seq& s) {
   Items r;
   r.qt = (s.len_q * p.G + RT - 1) / RT;
@@ -49,7 +52,7 @@ __device__ __forceinline__ Items items_of(const Batch& p, const Seq& s) {
       tiles = static_cast<int>(min(static_cast<long long>(tiles),
                                    (p.sinks + KT - 1LL) / KT + (static_cast<long long>(p.window) + (RT - 1) / p.G + 2 + 2 * KT) / KT));
   }
-  r.units = max((tiles + NW - 1) / NW, 1);
+  r.units = max((tiles + W - 1) / W, 1);
   return r;
 }
 
@@ -69,17 +72,20 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t& a, uint32_t
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(NW * 32) attn_rows_kernel(const __grid_constant__ CUtensorMap tm, const Batch p, const Outs w) {
+template <int D, bool BF16, int W>
+__global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_constant__ CUtensorMap tm, const Batch p, const Outs w) {
   using C = Cfg<D>;
+  constexpr int KT = C::KT;
+  constexpr int PER_CTA = NW / W;                                              // workers of a CTA
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* tail = smem + C::RING;
   uint64_t* bars = reinterpret_cast<uint64_t*>(tail);                          // [NW][STAGES]
-  float* ml = reinterpret_cast<float*>(tail + 256);                            // [NW][RT][2]
-  long long* sums = reinterpret_cast<long long*>(tail + 1024);                 // [NW], then base of the first item
-  int* found = reinterpret_cast<int*>(tail + 1024 + 64);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 1024 + 96);
+  long long* sums = reinterpret_cast<long long*>(tail + 256);                  // [NW]
+  long long* found_base = reinterpret_cast<long long*>(tail + 320);            // [NW]
+  int* found = reinterpret_cast<int*>(tail + 384);                             // [NW]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 416);
+  float* ml = reinterpret_cast<float*>(tail + 1024);                           // [NW][RT][2]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nb = p.a.B + p.b.B;
   if (tid == 0) {
@@ -87,14 +93,11 @@ __global__ void __launch_bounds__(NW * 32) attn_rows_kernel(const __grid_constan
     *abort_flag = 0;
     rb::mbar_fence_init();
   }
-  // ---- this CTA's share of the keys
+  // ---- the workers' shares of the keys
   const int per = (nb + NW * 32 - 1) / (NW * 32);
+  auto units_of = [&](const Items& it) { return static_cast<long long>(it.qt) * it.units * p.Hkv; };
   long long mine = 0;
-  for (int i = tid * per; i < min((tid + 1) * per, nb); ++i) {
-    const Seq s = seq_of(p, i);
-    const Items it = items_of<D>(p, s);
-    mine += static_cast<long long>(it.qt) * it.units * p.Hkv;
-  }
+  for (int i = tid * per; i < min((tid + 1) * per, nb); ++i) mine += units_of(items_of<KT, W>(p, seq_of(p, i)));
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -108,68 +111,76 @@ __global__ void __launch_bounds__(NW * 32) attn_rows_kernel(const __grid_constan
     if (i < warp) before += sums[i];
     total += sums[i];
   }
-  const int n_sh = static_cast<int>(min(static_cast<long long>(gridDim.x), total));   // no share is empty
-  const int cta = blockIdx.x;
-  const long long p0 = cta < n_sh ? share(cta, n_sh, total) : 0, p1 = cta < n_sh ? share(cta + 1, n_sh, total) : 0;
-  if (p0 < p1 && before <= p0 && p0 < before + mine) {
-    long long base = before;
-    for (int i = tid * per;; ++i) {
-      const Seq s = seq_of(p, i);
-      const Items it = items_of<D>(p, s);
-      const long long n = static_cast<long long>(it.qt) * it.units * p.Hkv;
-      if (p0 < base + n) { *found = i; sums[NW] = base; break; }
-      base += n;
+  const int n_sh = static_cast<int>(min(static_cast<long long>(gridDim.x) * PER_CTA, total));   // no share is empty
+  auto begin_of = [&](int c) { return c < n_sh ? share(c, n_sh, total) : total; };
+  for (int x = 0; x < PER_CTA; ++x) {
+    const int c = blockIdx.x * PER_CTA + x;
+    const long long at = c < n_sh ? share(c, n_sh, total) : -1;
+    if (at >= before && at < before + mine) {
+      long long base = before;
+      for (int i = tid * per;; ++i) {
+        const long long n = units_of(items_of<KT, W>(p, seq_of(p, i)));
+        if (at < base + n) { found[x] = i; found_base[x] = base; break; }
+        base += n;
+      }
     }
   }
   __syncthreads();
+  const int me = W == 1 ? warp : 0, turn = W == 1 ? 0 : warp;                  // worker of the CTA, this warp's turn in it
+  const int wk = blockIdx.x * PER_CTA + me;
+  const long long p0 = wk < n_sh ? begin_of(wk) : 0, p1 = wk < n_sh ? begin_of(wk + 1) : 0;
   Meta m;
   m.valid = 0;
   if (p0 < p1) {
-    int b = *found;
-    long long base = sums[NW], pos = p0;
-    uint8_t* ring = smem + warp * (C::STAGES * 2 * C::TILE);
+    int b = found[me];
+    long long base = found_base[me], pos = p0;
+    uint8_t* ring = smem + warp * C::WARP_RING;
     uint64_t* bar = bars + warp * C::STAGES;
-    int issued = 0, used = 0;                                                  // tiles of this warp so far
+    int issued = 0, used = 0, st_in = 0, st_out = 0;                           // tiles of this warp so far, ring slots
+    uint32_t par = 0;
     bool dead = false;
+    const int boxes = KT / p.box_rows, batch = 32 / boxes;
+    const int my_kind = lane / (boxes * C::CH), my_box = lane / C::CH % boxes, my_chunk = lane % C::CH;   // this lane's TMA box
     while (pos < p1 && b < nb) {
       const Seq s = seq_of(p, b);
-      const Items it = items_of<D>(p, s);
-      const long long n_b = static_cast<long long>(it.qt) * it.units * p.Hkv;
+      const Items it = items_of<KT, W>(p, s);
+      const long long n_b = units_of(it);
       if (pos >= base + n_b) { base += n_b; ++b; continue; }
-      const int off = static_cast<int>((pos - base) % it.units);
       const int item = static_cast<int>((pos - base) / it.units);
+      const int off = static_cast<int>(pos - base - static_cast<long long>(item) * it.units);
       const int u1 = static_cast<int>(min(static_cast<long long>(it.units), off + (p1 - pos)));
-      const int qt = item / p.Hkv, h = item % p.Hkv;
+      const int qt = item / p.Hkv, h = item - qt * p.Hkv;
       const int rows = min(s.len_q * p.G - qt * RT, RT);
       const Span sp = span_of<KT>(p, s, qt * RT / p.G, (qt * RT + rows - 1) / p.G);
       const long long t0 = pos - off;
-      if (pos == p0 && off > 0 && share(cta - 1, n_sh, total) <= t0) {
+      if (pos == p0 && off > 0 && begin_of(wk - 1) <= t0) {
         // the first border inside this item: the second kernel joins its pieces
         m.valid = 1; m.seq = b; m.row0 = qt * RT; m.rows = rows; m.h = h; m.t0 = t0; m.total = total; m.n = n_sh;
-        m.c0 = cta - 1;
+        m.c0 = wk - 1;
         m.c1 = static_cast<int>(((t0 + it.units) * n_sh - 1) / total);        // the share that holds the item's last unit
       }
-      const int v0 = off * NW + warp, v1 = min(u1 * NW, sp.tiles);
-      auto issue = [&](int v) {
-        if (lane == 0) {
-          const int st = issued % C::STAGES;
-          uint8_t* k_dst = ring + st * 2 * C::TILE;
-          uint8_t* v_dst = k_dst + C::TILE;
-          rb::mbar_expect_tx(&bar[st], 2 * C::TILE);
-          const int j0 = sp.tile(v) * KT;
-          for (int x = 0; x < KT; x += p.box_rows) {
-            const int row = box_row(p, s, sp, j0 + x);
-#pragma unroll
-            for (int c = 0; c < C::CH; ++c) {
-              rb::tma_load_2d(k_dst + c * (KT * 128) + x * 128, &tm, &bar[st], h * D + c * 64, row);
-              rb::tma_load_2d(v_dst + c * (KT * 128) + x * 128, &tm, &bar[st], h * D + c * 64, row + p.page_size);
-            }
-          }
-        }
-        ++issued;
+      // this warp's tiles: v0 + k * W for k < n
+      const int v0 = off * W + turn, n = (min(u1 * W, sp.tiles) - v0 + W - 1) / W;
+      int rows_at = 0, rows_box = 0;                                           // rows of the boxes of `batch` tiles from rows_at on
+      auto look_up = [&](int k) {
+        const int mine_k = k + lane / boxes;
+        rows_box = mine_k < n && lane < batch * boxes ? box_row(p, s, sp, sp.tile(v0 + mine_k * W) * KT + (lane % boxes) * p.box_rows) : p.total_rows;
+        rows_at = k;
       };
-      int nxt = v0;
-      for (int i = 0; i < C::STAGES && nxt < v1 && !dead; ++i, nxt += NW) issue(nxt);
+      auto issue = [&](int k) {
+        if (k == rows_at + batch) look_up(k);
+        const int row = __shfl_sync(0xffffffffu, rows_box, ((k - rows_at) * boxes + my_box) & 31) + my_kind * p.page_size;
+        if (lane == 0) rb::mbar_expect_tx(&bar[st_in], 2 * C::TILE);
+        __syncwarp();
+        if (my_kind < 2)
+          rb::tma_load_2d(ring + (st_in * 2 + my_kind) * C::TILE + my_chunk * (KT * 128) + my_box * p.box_rows * 128, &tm, &bar[st_in],
+                          h * D + my_chunk * 64, row);
+        ++issued;
+        if (++st_in == C::STAGES) st_in = 0;
+      };
+      if (n > 0) look_up(0);
+      int nxt = 0;
+      for (; nxt < min(n, C::STAGES) && !dead; ++nxt) issue(nxt);
       // ---- the 16 query rows as A fragments: this thread's rows are lane / 4 and lane / 4 + 8
       uint32_t qf[D / 16][4];
       int rpos[2];
@@ -191,13 +202,12 @@ __global__ void __launch_bounds__(NW * 32) attn_rows_kernel(const __grid_constan
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
       float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-      for (int v = v0; v < v1 && !dead; v += NW) {
-        const int st = used % C::STAGES;
-        const bool ok = rb::mbar_wait(&bar[st], (used / C::STAGES) & 1, abort_flag, p.status);
+      for (int k = 0; k < n && !dead; ++k) {
+        const bool ok = rb::mbar_wait(&bar[st_out], par, abort_flag, p.status);
         if (!__all_sync(0xffffffffu, ok)) { dead = true; break; }
         ++used;
-        const uint32_t k_addr = rb::smem_u32(ring + st * 2 * C::TILE), v_addr = k_addr + C::TILE;
-        const int j0 = sp.tile(v) * KT;
+        const uint32_t k_addr = rb::smem_u32(ring + st_out * 2 * C::TILE), v_addr = k_addr + C::TILE;
+        const int j0 = sp.tile(v0 + k * W) * KT;
         const bool full = (s.causal ? j0 + KT - 1 <= sp.p_min : j0 + KT <= sp.hi) &&
                           (!s.causal || p.window <= 0 || j0 > sp.p_max - p.window || j0 + KT <= p.sinks);
         float sc[KT / 8][4];
@@ -207,13 +217,13 @@ __global__ void __launch_bounds__(NW * 32) attn_rows_kernel(const __grid_constan
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
 #pragma unroll
-          for (int n = 0; n < KT / 16; ++n) {
-            const int r = n * 16 + (lane & 7) + ((lane >> 4) << 3);
+          for (int i = 0; i < KT / 16; ++i) {
+            const int r = i * 16 + (lane & 7) + ((lane >> 4) << 3);
             const int unit = (kk & 3) * 2 + ((lane >> 3) & 1);
             uint32_t b0, b1, b2, b3;
             ldsm4(k_addr + (kk >> 2) * (KT * 128) + r * 128 + ((unit ^ (r & 7)) << 4), b0, b1, b2, b3);
-            mma16816<BF16>(sc[2 * n], qf[kk], b0, b1);
-            mma16816<BF16>(sc[2 * n + 1], qf[kk], b2, b3);
+            mma16816<BF16>(sc[2 * i], qf[kk], b0, b1);
+            mma16816<BF16>(sc[2 * i + 1], qf[kk], b2, b3);
           }
         }
         float mn[2] = {mx[0], mx[1]};
@@ -259,12 +269,12 @@ __global__ void __launch_bounds__(NW * 32) attn_rows_kernel(const __grid_constan
         if (!full) {
           // V of keys that no row of the block sees may be anything (0 x NaN is NaN): clear it
           const int j = j0 + lane;
-          if (!(j < sp.hi && (j >= sp.lo || j < sp.sinks))) {
-            uint4* vr = reinterpret_cast<uint4*>(ring + st * 2 * C::TILE + C::TILE + lane * 128);
+          if (lane < KT && !(j < sp.hi && (j >= sp.lo || j < sp.sinks))) {
+            uint4* vr = reinterpret_cast<uint4*>(ring + (st_out * 2 + 1) * C::TILE + lane * 128);
 #pragma unroll
             for (int c = 0; c < C::CH; ++c)
 #pragma unroll
-              for (int i = 0; i < 8; ++i) vr[c * (KT * 8) + i] = make_uint4(0, 0, 0, 0);
+              for (int i = 0; i < 8; ++i) vr[c * (KT * 8) + ((i + lane) & 7)] = make_uint4(0, 0, 0, 0);
           }
           rb::fence_proxy_async_smem();
           __syncwarp();
@@ -273,35 +283,62 @@ __global__ void __launch_bounds__(NW * 32) attn_rows_kernel(const __grid_constan
 #pragma unroll
         for (int kk = 0; kk < KT / 16; ++kk) {
 #pragma unroll
-          for (int n = 0; n < D / 16; ++n) {
+          for (int i = 0; i < D / 16; ++i) {
             const int r = kk * 16 + (lane & 15);
-            const int unit = (n & 3) * 2 + (lane >> 4);
+            const int unit = (i & 3) * 2 + (lane >> 4);
             uint32_t b0, b1, b2, b3;
-            ldsm4_trans(v_addr + (n >> 2) * (KT * 128) + r * 128 + ((unit ^ (r & 7)) << 4), b0, b1, b2, b3);
-            mma16816<BF16>(o[2 * n], pf[kk], b0, b1);
-            mma16816<BF16>(o[2 * n + 1], pf[kk], b2, b3);
+            ldsm4_trans(v_addr + (i >> 2) * (KT * 128) + r * 128 + ((unit ^ (r & 7)) << 4), b0, b1, b2, b3);
+            mma16816<BF16>(o[2 * i], pf[kk], b0, b1);
+            mma16816<BF16>(o[2 * i + 1], pf[kk], b2, b3);
           }
         }
         __syncwarp();
-        if (nxt < v1) { issue(nxt); nxt += NW; }
+        if (++st_out == C::STAGES) { st_out = 0; par ^= 1; }
+        if (nxt < n) issue(nxt++);
       }
       if (dead) {                                                              // the kernel's own copies end before it does
-        for (; used < issued; ++used)
-          for (uint32_t i = 0; i < (1u << 20) && !rb::mbar_try_wait(&bar[used % C::STAGES], (used / C::STAGES) & 1); ++i) {}
+        for (; used < issued; ++used) {
+          for (uint32_t i = 0; i < (1u << 20) && !rb::mbar_try_wait(&bar[st_out], par); ++i) {}
+          if (++st_out == C::STAGES) { st_out = 0; par ^= 1; }
+        }
       }
-      // ---- join the warps: o [RT][D] in the warp's own, now idle ring
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
         sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
-        const int r = (lane >> 2) + 8 * e;
-        float* dst = reinterpret_cast<float*>(ring) + r * D + (lane & 3) * 2;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
-        if ((lane & 3) == 0) { ml[(warp * RT + r) * 2] = mx[e]; ml[(warp * RT + r) * 2 + 1] = sum[e]; }
       }
-      __syncthreads();
-      {
+      const bool whole = off == 0 && u1 == it.units;
+      const long long cut = static_cast<long long>(wk) * 2 + (pos == p0 ? 0 : 1);
+      if (W == 1) {
+        // ---- the warp's own result, straight from the fragments
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = (lane >> 2) + 8 * e;
+          if (r < rows) {
+            const float inv = sum[e] == 0.f ? 0.f : 1.f / sum[e];
+            const float lse2 = sum[e] == 0.f ? -INFINITY : mx[e] + log2f(sum[e]);
+            const RowOut to = row_out(p, w, s, qt * RT + r, h, D, whole, cut * RT + r);
+            if ((lane & 3) == 0 && to.lse) *to.lse = to.natural ? lse2 * LN2 : lse2;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+              const float x = o[i][2 * e] * inv, y = o[i][2 * e + 1] * inv;
+              const int col = i * 8 + (lane & 3) * 2;
+              if (to.o16) *reinterpret_cast<uint32_t*>(to.o16 + col) = pack16<BF16>(x, y);
+              else *reinterpret_cast<float2*>(to.o32 + col) = make_float2(x, y);
+            }
+          }
+        }
+      } else {
+        // ---- join the warps: o [RT][D] in the warp's own, now idle ring
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = (lane >> 2) + 8 * e;
+          float* dst = reinterpret_cast<float*>(ring) + r * D + (lane & 3) * 2;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
+          if ((lane & 3) == 0) { ml[(warp * RT + r) * 2] = mx[e]; ml[(warp * RT + r) * 2 + 1] = sum[e]; }
+        }
+        __syncthreads();
         constexpr int TPR = NW * 32 / RT, N = 4;                               // threads per row, elements at a time
         const int r = tid / TPR;
         if (r < rows) {
@@ -317,32 +354,26 @@ __global__ void __launch_bounds__(NW * 32) attn_rows_kernel(const __grid_constan
           }
           const float inv = l == 0.f ? 0.f : 1.f / l;
           const float lse2 = l == 0.f ? -INFINITY : mm + log2f(l);
-          const bool whole = off == 0 && u1 == it.units;
-          const long long cut = static_cast<long long>(cta) * 2 + (pos == p0 ? 0 : 1);
+          const RowOut to = row_out(p, w, s, qt * RT + r, h, D, whole, cut * RT + r);
+          if (tid % TPR == 0 && to.lse) *to.lse = to.natural ? lse2 * LN2 : lse2;
           for (int col = (tid % TPR) * N; col < D; col += TPR * N) {
             float x[N] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
-              const float4 y = *reinterpret_cast<const float4*>(smem + i * (C::STAGES * 2 * C::TILE) + (r * D + col) * 4);
+              const float4 y = *reinterpret_cast<const float4*>(smem + i * C::WARP_RING + (r * D + col) * 4);
               x[0] += f[i] * y.x; x[1] += f[i] * y.y; x[2] += f[i] * y.z; x[3] += f[i] * y.w;
             }
-#pragma unroll
-            for (int i = 0; i < N; ++i) x[i] *= inv;
-            if (whole) {
-              write_row<D, BF16, N>(p, w, s, qt * RT + r, h, col, x, lse2);
-            } else {
-              *reinterpret_cast<float4*>(w.cut_o + (cut * RT + r) * D + col) = make_float4(x[0], x[1], x[2], x[3]);
-              if (col == 0) w.cut_lse[cut * RT + r] = lse2;
-            }
+            if (to.o16) *reinterpret_cast<uint2*>(to.o16 + col) = make_uint2(pack16<BF16>(x[0] * inv, x[1] * inv), pack16<BF16>(x[2] * inv, x[3] * inv));
+            else *reinterpret_cast<float4*>(to.o32 + col) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
           }
         }
+        rb::fence_proxy_async_smem();
+        __syncthreads();
       }
-      rb::fence_proxy_async_smem();
-      __syncthreads();
       pos += u1 - off;
     }
   }
-  if (tid == 0) w.meta[cta] = m;
+  if (lane == 0 && (W == 1 || warp == 0)) w.meta[wk] = m;
 }
 
 // Joins the pieces of the items that borders cut: block (c, y) looks after 16 rows of the item whose first border is share
@@ -378,11 +409,13 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const Batch p, const Out
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const float lse2 = l == 0.f ? -INFINITY : mm + log2f(l);
+  const RowOut to = row_out(p, w, s, m.row0 + r, m.h, D, true, 0);
+  if (threadIdx.x % TPR == 0 && to.lse) *to.lse = to.natural ? lse2 * LN2 : lse2;
 #pragma unroll
   for (int k = 0; k < D / (TPR * N); ++k) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[k][i] *= inv;
-    write_row<D, BF16, N>(p, w, s, m.row0 + r, m.h, (threadIdx.x % TPR) * N + k * TPR * N, x[k], lse2);
+    const int col = (threadIdx.x % TPR) * N + k * TPR * N;
+    if (to.o16) *reinterpret_cast<uint2*>(to.o16 + col) = make_uint2(pack16<BF16>(x[k][0] * inv, x[k][1] * inv), pack16<BF16>(x[k][2] * inv, x[k][3] * inv));
+    else *reinterpret_cast<float4*>(to.o32 + col) = make_float4(x[k][0] * inv, x[k][1] * inv, x[k][2] * inv, x[k][3] * inv);
   }
 }
 
@@ -424,7 +457,7 @@ Space space_of(int n_cta, int D, long long rows, bool with_rows, bool with_tiles
   long long at = 0;
   auto take = [&](long long bytes) { const long long was = at; at = align256(at + bytes); return was; };
   for (int k = 0; k < 2; ++k) {
-    const long long n = (k ? with_tiles : with_rows) ? static_cast<long long>(n_cta) : 0, block = k ? TILE_ROWS : RT;
+    const long long n = (k ? with_tiles : with_rows) ? static_cast<long long>(n_cta) * (k ? 1 : NW) : 0, block = k ? TILE_ROWS : RT;
     s.cut_o[k] = take(n * 2 * block * D * 4);
     s.cut_lse[k] = take(n * 2 * block * 4);
     s.meta[k] = take(n * static_cast<long long>(sizeof(Meta)));
@@ -452,8 +485,15 @@ Plan plan_of(long long Tq, int G, int B, int groups, float scale) {
 }
 
 template <int D, bool BF16>
-int join(const Batch& p, const Outs& w, int n_cta, int block_rows, cudaStream_t st) {
-  attn_join_kernel<D, BF16><<<dim3(n_cta, block_rows / RT), 128, 0, st>>>(p, w, block_rows);
+int join(const Batch& p, const Outs& w, int shares, int block_rows, cudaStream_t st) {
+  attn_join_kernel<D, BF16><<<dim3(shares, block_rows / RT), 128, 0, st>>>(p, w, block_rows);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <int D, bool BF16, int W>
+int launch_rows(const CUtensorMap& tm, const Batch& p, const Outs& w, int n_cta, cudaStream_t st) {
+  RB_CUDA_CHECK(cudaFuncSetAttribute(attn_rows_kernel<D, BF16, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM));
+  attn_rows_kernel<D, BF16, W><<<n_cta, NW * 32, Cfg<D>::SMEM, st>>>(tm, p, w);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -468,20 +508,23 @@ int launch(const Batch& p, Outs w, const Plan& plan, const Space& sp, char* ws, 
     w.cut_o = reinterpret_cast<float*>(ws + sp.cut_o[tiles]);
     w.cut_lse = reinterpret_cast<float*>(ws + sp.cut_lse[tiles]);
     w.meta = reinterpret_cast<Meta*>(ws + sp.meta[tiles]);
+    int shares = n_cta;
     if (tiles) {
       const int rc = launch_tiles(q, w, cache, D, BF16, n_cta, st);
       if (rc) return rc;
     } else {
       CUtensorMap tm;
-      q.box_rows = p.page_size % KT == 0 ? KT : 16;
-      const int rc = rb_host::make_map_2d(&tm, cache, p.total_rows, static_cast<long long>(p.Hkv) * D, static_cast<long long>(p.Hkv) * D,
-                                          64, q.box_rows, BF16);
+      q.box_rows = p.page_size % Cfg<D>::KT == 0 ? Cfg<D>::KT : 16;
+      int rc = rb_host::make_map_2d(&tm, cache, p.total_rows, static_cast<long long>(p.Hkv) * D, static_cast<long long>(p.Hkv) * D, 64,
+                                    q.box_rows, BF16);
       if (rc) return rc;
-      RB_CUDA_CHECK(cudaFuncSetAttribute(attn_rows_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM));
-      attn_rows_kernel<D, BF16><<<n_cta, NW * 32, Cfg<D>::SMEM, st>>>(tm, q, w);
-      RB_CUDA_CHECK(cudaGetLastError());
+      // a worker per warp where the items (at least one per sequence and key head) go round at least a quarter of them
+      const bool single = static_cast<long long>(q.a.B + q.b.B) * p.Hkv * 4 >= static_cast<long long>(n_cta) * NW;
+      if (single) shares = n_cta * NW;
+      rc = single ? launch_rows<D, BF16, 1>(tm, q, w, n_cta, st) : launch_rows<D, BF16, NW>(tm, q, w, n_cta, st);
+      if (rc) return rc;
     }
-    const int rc = join<D, BF16>(q, w, n_cta, tiles ? TILE_ROWS : RT, st);
+    const int rc = join<D, BF16>(q, w, shares, tiles ? TILE_ROWS : RT, st);
     if (rc) return rc;
   }
   if (parts) {

@@ -132,32 +132,26 @@ struct Outs {
   Meta* meta;                              // [shares]
 };
 
-// N consecutive elements of one finished row: o normalised, lse in log2
-template <int D, bool BF16, int N>
-__device__ __forceinline__ void write_row(const Batch& p, const Outs& w, const Seq& s, int row, int h, int col, const float (&o)[N],
-                                          float lse2) {
+// Where a row's result goes: 16 bits to the output, or fp32 to its part or to its place among the cut pieces
+struct RowOut { uint16_t* o16; float* o32; float* lse; int natural; };   // natural: lse to base e, else log2
+
+__device__ __forceinline__ RowOut row_out(const Batch& p, const Outs& w, const Seq& s, int row, int h, int D, bool whole, long long cut) {
+  RowOut r = {nullptr, nullptr, nullptr, 0};
   const long long t = s.q_begin + row / p.G;
   const int head = h * p.G + row % p.G;
-  if (w.part_o) {
+  if (!whole) {
+    r.o32 = w.cut_o + cut * D;
+    r.lse = w.cut_lse + cut;
+  } else if (w.part_o) {
     const long long at = (static_cast<long long>(s.part) * p.Tq + t) * p.H + head;
-    float* dst = w.part_o + at * D + col;
-#pragma unroll
-    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-    if (col == 0) w.part_lse[at] = lse2;
+    r.o32 = w.part_o + at * D;
+    r.lse = w.part_lse + at;
   } else {
-    uint16_t* dst = reinterpret_cast<uint16_t*>(w.out) + t * w.ld_o + static_cast<long long>(head) * D + col;
-    if (N % 8 == 0) {
-#pragma unroll
-      for (int i = 0; i + 8 <= N; i += 8)
-        *reinterpret_cast<uint4*>(dst + i) = make_uint4(pack16<BF16>(o[i], o[i + 1]), pack16<BF16>(o[i + 2], o[i + 3]),
-                                                        pack16<BF16>(o[i + 4], o[i + 5]), pack16<BF16>(o[i + 6], o[i + 7]));
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; i += 4)
-        *reinterpret_cast<uint2*>(dst + i) = make_uint2(pack16<BF16>(o[i], o[i + 1]), pack16<BF16>(o[i + 2], o[i + 3]));
-    }
-    if (col == 0 && w.lse) w.lse[t * p.H + head] = lse2 * LN2;
+    r.o16 = reinterpret_cast<uint16_t*>(w.out) + t * w.ld_o + static_cast<long long>(head) * D;
+    r.lse = w.lse ? w.lse + t * p.H + head : nullptr;
+    r.natural = 1;
   }
+  return r;
 }
 
 // softmax_attention_tiles.cu: the kernel for many rows per sequence; fills out / part and the cut pieces (blocks of

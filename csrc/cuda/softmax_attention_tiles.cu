@@ -500,7 +500,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int row = quarter * 32 + lane;
     const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t t_s = tmem + lane_sel + x * 128, t_o = tmem + lane_sel + 256 + x * 128;
-    const int my_tok = row / p.G, my_head = row % p.G;                         // of the row tile, of the group
+    const int my_tok = row / p.G;                                              // of the row tile
     uint32_t n_s = 0, par_o = 0, par_swap = 0;                                  // key tiles so far; bit y: of row tile y's o_full
     while (const Piece* q = next_piece()) {
       const bool two = q->two;
@@ -622,27 +622,10 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const int r_cut = two ? x * tpt * p.G + row : row;                      // row of the block
         const int tok = (two ? x * tpt : 0) + my_tok;
         const bool live = row < tpt * p.G && tok < q->tokens;
-        const long long t = q->s.q_begin + q->t_lo + tok;
-        const int head = q->h * p.G + my_head;
-        // where this row goes: a 16-bit row of the result, or an fp32 row of a part or of a cut item's piece
-        float* dst32 = nullptr;
-        float* dst_lse;
-        uint16_t* dst16 = nullptr;
-        float lse_out = lse2;
-        if (!q->whole) {
-          const long long cut = static_cast<long long>(q->cut) * TILE_ROWS + r_cut;
-          dst32 = w.cut_o + cut * D;
-          dst_lse = w.cut_lse + cut;
-        } else if (w.part_o) {
-          const long long at = (static_cast<long long>(q->s.part) * p.Tq + t) * p.H + head;
-          dst32 = w.part_o + at * D;
-          dst_lse = w.part_lse + at;
-        } else {
-          dst16 = reinterpret_cast<uint16_t*>(w.out) + t * w.ld_o + static_cast<long long>(head) * D;
-          dst_lse = w.lse ? w.lse + t * p.H + head : nullptr;
-          lse_out = lse2 * LN2;
-        }
-        if (live && c_lo == 0 && dst_lse) *dst_lse = lse_out;
+        const RowOut to = row_out(p, w, q->s, q->t_lo * p.G + r_cut, q->h, D, q->whole != 0, static_cast<long long>(q->cut) * TILE_ROWS + r_cut);
+        if (live && c_lo == 0 && to.lse) *to.lse = to.natural ? lse2 * LN2 : lse2;
+        uint16_t* dst16 = to.o16;
+        float* dst32 = to.o32;
 #pragma unroll 1
         for (int c = c_lo; c < c_hi; c += 32) {
           uint32_t a[32];
