@@ -438,8 +438,38 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (!wait(&bars->q_full, par_q)) break;
       par_q ^= 1;
       const int ahead = two ? 2 : 4;
+      // steps whose K and V are both this row tile's and need no clearing
+      const int clean0 = max(c_lo - skip, sink_tiles) - v0, clean1 = c_hi - skip - v0;
+      const int plain0 = two ? max(max(clean0, fi) + ahead, fi) : max(clean0, 0) + ahead;
+      const int plain1 = two ? min(min(clean1, en) + ahead, min(en, n)) : min(clean1 + ahead, n);
+      const uint32_t q_at = (two ? x : 0) * (C::Q_TILE >> 4);
       for (int e = 0; e < n + ahead; ++e) {
         const int m = e - ahead;
+        if (e >= plain0 && e < plain1 && (two || (e & 1) == x) && started) {
+          // the same as below, without its questions: this is where the time goes
+          if (!wait(&bars->full[st], par)) break;
+          const uint32_t bp = n_p & 1, bs = n_s & 1;
+          if (!wait(&bars->p_full[x][bp], (n_p >> 1) & 1)) break;
+          ++n_p;
+          ++n_s;
+          rb::tc_fence_after();
+          if (elect()) {
+            const uint32_t at = st * (C::TILE >> 3);
+            const uint64_t dv = d_v + at, dq = d_q + q_at, dk = d_k + at;
+#pragma unroll
+            for (int kk = 0; kk < KT / 16; ++kk) rb::umma_f16_ts(t_o, t_s + bp * KT + kk * 8, dv + kk * 128, idesc_o, 1u);
+            rb::umma_commit(&bars->o_done[x]);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              rb::umma_f16_ss(t_s + bs * KT, dq + (((kk / 4) * (MT * 128) + (kk % 4) * 32) >> 4),
+                              dk + (((kk / 4) * (KT * 128) + (kk % 4) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+            rb::umma_commit(&bars->s_full[x][bs]);
+            rb::umma_commit(&bars->empty[st]);
+            if (e == n - 1) rb::umma_commit(&bars->q_empty);
+          }
+          if (++st == C::STAGES) { st = 0; par ^= 1; }
+          continue;
+        }
         const bool use_k = e < n && mine(e), use_v = m >= 0 && mine(m);
         if (!wait(&bars->full[st], par)) break;
         if (m >= 0 && (two || use_v)) {
