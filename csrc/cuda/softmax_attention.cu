@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
   float* ml = reinterpret_cast<float*>(tail + 1024);                           // [NW][RT][2]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nb = p.a.B + p.b.B;
+  launch_dependents();
   if (tid == 0) {
     for (int i = 0; i < NW * C::STAGES; ++i) rb::mbar_init(&bars[i], 1);
     *abort_flag = 0;
@@ -374,54 +375,63 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
     }
   }
   if (lane == 0 && (W == 1 || warp == 0)) w.meta[wk] = m;
+  if (tid == 0) wait_before();                                                 // what ran before is done when this kernel is
 }
 
-// Joins the pieces of the items that borders cut: block (c, y) looks after 16 rows of the item whose first border is share
-// c's begin.  Items have up to `block_rows` rows.
+// Joins the pieces of the items that borders cut: blocks (c, y) look after the item whose first border is share c's begin,
+// 16 rows at a time and four columns per thread.  Items have up to `block_rows` rows.  (Few blocks: most of them find nothing to
+// do, and it is their number that this kernel's time goes by.)
 template <int D, bool BF16>
-__global__ void __launch_bounds__(128) attn_join_kernel(const Batch p, const Outs w, int block_rows) {
+__global__ void __launch_bounds__(RT * D / 4) attn_join_kernel(const Batch p, const Outs w, int block_rows) {
+  launch_dependents();
+  wait_before();
   const Meta m = w.meta[blockIdx.x];
-  constexpr int TPR = 128 / RT, N = 4;
-  const int r = blockIdx.y * RT + threadIdx.x / TPR;
-  if (!m.valid || r >= m.rows) return;
+  if (!m.valid) return;
+  constexpr int STEP = 8;                                                      // pieces in flight
+  const int col = threadIdx.x % (D / 4) * 4;
   const Seq s = seq_of(p, m.seq);
-  auto cut = [&](int c) {
-    const long long b = share(c, m.n, m.total);
-    return (static_cast<long long>(c) * 2 + (b >= m.t0 ? 0 : 1)) * block_rows + r;
-  };
-  float mm = -INFINITY;
-  for (int c = m.c0; c <= m.c1; ++c) mm = fmaxf(mm, w.cut_lse[cut(c)]);
-  const float bm = mm == -INFINITY ? 0.f : mm;
-  float l = 0.f;
-  float x[D / (TPR * N)][N];
+  for (int r = blockIdx.y * RT + threadIdx.x / (D / 4); r < m.rows; r += gridDim.y * RT) {
+    // the first piece is its share's last unless the item begins the share, the others are their shares' first
+    const long long first = (static_cast<long long>(m.c0) * 2 + (share(m.c0, m.n, m.total) >= m.t0 ? 0 : 1)) * block_rows + r;
+    auto place = [&](int c) { return c == m.c0 ? first : static_cast<long long>(c) * 2 * block_rows + r; };
+    float mm = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = m.c0; c <= m.c1; c += STEP) {
+      float lse[STEP];
+      float4 y[STEP];
 #pragma unroll
-  for (int k = 0; k < D / (TPR * N); ++k) x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0.f;
-#pragma unroll 4
-  for (int c = m.c0; c <= m.c1; ++c) {
-    const long long at = cut(c);
-    const float f = exp2_approx(w.cut_lse[at] - bm);
-    l += f;
+      for (int i = 0; i < STEP; ++i) {
+        const long long at = place(min(c + i, m.c1));
+        lse[i] = c + i <= m.c1 ? w.cut_lse[at] : -INFINITY;
+        y[i] = *reinterpret_cast<const float4*>(w.cut_o + at * D + col);
+      }
+      float top = mm;
 #pragma unroll
-    for (int k = 0; k < D / (TPR * N); ++k) {
-      const float4 y = *reinterpret_cast<const float4*>(w.cut_o + at * D + (threadIdx.x % TPR) * N + k * TPR * N);
-      x[k][0] += f * y.x; x[k][1] += f * y.y; x[k][2] += f * y.z; x[k][3] += f * y.w;
+      for (int i = 0; i < STEP; ++i) top = fmaxf(top, lse[i]);
+      const float bm = top == -INFINITY ? 0.f : top, f0 = exp2_approx(mm - bm);
+      mm = top;
+      l *= f0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] *= f0;
+#pragma unroll
+      for (int i = 0; i < STEP; ++i) {
+        const float f = exp2_approx(lse[i] - bm);
+        l += f;
+        x[0] += f * y[i].x; x[1] += f * y[i].y; x[2] += f * y[i].z; x[3] += f * y[i].w;
+      }
     }
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const float lse2 = l == 0.f ? -INFINITY : mm + log2f(l);
-  const RowOut to = row_out(p, w, s, m.row0 + r, m.h, D, true, 0);
-  if (threadIdx.x % TPR == 0 && to.lse) *to.lse = to.natural ? lse2 * LN2 : lse2;
-#pragma unroll
-  for (int k = 0; k < D / (TPR * N); ++k) {
-    const int col = (threadIdx.x % TPR) * N + k * TPR * N;
-    if (to.o16) *reinterpret_cast<uint2*>(to.o16 + col) = make_uint2(pack16<BF16>(x[k][0] * inv, x[k][1] * inv), pack16<BF16>(x[k][2] * inv, x[k][3] * inv));
-    else *reinterpret_cast<float4*>(to.o32 + col) = make_float4(x[k][0] * inv, x[k][1] * inv, x[k][2] * inv, x[k][3] * inv);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float lse2 = l == 0.f ? -INFINITY : mm + log2f(l);
+    const RowOut to = row_out(p, w, s, m.row0 + r, m.h, D, true, 0);
+    if (col == 0 && to.lse) *to.lse = to.natural ? lse2 * LN2 : lse2;
+    if (to.o16) *reinterpret_cast<uint2*>(to.o16 + col) = make_uint2(pack16<BF16>(x[0] * inv, x[1] * inv), pack16<BF16>(x[2] * inv, x[3] * inv));
+    else *reinterpret_cast<float4*>(to.o32 + col) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
   }
 }
 
 // out = the two parts of every row (prefix, suffix), weighted by their sums
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) attn_merge_kernel(const Batch p, const Outs w) {
+  wait_before();
   constexpr int TPR = D / 4;
   const long long rows = static_cast<long long>(p.Tq) * p.H;
   const long long row = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / TPR;
@@ -486,20 +496,19 @@ Plan plan_of(long long Tq, int G, int B, int groups, float scale) {
 
 template <int D, bool BF16>
 int join(const Batch& p, const Outs& w, int shares, int block_rows, cudaStream_t st) {
-  attn_join_kernel<D, BF16><<<dim3(shares, block_rows / RT), 128, 0, st>>>(p, w, block_rows);
-  return static_cast<int>(cudaGetLastError());
+  return launch_kernel(true, attn_join_kernel<D, BF16>, dim3(shares, block_rows > RT ? 4 : 1), dim3(RT * D / 4), 0, st, p, w, block_rows);
 }
 
 template <int D, bool BF16, int W>
-int launch_rows(const CUtensorMap& tm, const Batch& p, const Outs& w, int n_cta, cudaStream_t st) {
+int launch_rows(const CUtensorMap& tm, const Batch& p, const Outs& w, int n_cta, bool after, cudaStream_t st) {
   RB_CUDA_CHECK(cudaFuncSetAttribute(attn_rows_kernel<D, BF16, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM));
-  attn_rows_kernel<D, BF16, W><<<n_cta, NW * 32, Cfg<D>::SMEM, st>>>(tm, p, w);
-  return static_cast<int>(cudaGetLastError());
+  return launch_kernel(after, attn_rows_kernel<D, BF16, W>, dim3(n_cta), dim3(NW * 32), Cfg<D>::SMEM, st, tm, p, w);
 }
 
 template <int D, bool BF16>
 int launch(const Batch& p, Outs w, const Plan& plan, const Space& sp, char* ws, const void* cache, int n_cta, cudaStream_t st) {
   const bool parts = p.b.B > 0;
+  bool after = false;
   for (int tiles = 0; tiles < 2; ++tiles) {
     Batch q = p;
     if (plan.tiles_a != (tiles != 0)) q.a.B = 0;
@@ -510,7 +519,7 @@ int launch(const Batch& p, Outs w, const Plan& plan, const Space& sp, char* ws, 
     w.meta = reinterpret_cast<Meta*>(ws + sp.meta[tiles]);
     int shares = n_cta;
     if (tiles) {
-      const int rc = launch_tiles(q, w, cache, D, BF16, n_cta, st);
+      const int rc = launch_tiles(q, w, cache, D, BF16, n_cta, after, st);
       if (rc) return rc;
     } else {
       CUtensorMap tm;
@@ -521,17 +530,18 @@ int launch(const Batch& p, Outs w, const Plan& plan, const Space& sp, char* ws, 
       // a worker per warp where the items (at least one per sequence and key head) go round at least a quarter of them
       const bool single = static_cast<long long>(q.a.B + q.b.B) * p.Hkv * 4 >= static_cast<long long>(n_cta) * NW;
       if (single) shares = n_cta * NW;
-      rc = single ? launch_rows<D, BF16, 1>(tm, q, w, n_cta, st) : launch_rows<D, BF16, NW>(tm, q, w, n_cta, st);
+      rc = single ? launch_rows<D, BF16, 1>(tm, q, w, n_cta, after, st) : launch_rows<D, BF16, NW>(tm, q, w, n_cta, after, st);
       if (rc) return rc;
     }
     const int rc = join<D, BF16>(q, w, shares, tiles ? TILE_ROWS : RT, st);
     if (rc) return rc;
+    after = true;
   }
   if (parts) {
     const long long rows = static_cast<long long>(p.Tq) * p.H;
     const int per = 256 / (D / 4);
-    attn_merge_kernel<D, BF16><<<static_cast<int>((rows + per - 1) / per), 256, 0, st>>>(p, w);
-    RB_CUDA_CHECK(cudaGetLastError());
+    const int rc = launch_kernel(true, attn_merge_kernel<D, BF16>, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(256), 0, st, p, w);
+    if (rc) return rc;
   }
   return 0;
 }

@@ -157,6 +157,27 @@ __device__ __forceinline__ RowOut row_out(const Batch& p, const Outs& w, const S
 // softmax_attention_tiles.cu: the kernel for many rows per sequence; fills out / part and the cut pieces (blocks of
 // TILE_ROWS rows) of all sequences of p
 constexpr int TILE_ROWS = 256;
-int launch_tiles(const Batch& p, const Outs& w, const void* cache, int D, bool is_bf16, int n_cta, cudaStream_t st);
+int launch_tiles(const Batch& p, const Outs& w, const void* cache, int D, bool is_bf16, int n_cta, bool after, cudaStream_t st);
+
+// The kernels of a call follow one another with programmatic launches: each lets the next one start early, and the next
+// one waits (for the whole of what ran before, and by that for what ran before that) where it needs its results.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// `after`: not the first kernel of a call (that one is ordered behind the caller's work as usual)
+template <typename... P, typename... A>
+int launch_kernel(bool after, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = after ? 1 : 0;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, static_cast<A&&>(args)...));
+}
 
 }  // namespace rb_attn

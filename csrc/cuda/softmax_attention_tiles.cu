@@ -138,6 +138,13 @@ __device__ __forceinline__ bool elect() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
   return ok != 0;
 }
+// (address 32-byte aligned)
+__device__ __forceinline__ void store32(void* to, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // rb::mbar_wait without the sleep between tries: the waits here are on the critical path and short
 __device__ __forceinline__ bool spin_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status) {
   for (uint32_t it = 0; it < WAIT; ++it) {
@@ -185,6 +192,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     rb::mbar_fence_init();
   }
   if (warp == 2) { rb::tmem_alloc(tmem_slot, 512); rb::tmem_relinquish(); }
+  launch_dependents();
 
   // ---- this CTA's share.  Blocks per sequence differ, so they are counted first and then dealt to the threads evenly.
   const int per = (nb + THREADS - 1) / THREADS;
@@ -672,14 +680,23 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = fmaf(f1, __uint_as_float(a[e]), o[e]);
           }
+          // 32 bytes a store: a row per thread means a line per lane, and what counts is how many stores there are
           if (live && dst16) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              *reinterpret_cast<uint4*>(dst16 + c + e) = make_uint4(pack16<BF16>(o[e], o[e + 1]), pack16<BF16>(o[e + 2], o[e + 3]),
-                                                                    pack16<BF16>(o[e + 4], o[e + 5]), pack16<BF16>(o[e + 6], o[e + 7]));
+            for (int e = 0; e < 32; e += 16) {
+              uint32_t v[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = pack16<BF16>(o[e + 2 * i], o[e + 2 * i + 1]);
+              store32(dst16 + c + e, v);
+            }
           } else if (live) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(dst32 + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int e = 0; e < 32; e += 8) {
+              uint32_t v[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(o[e + i]);
+              store32(dst32 + c + e, v);
+            }
           }
         }
       }
@@ -697,6 +714,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   rb::tc_fence_before();
   __syncthreads();
   if (warp == 2) rb::tmem_dealloc(tmem, 512);
+  if (tid == 0) wait_before();                                                // what ran before is done when this kernel is
 }
 
 // q as [Tq][H][D]: boxes of 64 elements x G heads x the tokens of a row tile
@@ -715,22 +733,21 @@ int make_map_q(CUtensorMap* map, const Batch& p, int D, int tpt, bool is_bf16) {
 }
 
 template <int D, bool BF16>
-int launch(const Batch& p, const Outs& w, const void* cache, int n_cta, cudaStream_t st) {
+int launch(const Batch& p, const Outs& w, const void* cache, int n_cta, bool after, cudaStream_t st) {
   CUtensorMap tq, tkv;
   int rc = make_map_q(&tq, p, D, MT / p.G, BF16);
   if (rc) return rc;
   rc = rb_host::make_map_2d(&tkv, cache, p.total_rows, static_cast<long long>(p.Hkv) * D, static_cast<long long>(p.Hkv) * D, 64, p.box_rows, BF16);
   if (rc) return rc;
   RB_CUDA_CHECK(cudaFuncSetAttribute(attn_tiles_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM));
-  attn_tiles_kernel<D, BF16><<<n_cta, THREADS, Cfg<D>::SMEM, st>>>(tq, tkv, p, w);
-  return static_cast<int>(cudaGetLastError());
+  return launch_kernel(after, attn_tiles_kernel<D, BF16>, dim3(n_cta), dim3(THREADS), Cfg<D>::SMEM, st, tq, tkv, p, w);
 }
 
 }  // namespace
 
-int rb_attn::launch_tiles(const Batch& batch, const Outs& w, const void* cache, int D, bool is_bf16, int n_cta, cudaStream_t st) {
+int rb_attn::launch_tiles(const Batch& batch, const Outs& w, const void* cache, int D, bool is_bf16, int n_cta, bool after, cudaStream_t st) {
   Batch p = batch;
   p.box_rows = p.page_size % 64 == 0 ? 64 : p.page_size % 32 == 0 ? 32 : 16;
-  if (D == 64) return is_bf16 ? launch<64, true>(p, w, cache, n_cta, st) : launch<64, false>(p, w, cache, n_cta, st);
-  return is_bf16 ? launch<128, true>(p, w, cache, n_cta, st) : launch<128, false>(p, w, cache, n_cta, st);
+  if (D == 64) return is_bf16 ? launch<64, true>(p, w, cache, n_cta, after, st) : launch<64, false>(p, w, cache, n_cta, after, st);
+  return is_bf16 ? launch<128, true>(p, w, cache, n_cta, after, st) : launch<128, false>(p, w, cache, n_cta, after, st);
 }
