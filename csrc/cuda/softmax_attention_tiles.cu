@@ -446,20 +446,26 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (!wait(&bars->q_full, par_q)) break;
       par_q ^= 1;
       const int ahead = two ? 2 : 4;
-      // steps whose K and V are both this row tile's and need no clearing
+      // steps whose V is this row tile's and needs no clearing
       const int clean0 = max(c_lo - skip, sink_tiles) - v0, clean1 = c_hi - skip - v0;
-      const int plain0 = two ? max(max(clean0, fi) + ahead, fi) : max(clean0, 0) + ahead;
-      const int plain1 = two ? min(min(clean1, en) + ahead, min(en, n)) : min(clean1 + ahead, n);
+      const int plain0 = max(clean0, two ? fi : 0) + ahead, plain1 = min(clean1, two ? min(en, n) : n) + ahead;
       const uint32_t q_at = (two ? x : 0) * (C::Q_TILE >> 4);
       for (int e = 0; e < n + ahead; ++e) {
         const int m = e - ahead;
-        if (e >= plain0 && e < plain1 && (two || (e & 1) == x) && started) {
+        if (!two && (e & 1) != x) {                                           // the other warp's step
+          if (!wait(&bars->full[st], par)) break;
+          if (e == n - 1 && elect()) rb::umma_commit(&bars->q_empty);
+          pass(false);
+          continue;
+        }
+        if (e >= plain0 && e < plain1 && started) {
           // the same as below, without its questions: this is where the time goes
+          const bool use_k = e < n && mine(e);
           if (!wait(&bars->full[st], par)) break;
           const uint32_t bp = n_p & 1, bs = n_s & 1;
           if (!wait(&bars->p_full[x][bp], (n_p >> 1) & 1)) break;
           ++n_p;
-          ++n_s;
+          n_s += use_k;
           rb::tc_fence_after();
           if (elect()) {
             const uint32_t at = st * (C::TILE >> 3);
@@ -467,11 +473,13 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
             for (int kk = 0; kk < KT / 16; ++kk) rb::umma_f16_ts(t_o, t_s + bp * KT + kk * 8, dv + kk * 128, idesc_o, 1u);
             rb::umma_commit(&bars->o_done[x]);
+            if (use_k) {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              rb::umma_f16_ss(t_s + bs * KT, dq + (((kk / 4) * (MT * 128) + (kk % 4) * 32) >> 4),
-                              dk + (((kk / 4) * (KT * 128) + (kk % 4) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
-            rb::umma_commit(&bars->s_full[x][bs]);
+              for (int kk = 0; kk < D / 16; ++kk)
+                rb::umma_f16_ss(t_s + bs * KT, dq + (((kk / 4) * (MT * 128) + (kk % 4) * 32) >> 4),
+                                dk + (((kk / 4) * (KT * 128) + (kk % 4) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+              rb::umma_commit(&bars->s_full[x][bs]);
+            }
             rb::umma_commit(&bars->empty[st]);
             if (e == n - 1) rb::umma_commit(&bars->q_empty);
           }
@@ -538,7 +546,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int row = quarter * 32 + lane;
     const uint32_t lane_sel = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t t_s = tmem + lane_sel + x * 128, t_o = tmem + lane_sel + 256 + x * 128;
-    const int my_tok = row / p.G;                                              // of the row tile
+    const int my_tok = row / p.G, my_head = row % p.G;                         // of the row tile, of the group
     uint32_t n_s = 0, par_o = 0, par_swap = 0;                                  // key tiles so far; bit y: of row tile y's o_full
     while (const Piece* q = next_piece()) {
       const bool two = q->two;
@@ -660,10 +668,25 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const int r_cut = two ? x * tpt * p.G + row : row;                      // row of the block
         const int tok = (two ? x * tpt : 0) + my_tok;
         const bool live = row < tpt * p.G && tok < q->tokens;
-        const RowOut to = row_out(p, w, q->s, q->t_lo * p.G + r_cut, q->h, D, q->whole != 0, static_cast<long long>(q->cut) * TILE_ROWS + r_cut);
-        if (live && c_lo == 0 && to.lse) *to.lse = to.natural ? lse2 * LN2 : lse2;
-        uint16_t* dst16 = to.o16;
-        float* dst32 = to.o32;
+        // where row_out would send it, without its divisions
+        const int t = q->s.q_begin + q->t_lo + tok, head = q->h * p.G + my_head;
+        uint16_t* dst16 = nullptr;
+        float *dst32 = nullptr, *dst_lse;
+        float lse = lse2;
+        if (!q->whole) {
+          const int cut = q->cut * TILE_ROWS + r_cut;
+          dst32 = w.cut_o + static_cast<long long>(cut) * D;
+          dst_lse = w.cut_lse + cut;
+        } else if (w.part_o) {
+          const long long at = (static_cast<long long>(q->s.part) * p.Tq + t) * p.H + head;
+          dst32 = w.part_o + at * D;
+          dst_lse = w.part_lse + at;
+        } else {
+          dst16 = reinterpret_cast<uint16_t*>(w.out) + t * w.ld_o + head * D;
+          dst_lse = w.lse ? w.lse + (static_cast<long long>(t) * p.H + head) : nullptr;
+          lse = lse2 * LN2;
+        }
+        if (live && c_lo == 0 && dst_lse) *dst_lse = lse;
 #pragma unroll 1
         for (int c = c_lo; c < c_hi; c += 32) {
           uint32_t a[32];
