@@ -149,229 +149,239 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
       if (pos >= base + n_b) { base += n_b; ++b; continue; }
       const int item = static_cast<int>((pos - base) / it.units);
       const int off = static_cast<int>(pos - base - static_cast<long long>(item) * it.units);
-      const int u1 = static_cast<int>(min(static_cast<long long>(it.units), off + (p1 - pos)));
-      const int qt = item / p.Hkv, h = item - qt * p.Hkv;
+      const int qt = item / p.Hkv, h0 = item - qt * p.Hkv;
       const int rows = min(s.len_q * p.G - qt * RT, RT);
       const Span sp = span_of<KT>(p, s, qt * RT / p.G, (qt * RT + rows - 1) / p.G);
       const long long t0 = pos - off;
       if (pos == p0 && off > 0 && begin_of(wk - 1) <= t0) {
         // the first border inside this item: the second kernel joins its pieces
-        m.valid = 1; m.seq = b; m.row0 = qt * RT; m.rows = rows; m.h = h; m.t0 = t0; m.total = total; m.n = n_sh;
+        m.valid = 1; m.seq = b; m.row0 = qt * RT; m.rows = rows; m.h = h0; m.t0 = t0; m.total = total; m.n = n_sh;
         m.c0 = wk - 1;
         m.c1 = static_cast<int>(((t0 + it.units) * n_sh - 1) / total);        // the share that holds the item's last unit
       }
-      // this warp's tiles: v0 + k * W for k < n
-      const int v0 = off * W + turn, n = (min(u1 * W, sp.tiles) - v0 + W - 1) / W;
-      int rows_at = 0, rows_box = 0;                                           // rows of the boxes of `batch` tiles from rows_at on
-      auto look_up = [&](int k) {
-        const int mine_k = k + lane / boxes;
-        rows_box = mine_k < n && lane < batch * boxes ? box_row(p, s, sp, sp.tile(v0 + mine_k * W) * KT + (lane % boxes) * p.box_rows) : p.total_rows;
-        rows_at = k;
-      };
-      auto issue = [&](int k) {
-        if (k == rows_at + batch) look_up(k);
-        const int row = __shfl_sync(0xffffffffu, rows_box, ((k - rows_at) * boxes + my_box) & 31) + my_kind * p.page_size;
+      // A warp on its own goes through all of its heads of the row tile in one: the ring runs on from one to the next.
+      const long long stop = min(p1, W == 1 ? t0 + static_cast<long long>(p.Hkv - h0) * it.units : t0 + it.units);
+      const int heads = W == 1 ? static_cast<int>((stop - t0 + it.units - 1) / it.units) : 1;
+      const int u_last = static_cast<int>(stop - t0 - static_cast<long long>(heads - 1) * it.units);   // units of the last head
+      // key tiles of head h0 + i: begin(i), begin(i) + W, ... below end(i)
+      auto begin = [&](int i) { return (i == 0 ? off * W : 0) + turn; };
+      auto end = [&](int i) { return min((i == heads - 1 ? u_last : it.units) * W, sp.tiles); };
+      int rows_at = -1, rows_box = 0;                                          // rows of the boxes of `batch` tiles from rows_at on
+      int in_h = 0, in_v = begin(0);                                           // the next tile to load
+      auto issue = [&]() {
+        while (in_v >= end(in_h)) {
+          if (++in_h >= heads) return;
+          in_v = begin(in_h);
+        }
+        if (rows_at < 0 || in_v < rows_at || in_v >= rows_at + batch * W) {
+          rows_at = in_v;
+          const int mine_v = in_v + lane / boxes * W;
+          rows_box = mine_v < sp.tiles && lane < batch * boxes ? box_row(p, s, sp, sp.tile(mine_v) * KT + (lane % boxes) * p.box_rows) : p.total_rows;
+        }
+        const int row = __shfl_sync(0xffffffffu, rows_box, ((in_v - rows_at) / W * boxes + my_box) & 31) + my_kind * p.page_size;
         if (lane == 0) rb::mbar_expect_tx(&bar[st_in], 2 * C::TILE);
         __syncwarp();
         if (my_kind < 2)
           rb::tma_load_2d(ring + (st_in * 2 + my_kind) * C::TILE + my_chunk * (KT * 128) + my_box * p.box_rows * 128, &tm, &bar[st_in],
-                          h * D + my_chunk * 64, row);
+                          (h0 + in_h) * D + my_chunk * 64, row);
+        in_v += W;
         ++issued;
         if (++st_in == C::STAGES) st_in = 0;
       };
-      if (n > 0) look_up(0);
-      int nxt = 0;
-      for (; nxt < min(n, C::STAGES) && !dead; ++nxt) issue(nxt);
-      // ---- the 16 query rows as A fragments: this thread's rows are lane / 4 and lane / 4 + 8
-      uint32_t qf[D / 16][4];
-      int rpos[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = (lane >> 2) + 8 * e;
-        const bool live = r < rows;
-        const int row = qt * RT + (live ? r : 0);
-        rpos[e] = row / p.G + s.delta();
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (s.q_begin + row / p.G) * p.ld_q +
-                              static_cast<long long>(h * p.G + row % p.G) * D + (lane & 3) * 2;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          qf[kk][e] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16)) : 0u;
-          qf[kk][e + 2] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16 + 8)) : 0u;
-        }
-      }
-      float o[D / 8][4];
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-      float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-      for (int k = 0; k < n && !dead; ++k) {
-        const bool ok = rb::mbar_wait(&bar[st_out], par, abort_flag, p.status);
-        if (!__all_sync(0xffffffffu, ok)) { dead = true; break; }
-        ++used;
-        const uint32_t k_addr = rb::smem_u32(ring + st_out * 2 * C::TILE), v_addr = k_addr + C::TILE;
-        const int j0 = sp.tile(v0 + k * W) * KT;
-        const bool full = (s.causal ? j0 + KT - 1 <= sp.p_min : j0 + KT <= sp.hi) &&
-                          (!s.causal || p.window <= 0 || j0 > sp.p_max - p.window || j0 + KT <= p.sinks);
-        float sc[KT / 8][4];
-#pragma unroll
-        for (int i = 0; i < KT / 8; ++i) sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.f;
-        // S = Q K^T: ldmatrix x4 = 16 keys x 16 columns
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-#pragma unroll
-          for (int i = 0; i < KT / 16; ++i) {
-            const int r = i * 16 + (lane & 7) + ((lane >> 4) << 3);
-            const int unit = (kk & 3) * 2 + ((lane >> 3) & 1);
-            uint32_t b0, b1, b2, b3;
-            ldsm4(k_addr + (kk >> 2) * (KT * 128) + r * 128 + ((unit ^ (r & 7)) << 4), b0, b1, b2, b3);
-            mma16816<BF16>(sc[2 * i], qf[kk], b0, b1);
-            mma16816<BF16>(sc[2 * i + 1], qf[kk], b2, b3);
-          }
-        }
-        float mn[2] = {mx[0], mx[1]};
-#pragma unroll
-        for (int i = 0; i < KT / 8; ++i) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = sc[i][e] * p.scale_log2;
-            if (!full) {
-              const int j = j0 + i * 8 + (lane & 3) * 2 + (e & 1);
-              if (!sees(rpos[e >> 1], j, s.len_k, s.causal, p.window, p.sinks)) x = -INFINITY;
-            }
-            sc[i][e] = x;
-            mn[e >> 1] = fmaxf(mn[e >> 1], x);
-          }
-        }
-        float corr[2], base_m[2];
+      if (!dead) for (int i = 0; i < C::STAGES && in_h < heads; ++i) issue();
+      for (int ih = 0; ih < heads; ++ih) {
+        const int h = h0 + ih;
+        // ---- the 16 query rows as A fragments: this thread's rows are lane / 4 and lane / 4 + 8
+        uint32_t qf[D / 16][4];
+        int rpos[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          mn[e] = fmaxf(mn[e], __shfl_xor_sync(0xffffffffu, mn[e], 1));
-          mn[e] = fmaxf(mn[e], __shfl_xor_sync(0xffffffffu, mn[e], 2));
-          base_m[e] = mn[e] == -INFINITY ? 0.f : mn[e];
-          corr[e] = exp2_approx(mx[e] - base_m[e]);
-          mx[e] = mn[e];
-          sum[e] *= corr[e];
-        }
-        uint32_t pf[KT / 16][4];
+          const int r = (lane >> 2) + 8 * e;
+          const bool live = r < rows;
+          const int row = qt * RT + (live ? r : 0);
+          rpos[e] = row / p.G + s.delta();
+          const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (s.q_begin + row / p.G) * p.ld_q +
+                                static_cast<long long>(h * p.G + row % p.G) * D + (lane & 3) * 2;
 #pragma unroll
-        for (int i = 0; i < KT / 8; ++i) {
-          float x[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = exp2_approx(sc[i][e] - base_m[e >> 1]);
-            sum[e >> 1] += x[e];
+          for (int kk = 0; kk < D / 16; ++kk) {
+            qf[kk][e] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16)) : 0u;
+            qf[kk][e + 2] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16 + 8)) : 0u;
           }
-          pf[i >> 1][(i & 1) * 2] = pack16<BF16>(x[0], x[1]);
-          pf[i >> 1][(i & 1) * 2 + 1] = pack16<BF16>(x[2], x[3]);
         }
+        float o[D / 8][4];
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1];
-        }
-        if (!full) {
-          // V of keys that no row of the block sees may be anything (0 x NaN is NaN): clear it
-          const int j = j0 + lane;
-          if (lane < KT && !(j < sp.hi && (j >= sp.lo || j < sp.sinks))) {
-            uint4* vr = reinterpret_cast<uint4*>(ring + (st_out * 2 + 1) * C::TILE + lane * 128);
+        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+        for (int v = begin(ih); v < end(ih) && !dead; v += W) {
+          const bool ok = rb::mbar_wait(&bar[st_out], par, abort_flag, p.status);
+          if (!__all_sync(0xffffffffu, ok)) { dead = true; break; }
+          ++used;
+          const uint32_t k_addr = rb::smem_u32(ring + st_out * 2 * C::TILE), v_addr = k_addr + C::TILE;
+          const int j0 = sp.tile(v) * KT;
+          const bool full = (s.causal ? j0 + KT - 1 <= sp.p_min : j0 + KT <= sp.hi) &&
+                            (!s.causal || p.window <= 0 || j0 > sp.p_max - p.window || j0 + KT <= p.sinks);
+          float sc[KT / 8][4];
 #pragma unroll
-            for (int c = 0; c < C::CH; ++c)
+          for (int i = 0; i < KT / 8; ++i) sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.f;
+          // S = Q K^T: ldmatrix x4 = 16 keys x 16 columns
 #pragma unroll
-              for (int i = 0; i < 8; ++i) vr[c * (KT * 8) + ((i + lane) & 7)] = make_uint4(0, 0, 0, 0);
+          for (int kk = 0; kk < D / 16; ++kk) {
+#pragma unroll
+            for (int i = 0; i < KT / 16; ++i) {
+              const int r = i * 16 + (lane & 7) + ((lane >> 4) << 3);
+              const int unit = (kk & 3) * 2 + ((lane >> 3) & 1);
+              uint32_t b0, b1, b2, b3;
+              ldsm4(k_addr + (kk >> 2) * (KT * 128) + r * 128 + ((unit ^ (r & 7)) << 4), b0, b1, b2, b3);
+              mma16816<BF16>(sc[2 * i], qf[kk], b0, b1);
+              mma16816<BF16>(sc[2 * i + 1], qf[kk], b2, b3);
+            }
           }
-          rb::fence_proxy_async_smem();
+          float mn[2] = {mx[0], mx[1]};
+#pragma unroll
+          for (int i = 0; i < KT / 8; ++i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float x = sc[i][e] * p.scale_log2;
+              if (!full) {
+                const int j = j0 + i * 8 + (lane & 3) * 2 + (e & 1);
+                if (!sees(rpos[e >> 1], j, s.len_k, s.causal, p.window, p.sinks)) x = -INFINITY;
+              }
+              sc[i][e] = x;
+              mn[e >> 1] = fmaxf(mn[e >> 1], x);
+            }
+          }
+          float corr[2], base_m[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            mn[e] = fmaxf(mn[e], __shfl_xor_sync(0xffffffffu, mn[e], 1));
+            mn[e] = fmaxf(mn[e], __shfl_xor_sync(0xffffffffu, mn[e], 2));
+            base_m[e] = mn[e] == -INFINITY ? 0.f : mn[e];
+            corr[e] = exp2_approx(mx[e] - base_m[e]);
+            mx[e] = mn[e];
+            sum[e] *= corr[e];
+          }
+          uint32_t pf[KT / 16][4];
+#pragma unroll
+          for (int i = 0; i < KT / 8; ++i) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[e] = exp2_approx(sc[i][e] - base_m[e >> 1]);
+              sum[e >> 1] += x[e];
+            }
+            pf[i >> 1][(i & 1) * 2] = pack16<BF16>(x[0], x[1]);
+            pf[i >> 1][(i & 1) * 2 + 1] = pack16<BF16>(x[2], x[3]);
+          }
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1];
+          }
+          if (!full) {
+            // V of keys that no row of the block sees may be anything (0 x NaN is NaN): clear it
+            const int j = j0 + lane;
+            if (lane < KT && !(j < sp.hi && (j >= sp.lo || j < sp.sinks))) {
+              uint4* vr = reinterpret_cast<uint4*>(ring + (st_out * 2 + 1) * C::TILE + lane * 128);
+#pragma unroll
+              for (int c = 0; c < C::CH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) vr[c * (KT * 8) + ((i + lane) & 7)] = make_uint4(0, 0, 0, 0);
+            }
+            rb::fence_proxy_async_smem();
+            __syncwarp();
+          }
+          // O += P V
+#pragma unroll
+          for (int kk = 0; kk < KT / 16; ++kk) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              const int r = kk * 16 + (lane & 15);
+              const int unit = (i & 3) * 2 + (lane >> 4);
+              uint32_t b0, b1, b2, b3;
+              ldsm4_trans(v_addr + (i >> 2) * (KT * 128) + r * 128 + ((unit ^ (r & 7)) << 4), b0, b1, b2, b3);
+              mma16816<BF16>(o[2 * i], pf[kk], b0, b1);
+              mma16816<BF16>(o[2 * i + 1], pf[kk], b2, b3);
+            }
+          }
           __syncwarp();
+          if (++st_out == C::STAGES) { st_out = 0; par ^= 1; }
+          if (in_h < heads) issue();
         }
-        // O += P V
-#pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk) {
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            const int r = kk * 16 + (lane & 15);
-            const int unit = (i & 3) * 2 + (lane >> 4);
-            uint32_t b0, b1, b2, b3;
-            ldsm4_trans(v_addr + (i >> 2) * (KT * 128) + r * 128 + ((unit ^ (r & 7)) << 4), b0, b1, b2, b3);
-            mma16816<BF16>(o[2 * i], pf[kk], b0, b1);
-            mma16816<BF16>(o[2 * i + 1], pf[kk], b2, b3);
+        if (dead) {                                                              // the kernel's own copies end before it does
+          for (; used < issued; ++used) {
+            for (uint32_t i = 0; i < (1u << 20) && !rb::mbar_try_wait(&bar[st_out], par); ++i) {}
+            if (++st_out == C::STAGES) { st_out = 0; par ^= 1; }
           }
         }
-        __syncwarp();
-        if (++st_out == C::STAGES) { st_out = 0; par ^= 1; }
-        if (nxt < n) issue(nxt++);
-      }
-      if (dead) {                                                              // the kernel's own copies end before it does
-        for (; used < issued; ++used) {
-          for (uint32_t i = 0; i < (1u << 20) && !rb::mbar_try_wait(&bar[st_out], par); ++i) {}
-          if (++st_out == C::STAGES) { st_out = 0; par ^= 1; }
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
-        sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
-      }
-      const bool whole = off == 0 && u1 == it.units;
-      const long long cut = static_cast<long long>(wk) * 2 + (pos == p0 ? 0 : 1);
-      if (W == 1) {
-        // ---- the warp's own result, straight from the fragments
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int r = (lane >> 2) + 8 * e;
-          if (r < rows) {
-            const float inv = sum[e] == 0.f ? 0.f : 1.f / sum[e];
-            const float lse2 = sum[e] == 0.f ? -INFINITY : mx[e] + log2f(sum[e]);
-            const RowOut to = row_out(p, w, s, qt * RT + r, h, D, whole, cut * RT + r);
-            if ((lane & 3) == 0 && to.lse) *to.lse = to.natural ? lse2 * LN2 : lse2;
+          sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
+          sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
+        }
+        const bool whole = (ih > 0 || off == 0) && (ih < heads - 1 || u_last == it.units);
+        const long long cut = static_cast<long long>(wk) * 2 + (pos == p0 && ih == 0 ? 0 : 1);
+        if (W == 1) {
+          // ---- the warp's own result, straight from the fragments
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-              const float x = o[i][2 * e] * inv, y = o[i][2 * e + 1] * inv;
-              const int col = i * 8 + (lane & 3) * 2;
-              if (to.o16) *reinterpret_cast<uint32_t*>(to.o16 + col) = pack16<BF16>(x, y);
-              else *reinterpret_cast<float2*>(to.o32 + col) = make_float2(x, y);
+          for (int e = 0; e < 2; ++e) {
+            const int r = (lane >> 2) + 8 * e;
+            if (r < rows) {
+              const float inv = sum[e] == 0.f ? 0.f : 1.f / sum[e];
+              const float lse2 = sum[e] == 0.f ? -INFINITY : mx[e] + log2f(sum[e]);
+              const RowOut to = row_out(p, w, s, qt * RT + r, h, D, whole, cut * RT + r);
+              if ((lane & 3) == 0 && to.lse) *to.lse = to.natural ? lse2 * LN2 : lse2;
+#pragma unroll
+              for (int i = 0; i < D / 8; ++i) {
+                const float x = o[i][2 * e] * inv, y = o[i][2 * e + 1] * inv;
+                const int col = i * 8 + (lane & 3) * 2;
+                if (to.o16) *reinterpret_cast<uint32_t*>(to.o16 + col) = pack16<BF16>(x, y);
+                else *reinterpret_cast<float2*>(to.o32 + col) = make_float2(x, y);
+              }
             }
           }
-        }
-      } else {
-        // ---- join the warps: o [RT][D] in the warp's own, now idle ring
+        } else {
+          // ---- join the warps: o [RT][D] in the warp's own, now idle ring
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = (lane >> 2) + 8 * e;
-          float* dst = reinterpret_cast<float*>(ring) + r * D + (lane & 3) * 2;
+          for (int e = 0; e < 2; ++e) {
+            const int r = (lane >> 2) + 8 * e;
+            float* dst = reinterpret_cast<float*>(ring) + r * D + (lane & 3) * 2;
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
-          if ((lane & 3) == 0) { ml[(warp * RT + r) * 2] = mx[e]; ml[(warp * RT + r) * 2 + 1] = sum[e]; }
-        }
-        __syncthreads();
-        constexpr int TPR = NW * 32 / RT, N = 4;                               // threads per row, elements at a time
-        const int r = tid / TPR;
-        if (r < rows) {
-          float mm = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < NW; ++i) mm = fmaxf(mm, ml[(i * RT + r) * 2]);
-          const float bm = mm == -INFINITY ? 0.f : mm;
-          float f[NW], l = 0.f;
-#pragma unroll
-          for (int i = 0; i < NW; ++i) {
-            f[i] = exp2_approx(ml[(i * RT + r) * 2] - bm);
-            l += f[i] * ml[(i * RT + r) * 2 + 1];
+            for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
+            if ((lane & 3) == 0) { ml[(warp * RT + r) * 2] = mx[e]; ml[(warp * RT + r) * 2 + 1] = sum[e]; }
           }
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          const float lse2 = l == 0.f ? -INFINITY : mm + log2f(l);
-          const RowOut to = row_out(p, w, s, qt * RT + r, h, D, whole, cut * RT + r);
-          if (tid % TPR == 0 && to.lse) *to.lse = to.natural ? lse2 * LN2 : lse2;
-          for (int col = (tid % TPR) * N; col < D; col += TPR * N) {
-            float x[N] = {0.f, 0.f, 0.f, 0.f};
+          __syncthreads();
+          constexpr int TPR = NW * 32 / RT, N = 4;                               // threads per row, elements at a time
+          const int r = tid / TPR;
+          if (r < rows) {
+            float mm = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) mm = fmaxf(mm, ml[(i * RT + r) * 2]);
+            const float bm = mm == -INFINITY ? 0.f : mm;
+            float f[NW], l = 0.f;
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
-              const float4 y = *reinterpret_cast<const float4*>(smem + i * C::WARP_RING + (r * D + col) * 4);
-              x[0] += f[i] * y.x; x[1] += f[i] * y.y; x[2] += f[i] * y.z; x[3] += f[i] * y.w;
+              f[i] = exp2_approx(ml[(i * RT + r) * 2] - bm);
+              l += f[i] * ml[(i * RT + r) * 2 + 1];
             }
-            if (to.o16) *reinterpret_cast<uint2*>(to.o16 + col) = make_uint2(pack16<BF16>(x[0] * inv, x[1] * inv), pack16<BF16>(x[2] * inv, x[3] * inv));
-            else *reinterpret_cast<float4*>(to.o32 + col) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float lse2 = l == 0.f ? -INFINITY : mm + log2f(l);
+            const RowOut to = row_out(p, w, s, qt * RT + r, h, D, whole, cut * RT + r);
+            if (tid % TPR == 0 && to.lse) *to.lse = to.natural ? lse2 * LN2 : lse2;
+            for (int col = (tid % TPR) * N; col < D; col += TPR * N) {
+              float x[N] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int i = 0; i < NW; ++i) {
+                const float4 y = *reinterpret_cast<const float4*>(smem + i * C::WARP_RING + (r * D + col) * 4);
+                x[0] += f[i] * y.x; x[1] += f[i] * y.y; x[2] += f[i] * y.z; x[3] += f[i] * y.w;
+              }
+              if (to.o16) *reinterpret_cast<uint2*>(to.o16 + col) = make_uint2(pack16<BF16>(x[0] * inv, x[1] * inv), pack16<BF16>(x[2] * inv, x[3] * inv));
+              else *reinterpret_cast<float4*>(to.o32 + col) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+            }
           }
+          rb::fence_proxy_async_smem();
+          __syncthreads();
         }
-        rb::fence_proxy_async_smem();
-        __syncthreads();
       }
-      pos += u1 - off;
+      pos = stop;
     }
   }
   if (lane == 0 && (W == 1 || warp == 0)) w.meta[wk] = m;
