@@ -112,11 +112,10 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
     if (i < warp) before += sums[i];
     total += sums[i];
   }
-  const int n_sh = static_cast<int>(min(static_cast<long long>(gridDim.x) * PER_CTA, total));   // no share is empty
-  auto begin_of = [&](int c) { return c < n_sh ? share(c, n_sh, total) : total; };
+  const Shares sh(total, gridDim.x * PER_CTA);
   for (int x = 0; x < PER_CTA; ++x) {
     const int c = blockIdx.x * PER_CTA + x;
-    const long long at = c < n_sh ? share(c, n_sh, total) : -1;
+    const long long at = c < sh.n ? sh.begin(c) : -1;
     if (at >= before && at < before + mine) {
       long long base = before;
       for (int i = tid * per;; ++i) {
@@ -129,7 +128,7 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
   __syncthreads();
   const int me = W == 1 ? warp : 0, turn = W == 1 ? 0 : warp;                  // worker of the CTA, this warp's turn in it
   const int wk = blockIdx.x * PER_CTA + me;
-  const long long p0 = wk < n_sh ? begin_of(wk) : 0, p1 = wk < n_sh ? begin_of(wk + 1) : 0;
+  const long long p0 = wk < sh.n ? sh.begin(wk) : 0, p1 = wk < sh.n ? sh.begin(wk + 1) : 0;
   Meta m;
   m.valid = 0;
   if (p0 < p1) {
@@ -153,11 +152,12 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
       const int rows = min(s.len_q * p.G - qt * RT, RT);
       const Span sp = span_of<KT>(p, s, qt * RT / p.G, (qt * RT + rows - 1) / p.G);
       const long long t0 = pos - off;
-      if (pos == p0 && off > 0 && begin_of(wk - 1) <= t0) {
+      if (pos == p0 && off > 0 && sh.begin(wk - 1) <= t0) {
         // the first border inside this item: the second kernel joins its pieces
-        m.valid = 1; m.seq = b; m.row0 = qt * RT; m.rows = rows; m.h = h0; m.t0 = t0; m.total = total; m.n = n_sh;
+        m.valid = 1; m.seq = b; m.row0 = qt * RT; m.rows = rows; m.h = h0;
         m.c0 = wk - 1;
-        m.c1 = static_cast<int>(((t0 + it.units) * n_sh - 1) / total);        // the share that holds the item's last unit
+        m.c1 = sh.of(t0 + it.units - 1);
+        m.first = 2 * m.c0 + (sh.begin(m.c0) == t0 ? 0 : 1);                  // its share's first piece or its last
       }
       // A warp on its own goes through all of its heads of the row tile in one: the ring runs on from one to the next.
       const long long stop = min(p1, W == 1 ? t0 + static_cast<long long>(p.Hkv - h0) * it.units : t0 + it.units);
@@ -189,23 +189,29 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
         if (++st_in == C::STAGES) st_in = 0;
       };
       if (!dead) for (int i = 0; i < C::STAGES && in_h < heads; ++i) issue();
+      // this thread's rows of the 16: lane / 4 and lane / 4 + 8
+      bool live[2];
+      int rtok[2], rhead[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = (lane >> 2) + 8 * e;
+        live[e] = r < rows;
+        const int row = qt * RT + (live[e] ? r : 0);
+        rtok[e] = row / p.G;
+        rhead[e] = row - rtok[e] * p.G;
+      }
       for (int ih = 0; ih < heads; ++ih) {
         const int h = h0 + ih;
-        // ---- the 16 query rows as A fragments: this thread's rows are lane / 4 and lane / 4 + 8
+        // ---- the 16 query rows as A fragments
         uint32_t qf[D / 16][4];
-        int rpos[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int r = (lane >> 2) + 8 * e;
-          const bool live = r < rows;
-          const int row = qt * RT + (live ? r : 0);
-          rpos[e] = row / p.G + s.delta();
-          const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (s.q_begin + row / p.G) * p.ld_q +
-                                static_cast<long long>(h * p.G + row % p.G) * D + (lane & 3) * 2;
+          const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (s.q_begin + rtok[e]) * p.ld_q +
+                                static_cast<long long>(h * p.G + rhead[e]) * D + (lane & 3) * 2;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            qf[kk][e] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16)) : 0u;
-            qf[kk][e + 2] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16 + 8)) : 0u;
+            qf[kk][e] = live[e] ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16)) : 0u;
+            qf[kk][e + 2] = live[e] ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16 + 8)) : 0u;
           }
         }
         float o[D / 8][4];
@@ -237,15 +243,17 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
             }
           }
           float mn[2] = {mx[0], mx[1]};
+          uint32_t seen[2] = {~0u, ~0u};                                       // bit j: the row sees key j0 + (lane & 3) * 2 + j
+          if (!full) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) seen[e] = seen_keys(rtok[e] + s.delta(), j0, s.len_k, s.causal, p.window, p.sinks) >> ((lane & 3) * 2);
+          }
 #pragma unroll
           for (int i = 0; i < KT / 8; ++i) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float x = sc[i][e] * p.scale_log2;
-              if (!full) {
-                const int j = j0 + i * 8 + (lane & 3) * 2 + (e & 1);
-                if (!sees(rpos[e >> 1], j, s.len_k, s.causal, p.window, p.sinks)) x = -INFINITY;
-              }
+              if (!(seen[e >> 1] & (1u << (i * 8 + (e & 1))))) x = -INFINITY;
               sc[i][e] = x;
               mn[e >> 1] = fmaxf(mn[e >> 1], x);
             }
@@ -276,7 +284,7 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
           for (int i = 0; i < D / 8; ++i) {
             o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1];
           }
-          if (!full) {
+          if (!(j0 + KT <= sp.hi && (j0 >= sp.lo || j0 + KT <= sp.sinks))) {
             // V of keys that no row of the block sees may be anything (0 x NaN is NaN): clear it
             const int j = j0 + lane;
             if (lane < KT && !(j < sp.hi && (j >= sp.lo || j < sp.sinks))) {
@@ -324,7 +332,7 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int r = (lane >> 2) + 8 * e;
-            if (r < rows) {
+            if (live[e]) {
               const float inv = sum[e] == 0.f ? 0.f : 1.f / sum[e];
               const float lse2 = sum[e] == 0.f ? -INFINITY : mx[e] + log2f(sum[e]);
               const RowOut to = row_out(p, w, s, qt * RT + r, h, D, whole, cut * RT + r);
@@ -401,18 +409,20 @@ __global__ void __launch_bounds__(RT * D / 4) attn_join_kernel(const Batch p, co
   const int col = threadIdx.x % (D / 4) * 4;
   const Seq s = seq_of(p, m.seq);
   for (int r = blockIdx.y * RT + threadIdx.x / (D / 4); r < m.rows; r += gridDim.y * RT) {
-    // the first piece is its share's last unless the item begins the share, the others are their shares' first
-    const long long first = (static_cast<long long>(m.c0) * 2 + (share(m.c0, m.n, m.total) >= m.t0 ? 0 : 1)) * block_rows + r;
-    auto place = [&](int c) { return c == m.c0 ? first : static_cast<long long>(c) * 2 * block_rows + r; };
+    auto place = [&](int c) { return static_cast<long long>(c == m.c0 ? m.first : 2 * c) * block_rows + r; };
     float mm = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
     for (int c = m.c0; c <= m.c1; c += STEP) {
       float lse[STEP];
       float4 y[STEP];
 #pragma unroll
       for (int i = 0; i < STEP; ++i) {
-        const long long at = place(min(c + i, m.c1));
-        lse[i] = c + i <= m.c1 ? w.cut_lse[at] : -INFINITY;
-        y[i] = *reinterpret_cast<const float4*>(w.cut_o + at * D + col);
+        lse[i] = -INFINITY;
+        y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c + i <= m.c1) {
+          const long long at = place(c + i);
+          lse[i] = w.cut_lse[at];
+          y[i] = *reinterpret_cast<const float4*>(w.cut_o + at * D + col);
+        }
       }
       float top = mm;
 #pragma unroll
@@ -506,7 +516,7 @@ Plan plan_of(long long Tq, int G, int B, int groups, float scale) {
 
 template <int D, bool BF16>
 int join(const Batch& p, const Outs& w, int shares, int block_rows, cudaStream_t st) {
-  return launch_kernel(true, attn_join_kernel<D, BF16>, dim3(shares, block_rows > RT ? 4 : 1), dim3(RT * D / 4), 0, st, p, w, block_rows);
+  return launch_kernel(true, attn_join_kernel<D, BF16>, dim3(shares, block_rows > RT ? 8 : 1), dim3(RT * D / 4), 0, st, p, w, block_rows);
 }
 
 template <int D, bool BF16, int W>

@@ -89,9 +89,12 @@ __device__ __forceinline__ Span span_of(const Batch& p, const Seq& s, int t_lo, 
   return r;
 }
 
-// whether the row at position pos sees key j (j < len_k)
-__device__ __forceinline__ bool sees(int pos, int j, int hi, int causal, int window, int sinks) {
-  return j < hi && (!causal || (j <= pos && (window <= 0 || j > pos - window || j < sinks)));
+// Which of the keys j0 .. j0 + 31 the row at position pos sees: bit i for key j0 + i
+__device__ __forceinline__ uint32_t seen_keys(int pos, int j0, int len_k, int causal, int window, int sinks) {
+  auto below = [&](int n) { const int d = n - j0; return d >= 32 ? 0xffffffffu : d <= 0 ? 0u : (1u << d) - 1u; };
+  uint32_t seen = below(causal ? min(pos + 1, len_k) : len_k);
+  if (causal && window > 0) seen &= ~below(pos - window + 1) | below(sinks);
+  return seen;
 }
 
 // Row of the cache matrix where the box of keys j.. starts (K; V is page_size rows further), or a row past the end, which
@@ -118,12 +121,24 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 
 // The keys of all items (sequence, block of rows, key head) are laid end to end in units and cut into as many equal shares as
-// there are CTAs; none is empty.  Share c begins at share(c).
-__device__ __forceinline__ long long share(int c, int n, long long total) { return total * c / n; }
+// there are workers; none is empty.
+struct Shares {
+  long long total, q;                      // q = total / n
+  uint32_t r;                              // total % n
+  int n;
+  __device__ __forceinline__ Shares(long long units, int workers) : total(units), n(static_cast<int>(min(static_cast<long long>(workers), units))) {
+    q = n ? units / n : 0;                 // the one division of 64 bits
+    r = static_cast<uint32_t>(units - q * n);
+  }
+  // floor(total * c / n): where share c begins
+  __device__ __forceinline__ long long begin(int c) const { return c < n ? q * c + r * static_cast<uint32_t>(c) / static_cast<uint32_t>(n) : total; }
+  // the share that holds a unit
+  __device__ __forceinline__ int of(long long unit) const { return static_cast<int>(((unit + 1) * n - 1) / total); }
+};
 
 // Rows [row0, row0 + rows) of a sequence (packed: token * G + head of the group) whose units shares c0..c1 hold; left by
 // the share c0 + 1 for the kernel that joins the pieces.
-struct Meta { int valid, seq, row0, rows, h, c0, c1, n; long long t0, total; };
+struct Meta { int valid, seq, row0, rows, h, c0, c1, first; };   // first: piece c0's place, 2 * c0 or 2 * c0 + 1
 
 struct Outs {
   void* out; long long ld_o; float* lse;   // final results: 16-bit rows [Tq][ld_o], lse [Tq][H] or null

@@ -60,8 +60,8 @@ __device__ __forceinline__ Block block_of(const Batch& p, const Seq& s, int i, i
 
 // The pieces of this CTA's share, one after another; every role walks its own copy.
 struct Walk {
-  int seq, block, n_sh;
-  long long base, pos, p0, p1, total;   // base: begin of the block's items (Hkv of them)
+  int seq, block;
+  long long base, pos, p0, p1;          // base: begin of the block's items (Hkv of them)
   // the current piece
   Seq s;
   Block b;
@@ -257,11 +257,10 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     total += wsum[i];
   }
   const int cta = blockIdx.x;
-  const int n_sh = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+  const Shares sh(total, gridDim.x);
   Walk walk;
-  walk.n_sh = n_sh; walk.total = total;
-  walk.p0 = cta < n_sh ? share(cta, n_sh, total) : 0;
-  walk.p1 = cta < n_sh ? share(cta + 1, n_sh, total) : 0;
+  walk.p0 = cta < sh.n ? sh.begin(cta) : 0;
+  walk.p1 = cta < sh.n ? sh.begin(cta + 1) : 0;
   if (walk.p0 < walk.p1 && before <= walk.p0 && walk.p0 < before + mine) {
     long long base = before;
     each([&](int sq, int bl, long long n) {
@@ -333,11 +332,12 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           q.whole = walk.u0 <= FIXED && walk.u1 == b.units;
           q.cut = cta * 2 + (walk.pos == walk.p0 ? 0 : 1);
           const long long t0 = walk.pos - walk.u0;
-          if (walk.pos == walk.p0 && walk.u0 > FIXED && share(cta - 1, n_sh, total) <= t0 + FIXED) {
+          if (walk.pos == walk.p0 && walk.u0 > FIXED && sh.begin(cta - 1) <= t0 + FIXED) {
             // the first border between this item's tiles: another kernel joins its pieces
             mt.valid = 1; mt.seq = walk.seq; mt.row0 = b.t_lo * p.G; mt.rows = b.tokens * p.G; mt.h = walk.h;
-            mt.t0 = t0; mt.total = total; mt.n = n_sh; mt.c0 = cta - 1;
-            mt.c1 = static_cast<int>(((t0 + b.units) * n_sh - 1) / total);
+            mt.c0 = cta - 1;
+            mt.c1 = sh.of(t0 + b.units - 1);
+            mt.first = 2 * mt.c0 + (sh.begin(mt.c0) >= t0 ? 0 : 1);           // its share's first piece or its last
           }
           walk.done();
         }
@@ -558,10 +558,6 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const int se = q->sink_end[x], fi = q->first[x], en = q->end[x];
         const int full_s = q->full_sinks, full_lo = q->full_lo, full_hi = q->full_hi;
         const int pos = q->t_lo + (two ? x * tpt : 0) + my_tok + q->s.delta();
-        // this row sees the keys below `upto`, of those the ones from `from` on and the sinks
-        const int upto = q->s.causal ? min(pos + 1, q->s.len_k) : q->s.len_k;
-        const bool win = q->s.causal && p.window > 0;
-        const int from = win ? pos - p.window + 1 : 0, sinks = win ? p.sinks : 0;
         for (int m = two ? 0 : x; m < n; m += two ? 1 : 2) {
           if (two && !(m < se || (m >= fi && m < en))) continue;
           const int t = v0 + m < sink_tiles ? v0 + m : v0 + m + skip;
@@ -575,9 +571,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           if (!(t < full_s || (t >= full_lo && t < full_hi))) {
 #pragma unroll
             for (int c = 0; c < KT / 32; ++c) {
-              const int k0 = t * KT + c * 32;
-              auto below = [&](int n_keys) { const int d = n_keys - k0; return d >= 32 ? 0xffffffffu : d <= 0 ? 0u : (1u << d) - 1u; };
-              const uint32_t seen = below(upto) & (~below(from) | below(sinks));
+              const uint32_t seen = seen_keys(pos, t * KT + c * 32, q->s.len_k, q->s.causal, p.window, p.sinks);
 #pragma unroll
               for (int e = 0; e < 32; ++e)
                 if (!(seen & (1u << e))) sr[c][e] = 0xff800000u;
