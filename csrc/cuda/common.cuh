@@ -314,6 +314,21 @@ __device__ __forceinline__ float warp_sum(float v) {
     if (_e != cudaSuccess) return (int)_e;    \
   } while (0)
 
+// The dynamic shared memory that a kernel may be launched with, raised once per kernel and device.
+#include <atomic>
+namespace rb_host {
+template <typename K>
+inline int allow_smem(K kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  RB_CUDA_CHECK(cudaGetDevice(&dev));
+  const unsigned long long bit = 1ULL << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return 0;
+  RB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return 0;
+}
+}  // namespace rb_host
+
 // Tensor-map encoding (driver entry point fetched through the runtime, no link against libcuda).
 //
 // `cuTensorMapEncodeTiled` is a driver call and needs a CUDA context current on the calling thread.  A thread whose

@@ -682,7 +682,9 @@ int launch(SampleArgs p, int num_sms, cudaStream_t st) {
   const long long room = slice + fixed_bytes <= half_bytes ? slice : min(slice, static_cast<long long>(max_bytes - fixed_bytes));
   p.cap = static_cast<int>(room / sizeof(T));
   const int bytes = fixed_bytes + static_cast<int>(room);
-  RB_CUDA_CHECK(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  static std::atomic<unsigned long long> done{0};
+  const int rc = rb_host::allow_smem(sample_kernel<T>, max_bytes, done);
+  if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(c) * static_cast<unsigned>(min(p.rows, 65536)));
   cfg.blockDim = dim3(NT);

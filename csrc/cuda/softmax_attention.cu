@@ -521,7 +521,9 @@ int join(const Batch& p, const Outs& w, int shares, int block_rows, cudaStream_t
 
 template <int D, bool BF16, int W>
 int launch_rows(const CUtensorMap& tm, const Batch& p, const Outs& w, int n_cta, bool after, cudaStream_t st) {
-  RB_CUDA_CHECK(cudaFuncSetAttribute(attn_rows_kernel<D, BF16, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM));
+  static std::atomic<unsigned long long> done{0};
+  const int rc = rb_host::allow_smem(attn_rows_kernel<D, BF16, W>, Cfg<D>::SMEM, done);
+  if (rc) return rc;
   return launch_kernel(after, attn_rows_kernel<D, BF16, W>, dim3(n_cta), dim3(NW * 32), Cfg<D>::SMEM, st, tm, p, w);
 }
 

@@ -756,7 +756,9 @@ int launch(const Batch& p, const Outs& w, const void* cache, int n_cta, bool aft
   if (rc) return rc;
   rc = rb_host::make_map_2d(&tkv, cache, p.total_rows, static_cast<long long>(p.Hkv) * D, static_cast<long long>(p.Hkv) * D, 64, p.box_rows, BF16);
   if (rc) return rc;
-  RB_CUDA_CHECK(cudaFuncSetAttribute(attn_tiles_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM));
+  static std::atomic<unsigned long long> done{0};
+  rc = rb_host::allow_smem(attn_tiles_kernel<D, BF16>, Cfg<D>::SMEM, done);
+  if (rc) return rc;
   return launch_kernel(after, attn_tiles_kernel<D, BF16>, dim3(n_cta), dim3(THREADS), Cfg<D>::SMEM, st, tq, tkv, p, w);
 }
 

@@ -114,6 +114,18 @@ def raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+_launch_env: Dict[int, tuple] = {}
+
+
+def launch_env(index: int) -> tuple:
+    """-> (kernel library, SMs of device ``index``, address of its status word): what every launch needs, looked up once."""
+    env = _launch_env.get(index)
+    if env is None:
+        dev = torch.device("cuda", index)
+        env = _launch_env[index] = (lib(), num_sms(dev), status_tensor(dev).data_ptr())
+    return env
+
+
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     if t is None:
         return None

@@ -81,10 +81,11 @@ def sample_scores(scores: torch.Tensor, uniform: torch.Tensor, offsets: Optional
         off_ptr, off_64 = offsets.data_ptr(), offsets.dtype is torch.int64
     ids = torch.empty(rows, dtype=torch.int64, device=dev)
     logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
-    rc = _lib.lib().rb_sample_scores(scores.data_ptr(), scores.stride(0) if offsets is None else 0, off_ptr, off_64, width, rows,
-                                     uniform.data_ptr(), _lib.ptr(t_t), _lib.ptr(k_t), _lib.ptr(p_t), _lib.ptr(m_t), float(t_v),
-                                     int(k_v), float(p_v), float(m_v), ids.data_ptr(), logprobs.data_ptr(),
-                                     _lib.dtype_code(scores.dtype), _lib.num_sms(dev), _lib.raw_stream(index))
+    lib, sms, _ = _lib.launch_env(index)
+    rc = lib.rb_sample_scores(scores.data_ptr(), scores.stride(0) if offsets is None else 0, off_ptr, off_64, width, rows,
+                              uniform.data_ptr(), _lib.ptr(t_t), _lib.ptr(k_t), _lib.ptr(p_t), _lib.ptr(m_t), float(t_v), int(k_v),
+                              float(p_v), float(m_v), ids.data_ptr(), logprobs.data_ptr(), _lib.dtype_code(scores.dtype), sms,
+                              _lib.raw_stream(index))
     _lib.check(rc, "rb_sample_scores")
     return ids, logprobs
 

@@ -143,12 +143,12 @@ def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache
         with torch.cuda.device(index):
             return append_kv_rotary(q, k, v, cache, batch_indices, positions, page_ids, page_indptr, page_size, table, interleaved,
                                     num_tokens, out)
-    rc = _lib.lib().rb_kv_append_rotary(
+    lib, sms, status = _lib.launch_env(index)
+    rc = lib.rb_kv_append_rotary(
         q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0),
         cache.data_ptr(), batch_indices.data_ptr(), positions.data_ptr(), page_ids.data_ptr(), page_indptr.data_ptr(),
         _lib.ptr(num_tokens), n, H, Hkv, D, page_indptr.shape[0] - 1, page_size, page_ids.shape[0], pages,
-        table.data_ptr(), table.shape[0], table.shape[1], interleaved, q.dtype is torch.bfloat16, _lib.num_sms(cache.device),
-        _lib.status_tensor(cache.device).data_ptr(), _lib.raw_stream(index))
+        table.data_ptr(), table.shape[0], table.shape[1], interleaved, q.dtype is torch.bfloat16, sms, status, _lib.raw_stream(index))
     _lib.check(rc, "rb_kv_append_rotary")
     return out
 
@@ -253,7 +253,7 @@ def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size,
     out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
     lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
     if T:
-        lib, sms = _lib.lib(), _lib.num_sms(dev)
+        lib, sms, status = _lib.launch_env(index)
         nbytes = _workspace_bytes(sms, T, H, Hkv, D, B, groups, scale)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         rc = lib.rb_softmax_attn_paged(
@@ -261,7 +261,7 @@ def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size,
             k_offsets.data_ptr(), page_ids.data_ptr(), page_indptr.data_ptr(), page_ids.shape[0], B, _lib.ptr(g_off),
             _lib.ptr(p_off), _lib.ptr(p_ids), _lib.ptr(p_ptr), p_ids.shape[0] if groups else 0, groups,
             min(window, 1 << 30), min(num_sinks, 1 << 30), scale, q.dtype is torch.bfloat16, out.data_ptr(), H * D,
-            _lib.ptr(lse), ws.data_ptr(), nbytes, sms, _lib.status_tensor(dev).data_ptr(), _lib.raw_stream(index))
+            _lib.ptr(lse), ws.data_ptr(), nbytes, sms, status, _lib.raw_stream(index))
         _lib.check(rc, "rb_softmax_attn_paged")
     return (out, lse) if return_lse else out
 
