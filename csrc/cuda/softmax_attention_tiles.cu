@@ -198,43 +198,47 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const int per = (nb + THREADS - 1) / THREADS;
   int n_mine = 0;
   for (int i = tid * per; i < min((tid + 1) * per, nb); ++i) n_mine += blocks_of(seq_of(p, i), tpt);
-  int n_incl = n_mine;
+  int seq0 = tid * per, blk0 = 0, n_own = n_mine;                             // this thread's blocks: from (seq0, blk0) on
+  if (__syncthreads_or(n_mine > 8)) {
+    // some threads have many: deal them all out anew
+    int n_incl = n_mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, n_incl, o);
-    if (lane >= o) n_incl += x;
-  }
-  if (lane == 31) wcnt[warp] = n_incl;
-  __syncthreads();
-  int n_all = 0, n_before = n_incl - n_mine;
-  for (int i = 0; i < THREADS / 32; ++i) {
-    if (i < warp) n_before += wcnt[i];
-    n_all += wcnt[i];
-  }
-  first_item[tid] = n_before;
-  __syncthreads();
-  const int ipt = (n_all + THREADS - 1) / THREADS;
-  // the sequence and block of item tid * ipt: the last thread whose first item is not after it owns it
-  int seq0 = nb, blk0 = 0;
-  const int my_first = tid * ipt, my_last = min(my_first + ipt, n_all);
-  if (my_first < my_last) {
-    int lo = 0, hi = THREADS - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (first_item[mid] <= my_first) lo = mid; else hi = mid - 1;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, n_incl, o);
+      if (lane >= o) n_incl += x;
     }
-    int left = my_first - first_item[lo];
-    seq0 = lo * per;
-    for (;;) {
-      const int n = blocks_of(seq_of(p, seq0), tpt);
-      if (left < n) { blk0 = left; break; }
-      left -= n;
-      ++seq0;
+    if (lane == 31) wcnt[warp] = n_incl;
+    __syncthreads();
+    int n_all = 0, n_before = n_incl - n_mine;
+    for (int i = 0; i < THREADS / 32; ++i) {
+      if (i < warp) n_before += wcnt[i];
+      n_all += wcnt[i];
+    }
+    first_item[tid] = n_before;
+    __syncthreads();
+    const int ipt = (n_all + THREADS - 1) / THREADS;
+    const int my_first = tid * ipt;
+    n_own = max(min(my_first + ipt, n_all) - my_first, 0);
+    if (n_own > 0) {
+      // the last thread whose first block is not after this one's owns it
+      int lo = 0, hi = THREADS - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first_item[mid] <= my_first) lo = mid; else hi = mid - 1;
+      }
+      int left = my_first - first_item[lo];
+      seq0 = lo * per;
+      for (;;) {
+        const int n = blocks_of(seq_of(p, seq0), tpt);
+        if (left < n) { blk0 = left; break; }
+        left -= n;
+        ++seq0;
+      }
     }
   }
   auto each = [&](auto&& f) {                                                 // f(seq, block, units of all its items)
     int sq = seq0, bl = blk0;
-    for (int i = my_first; i < my_last; ++i) {
+    for (int i = 0; i < n_own; ++i) {
       Seq s = seq_of(p, sq);
       while (bl >= blocks_of(s, tpt)) { ++sq; bl = 0; s = seq_of(p, sq); }
       if (f(sq, bl, static_cast<long long>(block_of(p, s, bl, tpt).units) * p.Hkv)) return;
@@ -433,7 +437,8 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
     };
     while (const Piece* q = next_piece()) {
-      const bool two = q->two, any = q->tiles[x] > 0;
+      const bool two = q->two;
+      int left = q->tiles[x];                                                 // of this row tile's products with V
       const int n = q->n;
       const int v0 = q->v0, sink_tiles = q->span.sink_tiles, skip = q->span.first - sink_tiles;
       const int c_sinks = q->clean_sinks, c_lo = q->clean_lo, c_hi = q->clean_hi;
@@ -473,6 +478,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
             for (int kk = 0; kk < KT / 16; ++kk) rb::umma_f16_ts(t_o, t_s + bp * KT + kk * 8, dv + kk * 128, idesc_o, 1u);
             rb::umma_commit(&bars->o_done[x]);
+            if (left == 1) rb::umma_commit(&bars->o_full[x]);
             if (use_k) {
 #pragma unroll
               for (int kk = 0; kk < D / 16; ++kk)
@@ -483,6 +489,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             rb::umma_commit(&bars->empty[st]);
             if (e == n - 1) rb::umma_commit(&bars->q_empty);
           }
+          --left;
           if (++st == C::STAGES) { st = 0; par ^= 1; }
           continue;
         }
@@ -526,7 +533,9 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             for (int kk = 0; kk < KT / 16; ++kk)
               rb::umma_f16_ts(t_o, t_s + buf * KT + kk * 8, dv + kk * 128, idesc_o, (kk > 0 || started) ? 1u : 0u);
             rb::umma_commit(&bars->o_done[x]);
+            if (left == 1) rb::umma_commit(&bars->o_full[x]);
           }
+          --left;
           started = true;
         }
         if (use_k) mma_s(two ? x : 0);
@@ -534,7 +543,6 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (e == n - 1 && elect()) rb::umma_commit(&bars->q_empty);           // the last S is issued: Q may go
       }
       if (gave_up) break;
-      if (any && elect()) rb::umma_commit(&bars->o_full[x]);
     }
     if (gave_up && lane == 0) {                                               // nothing of ours still runs when TMEM is freed
       rb::umma_commit(&bars->drain[x]);
