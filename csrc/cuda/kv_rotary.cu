@@ -118,28 +118,37 @@ __global__ void __launch_bounds__(256) kv_append_rotary_kernel(const RotaryArgs 
 
 }  // namespace
 
+// The arguments of rb_kv_append_rotary, 8-byte fields first (the caller packs them).
 // q [nnz][H][D], k / v [nnz][Hkv][D] 16-bit (bf16 or fp16), token strides in elements (multiples of 8, 16-byte aligned
 // bases); cache [num_pages][2][page_size][Hkv*D]; table [table_rows][R] fp32 = R/2 cosines, R/2 sines; D and R multiples of
-// 16, R <= D.  A token whose position, batch index or page is out of range is skipped and reported in status.
-RB_API int rb_kv_append_rotary(const void* q, long long ld_q, const void* k, long long ld_k, const void* v, long long ld_v,
-                               void* q_out, long long ld_o, void* cache, const int* batch_idx, const int* positions,
-                               const int* page_ids, const int* page_indptr, const int* num_tokens, int nnz, int H, int Hkv,
-                               int D, int B, int page_size, int num_page_ids, long long num_pages, const float* table,
-                               int table_rows, int R, int interleaved, int is_bf16, int num_sms, int* status, cudaStream_t st) {
-  if (nnz == 0) return 0;
-  if (D % 16 || R % 16 || R <= 0 || R > D || page_size <= 0) return -1;
-  if (ld_q % 8 || ld_k % 8 || ld_v % 8 || ld_o % 8) return -2;
+// 16, R <= D.  num_tokens: device [1] or null.  A token whose position, batch index or page is out of range is skipped and
+// reported in status.
+struct KvAppendCall {
+  const void* q; long long ld_q; const void* k; long long ld_k; const void* v; long long ld_v;
+  void* q_out; long long ld_o;
+  void* cache; long long num_pages;
+  const int *batch_idx, *positions, *page_ids, *page_indptr, *num_tokens;
+  const float* table;
+  int* status; cudaStream_t stream;
+  int nnz, H, Hkv, D, B, page_size, num_page_ids, table_rows, R, interleaved, is_bf16, num_sms;
+};
+
+RB_API int rb_kv_append_rotary(const void* call) {
+  const KvAppendCall& c = *static_cast<const KvAppendCall*>(call);
+  if (c.nnz == 0) return 0;
+  if (c.D % 16 || c.R % 16 || c.R <= 0 || c.R > c.D || c.page_size <= 0) return -1;
+  if (c.ld_q % 8 || c.ld_k % 8 || c.ld_v % 8 || c.ld_o % 8) return -2;
   RotaryArgs p;
-  p.q = (const uint16_t*)q; p.k = (const uint16_t*)k; p.v = (const uint16_t*)v; p.ld_q = ld_q; p.ld_k = ld_k; p.ld_v = ld_v;
-  p.q_out = (uint16_t*)q_out; p.ld_o = ld_o; p.cache = (uint16_t*)cache; p.batch_idx = batch_idx; p.positions = positions;
-  p.page_ids = page_ids; p.page_indptr = page_indptr; p.num_tokens = num_tokens; p.nnz = nnz; p.H = H; p.Hkv = Hkv; p.D = D;
-  p.B = B; p.page_size = page_size; p.num_page_ids = num_page_ids; p.num_pages = num_pages; p.table = table;
-  p.table_rows = table_rows; p.R = R; p.interleaved = interleaved; p.status = status;
-  const long long work = static_cast<long long>(nnz) * ((H + 2 * Hkv + HPT - 1) / HPT) * (D / 16);
-  const long long cap = static_cast<long long>(num_sms > 0 ? num_sms : 148) * 8 * 8;
+  p.q = (const uint16_t*)c.q; p.k = (const uint16_t*)c.k; p.v = (const uint16_t*)c.v; p.ld_q = c.ld_q; p.ld_k = c.ld_k; p.ld_v = c.ld_v;
+  p.q_out = (uint16_t*)c.q_out; p.ld_o = c.ld_o; p.cache = (uint16_t*)c.cache; p.batch_idx = c.batch_idx; p.positions = c.positions;
+  p.page_ids = c.page_ids; p.page_indptr = c.page_indptr; p.num_tokens = c.num_tokens; p.nnz = c.nnz; p.H = c.H; p.Hkv = c.Hkv; p.D = c.D;
+  p.B = c.B; p.page_size = c.page_size; p.num_page_ids = c.num_page_ids; p.num_pages = c.num_pages; p.table = c.table;
+  p.table_rows = c.table_rows; p.R = c.R; p.interleaved = c.interleaved; p.status = c.status;
+  const long long work = static_cast<long long>(c.nnz) * ((c.H + 2 * c.Hkv + HPT - 1) / HPT) * (c.D / 16);
+  const long long cap = static_cast<long long>(c.num_sms > 0 ? c.num_sms : 148) * 8 * 8;
   long long blocks = (work + 255) / 256;
   if (blocks > cap) blocks = cap;
-  if (is_bf16) kv_append_rotary_kernel<true><<<static_cast<int>(blocks), 256, 0, st>>>(p);
-  else kv_append_rotary_kernel<false><<<static_cast<int>(blocks), 256, 0, st>>>(p);
+  if (c.is_bf16) kv_append_rotary_kernel<true><<<static_cast<int>(blocks), 256, 0, c.stream>>>(p);
+  else kv_append_rotary_kernel<false><<<static_cast<int>(blocks), 256, 0, c.stream>>>(p);
   return static_cast<int>(cudaGetLastError());
 }

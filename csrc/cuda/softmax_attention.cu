@@ -578,43 +578,52 @@ RB_API long long rb_softmax_attn_workspace(int num_sms, long long Tq, int H, int
                   groups > 0).total;
 }
 
+// The arguments of rb_softmax_attn_paged, 8-byte fields first (the caller packs them: by far cheaper than 33 arguments).
 // q [Tq][H][D] (token stride ld_q), cache [num_pages][2][page_size][Hkv][D], bf16 or fp16; int32 offsets and page tables on
 // the device.  B requests own the queries q_offsets[b]..q_offsets[b+1] and k_offsets[b+1] - k_offsets[b] keys, the last of which are
 // the queries' own.  G groups (0: none) of requests group_offsets[g]..group_offsets[g+1] - or, without group_offsets, ONE
 // group of all requests - see prefix_offsets[g+1] - prefix_offsets[g] more keys in front of their own; window and sinks
 // are for calls without groups.  out [Tq][H][D] (token stride ld_o), lse [Tq][H] fp32 or null.
-RB_API int rb_softmax_attn_paged(const void* q, long long ld_q, long long Tq, int H, int Hkv, int D, const void* cache,
-                                 long long num_pages, int page_size, const int* q_offsets, const int* k_offsets,
-                                 const int* page_ids, const int* page_indptr, int num_page_ids, int B, const int* group_offsets,
-                                 const int* prefix_offsets, const int* prefix_page_ids, const int* prefix_page_indptr,
-                                 int num_prefix_page_ids, int groups, int window, int sinks, float scale, int is_bf16, void* out,
-                                 long long ld_o, float* lse, void* workspace, long long workspace_bytes, int num_sms, int* status,
-                                 cudaStream_t st) {
-  if (Tq == 0 || B == 0) return 0;
-  if ((D != 64 && D != 128) || Hkv <= 0 || H % Hkv) return -1;
-  if (ld_q % 8 || ld_o % 8) return -2;
-  if (page_size % 16 || page_size <= 0 || (groups > 0 && window > 0) || (groups > 1 && !group_offsets)) return -3;
-  const long long rows = num_pages * 2 * page_size;
-  if (Tq * H > 0x7fffffffLL || rows + page_size > 0x7fffffffLL) return -4;
-  const int n_cta = num_sms > 0 ? num_sms : 148;
-  const Plan plan = plan_of(Tq, H / Hkv, B, groups, scale);
-  const Space sp = space_of(n_cta, D, Tq * H, !plan.tiles_a || (groups > 0 && !plan.tiles_b), plan.tiles_a || plan.tiles_b, groups > 0);
-  if (workspace_bytes < sp.total) return -5;
+struct SoftmaxAttnCall {
+  const void* q; long long ld_q, Tq;
+  const void* cache; long long num_pages;
+  const int *q_offsets, *k_offsets, *page_ids, *page_indptr;
+  const int *group_offsets, *prefix_offsets, *prefix_page_ids, *prefix_page_indptr;
+  void* out; long long ld_o; float* lse;
+  void* workspace; long long workspace_bytes;
+  int* status; cudaStream_t stream;
+  int H, Hkv, D, page_size, num_page_ids, B, num_prefix_page_ids, groups, window, sinks, is_bf16, num_sms;
+  float scale;
+};
+
+RB_API int rb_softmax_attn_paged(const void* call) {
+  const SoftmaxAttnCall& c = *static_cast<const SoftmaxAttnCall*>(call);
+  if (c.Tq == 0 || c.B == 0) return 0;
+  if ((c.D != 64 && c.D != 128) || c.Hkv <= 0 || c.H % c.Hkv) return -1;
+  if (c.ld_q % 8 || c.ld_o % 16) return -2;
+  if (c.page_size % 16 || c.page_size <= 0 || (c.groups > 0 && c.window > 0) || (c.groups > 1 && !c.group_offsets)) return -3;
+  const long long rows = c.num_pages * 2 * c.page_size;
+  if (c.Tq * c.H > 0x7fffffffLL || rows + c.page_size > 0x7fffffffLL) return -4;
+  const int n_cta = c.num_sms > 0 ? c.num_sms : 148;
+  const Plan plan = plan_of(c.Tq, c.H / c.Hkv, c.B, c.groups, c.scale);
+  const Space sp = space_of(n_cta, c.D, c.Tq * c.H, !plan.tiles_a || (c.groups > 0 && !plan.tiles_b), plan.tiles_a || plan.tiles_b, c.groups > 0);
+  if (c.workspace_bytes < sp.total) return -5;
   Batch p;
-  const Seqs own = {q_offsets, nullptr, 0, k_offsets, page_ids, page_indptr, num_page_ids, B, B, 1};
+  const Seqs own = {c.q_offsets, nullptr, 0, c.k_offsets, c.page_ids, c.page_indptr, c.num_page_ids, c.B, c.B, 1};
   const Seqs none = {nullptr, nullptr, 0, nullptr, nullptr, nullptr, 0, 0, 0, 0};
-  const Seqs pre = {q_offsets, group_offsets, group_offsets == nullptr, prefix_offsets, prefix_page_ids, prefix_page_indptr, num_prefix_page_ids,
-                    groups, B, 0};
-  p.a = groups > 0 ? pre : own;
-  p.b = groups > 0 ? own : none;
-  p.q = q; p.ld_q = ld_q; p.Tq = static_cast<int>(Tq); p.H = H; p.Hkv = Hkv; p.G = H / Hkv; p.page_size = page_size;
-  p.box_rows = 16; p.total_rows = static_cast<int>(rows); p.window = window; p.sinks = sinks;
-  p.scale_log2 = scale * LOG2E; p.status = status;
-  char* ws = static_cast<char*>(workspace);
+  const Seqs pre = {c.q_offsets, c.group_offsets, c.group_offsets == nullptr, c.prefix_offsets, c.prefix_page_ids, c.prefix_page_indptr,
+                    c.num_prefix_page_ids, c.groups, c.B, 0};
+  p.a = c.groups > 0 ? pre : own;
+  p.b = c.groups > 0 ? own : none;
+  p.q = c.q; p.ld_q = c.ld_q; p.Tq = static_cast<int>(c.Tq); p.H = c.H; p.Hkv = c.Hkv; p.G = c.H / c.Hkv; p.page_size = c.page_size;
+  p.box_rows = 16; p.total_rows = static_cast<int>(rows); p.window = c.window; p.sinks = c.sinks;
+  p.scale_log2 = c.scale * LOG2E; p.status = c.status;
+  char* ws = static_cast<char*>(c.workspace);
   Outs w;
-  w.out = out; w.ld_o = ld_o; w.lse = lse;
-  w.part_o = groups > 0 ? reinterpret_cast<float*>(ws + sp.part_o) : nullptr;
+  w.out = c.out; w.ld_o = c.ld_o; w.lse = c.lse;
+  w.part_o = c.groups > 0 ? reinterpret_cast<float*>(ws + sp.part_o) : nullptr;
   w.part_lse = reinterpret_cast<float*>(ws + sp.part_lse);
-  if (D == 64) return is_bf16 ? launch<64, true>(p, w, plan, sp, ws, cache, n_cta, st) : launch<64, false>(p, w, plan, sp, ws, cache, n_cta, st);
-  return is_bf16 ? launch<128, true>(p, w, plan, sp, ws, cache, n_cta, st) : launch<128, false>(p, w, plan, sp, ws, cache, n_cta, st);
+  if (c.D == 64)
+    return c.is_bf16 ? launch<64, true>(p, w, plan, sp, ws, c.cache, n_cta, c.stream) : launch<64, false>(p, w, plan, sp, ws, c.cache, n_cta, c.stream);
+  return c.is_bf16 ? launch<128, true>(p, w, plan, sp, ws, c.cache, n_cta, c.stream) : launch<128, false>(p, w, plan, sp, ws, c.cache, n_cta, c.stream);
 }

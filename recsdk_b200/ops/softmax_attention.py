@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import functools
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -22,6 +23,9 @@ import torch
 from . import _lib
 
 _HEAD_DIMS = (64, 128)
+# the launchers' argument records (KvAppendCall, SoftmaxAttnCall): 8-byte fields, ints, floats
+_APPEND_CALL = struct.Struct("@18q12i")
+_ATTEND_CALL = struct.Struct("@20q12if")
 
 
 def rotary_table(max_positions: int, rotary_dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
@@ -54,12 +58,13 @@ def _rows(name: str, x: torch.Tensor, heads: Optional[int], dim: int, like: torc
     return x
 
 
-def _ints(name: str, x: torch.Tensor, like: torch.Tensor, n: Optional[int] = None) -> torch.Tensor:
+def _ints(name: str, x: torch.Tensor, index: int, n: Optional[int] = None) -> torch.Tensor:
+    """A vector of int32 on device ``index`` (-1: CPU); int64 is converted."""
     shape = x.shape
     if len(shape) != 1 or (n is not None and shape[0] != n):
         raise ValueError("%s must be a vector%s, got %s" % (name, "" if n is None else " of %d" % n, tuple(shape)))
-    if x.get_device() != like.get_device() or x.dtype not in (torch.int32, torch.int64):
-        raise ValueError("%s must be int32 or int64 on %s, got %s on %s" % (name, like.device, x.dtype, x.device))
+    if x.get_device() != index or x.dtype not in (torch.int32, torch.int64):
+        raise ValueError("%s must be int32 or int64 on the cache's device, got %s on %s" % (name, x.dtype, x.device))
     return x if x.dtype is torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
 
 
@@ -106,6 +111,7 @@ def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache
     ``_lib.check_status``."""
     cache = _cache(kv_cache, page_size)
     pages, _, _, Hkv, D = cache.shape
+    index = cache.get_device()
     if D % 16:
         raise ValueError("head_dim must be a multiple of 16, got %d" % D)
     q, k, v = _rows("q", q, None, D, cache), _rows("k", k, Hkv, D, cache), _rows("v", v, Hkv, D, cache)
@@ -116,14 +122,14 @@ def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache
             or table.shape[1] % 16 or not 0 < table.shape[1] <= D or (table.is_cuda and table.data_ptr() & 15):
         raise ValueError("table must be a contiguous fp32 [max_positions, rotary_dim] on %s with rotary_dim a multiple of 16 and "
                          "at most %d, got %s %s on %s" % (cache.device, D, table.dtype, tuple(table.shape), table.device))
-    batch_indices, positions = _ints("batch_indices", batch_indices, cache, n), _ints("positions", positions, cache, n)
-    page_ids, page_indptr = _ints("page_ids", page_ids, cache), _ints("page_indptr", page_indptr, cache)
+    batch_indices, positions = _ints("batch_indices", batch_indices, index, n), _ints("positions", positions, index, n)
+    page_ids, page_indptr = _ints("page_ids", page_ids, index), _ints("page_indptr", page_indptr, index)
     if num_tokens is not None:
-        num_tokens = _ints("num_tokens", num_tokens, cache, 1)
+        num_tokens = _ints("num_tokens", num_tokens, index, 1)
     if page_indptr.shape[0] < 1:
         raise ValueError("page_indptr must be [requests + 1]")
     if out is None:
-        out = torch.empty((n, H, D), dtype=q.dtype, device=cache.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != cache.device or (out.numel() and (
             out.stride(2) != 1 or out.stride(1) != D or out.stride(0) % 8 or out.stride(0) < H * D or out.data_ptr() % 16)):
         raise ValueError("out must be %s %s on %s with adjacent heads and 16-byte aligned rows" % (tuple(q.shape), q.dtype, cache.device))
@@ -138,17 +144,16 @@ def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache
         cache[at, 0, pos % page_size] = _rotate_ref(k[:m], cos, sin, interleaved)
         cache[at, 1, pos % page_size] = v[:m]
         return out
-    index = cache.get_device()
     if not _lib.is_current(index):
         with torch.cuda.device(index):
             return append_kv_rotary(q, k, v, cache, batch_indices, positions, page_ids, page_indptr, page_size, table, interleaved,
                                     num_tokens, out)
     lib, sms, status = _lib.launch_env(index)
-    rc = lib.rb_kv_append_rotary(
+    rc = lib.rb_kv_append_rotary(_APPEND_CALL.pack(
         q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0),
-        cache.data_ptr(), batch_indices.data_ptr(), positions.data_ptr(), page_ids.data_ptr(), page_indptr.data_ptr(),
-        _lib.ptr(num_tokens), n, H, Hkv, D, page_indptr.shape[0] - 1, page_size, page_ids.shape[0], pages,
-        table.data_ptr(), table.shape[0], table.shape[1], interleaved, q.dtype is torch.bfloat16, sms, status, _lib.raw_stream(index))
+        cache.data_ptr(), pages, batch_indices.data_ptr(), positions.data_ptr(), page_ids.data_ptr(), page_indptr.data_ptr(),
+        0 if num_tokens is None else num_tokens.data_ptr(), table.data_ptr(), status, _lib.raw_stream(index), n, H, Hkv, D,
+        page_indptr.shape[0] - 1, page_size, page_ids.shape[0], table.shape[0], table.shape[1], interleaved, q.dtype is torch.bfloat16, sms))
     _lib.check(rc, "rb_kv_append_rotary")
     return out
 
@@ -214,6 +219,7 @@ def _workspace_bytes(*sizes) -> int:
 def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks, return_lse, prefix=None):
     cache = _cache(kv_cache, page_size, _HEAD_DIMS)
     pages, _, _, Hkv, D = cache.shape
+    index = cache.get_device()
     q = _rows("q", q, None, D, cache)
     T, H, _ = q.shape
     if H == 0 or H % Hkv:
@@ -221,8 +227,8 @@ def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size,
     B = q_offsets.numel() - 1
     if B < 0:
         raise ValueError("q_offsets must be [requests + 1]")
-    q_offsets, k_offsets = _ints("q_offsets", q_offsets, cache), _ints("k_offsets", k_offsets, cache, B + 1)
-    page_ids, page_indptr = _ints("page_ids", page_ids, cache), _ints("page_indptr", page_indptr, cache, B + 1)
+    q_offsets, k_offsets = _ints("q_offsets", q_offsets, index), _ints("k_offsets", k_offsets, index, B + 1)
+    page_ids, page_indptr = _ints("page_ids", page_ids, index), _ints("page_indptr", page_indptr, index, B + 1)
     if window < 0 or num_sinks < 0:
         raise ValueError("window and num_sinks must not be negative")
     scale = D ** -0.5 if scale is None else float(scale)
@@ -234,10 +240,10 @@ def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size,
         groups = p_off.numel() - 1
         if groups < 0 or (g_off is None and groups != 1):
             raise ValueError("prefix_offsets must be [groups + 1], and [2] without group_offsets")
-        p_off, p_ids = _ints("prefix_offsets", p_off, cache), _ints("prefix_page_ids", p_ids, cache)
-        p_ptr = _ints("prefix_page_indptr", p_ptr, cache, groups + 1)
+        p_off, p_ids = _ints("prefix_offsets", p_off, index), _ints("prefix_page_ids", p_ids, index)
+        p_ptr = _ints("prefix_page_indptr", p_ptr, index, groups + 1)
         if g_off is not None:
-            g_off = _ints("group_offsets", g_off, cache, groups + 1)
+            g_off = _ints("group_offsets", g_off, index, groups + 1)
     if not cache.is_cuda:
         o, lse = softmax_attention_ref(q, cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks,
                                        p_off, p_ids, p_ptr, g_off)
@@ -246,22 +252,22 @@ def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size,
         raise ValueError("page_size must be a multiple of 16, got %d" % page_size)
     if T and B == 0:
         raise ValueError("q holds %d tokens but there are no requests" % T)
-    index, dev = cache.get_device(), cache.device
     if not _lib.is_current(index):
         with torch.cuda.device(index):
             return _attend(q, cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks, return_lse, prefix)
-    out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
-    lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty((T, H), dtype=torch.float32, device=cache.device) if return_lse else None
     if T:
         lib, sms, status = _lib.launch_env(index)
         nbytes = _workspace_bytes(sms, T, H, Hkv, D, B, groups, scale)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        rc = lib.rb_softmax_attn_paged(
-            q.data_ptr(), q.stride(0), T, H, Hkv, D, cache.data_ptr(), pages, page_size, q_offsets.data_ptr(),
-            k_offsets.data_ptr(), page_ids.data_ptr(), page_indptr.data_ptr(), page_ids.shape[0], B, _lib.ptr(g_off),
-            _lib.ptr(p_off), _lib.ptr(p_ids), _lib.ptr(p_ptr), p_ids.shape[0] if groups else 0, groups,
-            min(window, 1 << 30), min(num_sinks, 1 << 30), scale, q.dtype is torch.bfloat16, out.data_ptr(), H * D,
-            _lib.ptr(lse), ws.data_ptr(), nbytes, sms, status, _lib.raw_stream(index))
+        ws = q.new_empty(nbytes // 2)                                   # (16-bit elements)
+        rc = lib.rb_softmax_attn_paged(_ATTEND_CALL.pack(
+            q.data_ptr(), q.stride(0), T, cache.data_ptr(), pages, q_offsets.data_ptr(), k_offsets.data_ptr(), page_ids.data_ptr(),
+            page_indptr.data_ptr(), 0 if g_off is None else g_off.data_ptr(), p_off.data_ptr() if groups else 0,
+            p_ids.data_ptr() if groups else 0, p_ptr.data_ptr() if groups else 0, out.data_ptr(), H * D,
+            0 if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes, status, _lib.raw_stream(index), H, Hkv, D, page_size,
+            page_ids.shape[0], B, p_ids.shape[0] if groups else 0, groups, min(window, 1 << 30), min(num_sinks, 1 << 30),
+            q.dtype is torch.bfloat16, sms, scale))
         _lib.check(rc, "rb_softmax_attn_paged")
     return (out, lse) if return_lse else out
 
