@@ -21,6 +21,7 @@ struct RotaryArgs {
   uint16_t* q_out; long long ld_o;
   uint16_t* cache;
   const int *batch_idx, *positions, *page_ids, *page_indptr;
+  const int* slots;                  // place among the request's tokens, or null: its position
   const int* num_tokens;             // device [1] or null: tokens at or past it are left alone
   int nnz, H, Hkv, D, B, page_size, num_page_ids;
   long long num_pages;
@@ -77,11 +78,11 @@ __global__ void __launch_bounds__(256) kv_append_rotary_kernel(const RotaryArgs 
       a[t] = __ldg(reinterpret_cast<const uint4*>(src) + va);
       b[t] = __ldg(reinterpret_cast<const uint4*>(src) + vb);
     }
-    const int pos = p.positions[i], bi = p.batch_idx[i];
-    bool ok = pos >= 0 && pos < p.table_rows && bi >= 0 && bi < p.B;
+    const int pos = p.positions[i], at_token = p.slots ? p.slots[i] : pos, bi = p.batch_idx[i];
+    bool ok = pos >= 0 && pos < p.table_rows && at_token >= 0 && bi >= 0 && bi < p.B;
     long long page = 0;
     if (ok) {
-      const int at = p.page_indptr[bi] + pos / p.page_size;
+      const int at = p.page_indptr[bi] + at_token / p.page_size;
       ok = at >= 0 && at < p.page_indptr[bi + 1] && at < p.num_page_ids;
       if (ok) {
         page = p.page_ids[at];
@@ -101,7 +102,7 @@ __global__ void __launch_bounds__(256) kv_append_rotary_kernel(const RotaryArgs 
       s[0] = s0.x; s[1] = s0.y; s[2] = s0.z; s[3] = s0.w; s[4] = s1.x; s[5] = s1.y; s[6] = s1.z; s[7] = s1.w;
     }
     const long long row_elems = static_cast<long long>(p.Hkv) * p.D;
-    uint16_t* k_row = p.cache + ((page * 2) * p.page_size + pos % p.page_size) * row_elems;
+    uint16_t* k_row = p.cache + ((page * 2) * p.page_size + at_token % p.page_size) * row_elems;
 #pragma unroll
     for (int t = 0; t < HPT; ++t) {
       const int h = slot + t * slots;
@@ -121,13 +122,13 @@ __global__ void __launch_bounds__(256) kv_append_rotary_kernel(const RotaryArgs 
 // The arguments of rb_kv_append_rotary, 8-byte fields first (the caller packs them).
 // q [nnz][H][D], k / v [nnz][Hkv][D] 16-bit (bf16 or fp16), token strides in elements (multiples of 8, 16-byte aligned
 // bases); cache [num_pages][2][page_size][Hkv*D]; table [table_rows][R] fp32 = R/2 cosines, R/2 sines; D and R multiples of
-// 16, R <= D.  num_tokens: device [1] or null.  A token whose position, batch index or page is out of range is skipped and
+// 16, R <= D.  slots [nnz] or null, num_tokens: device [1] or null.  A token whose position, batch index or page is out of range is skipped and
 // reported in status.
 struct KvAppendCall {
   const void* q; long long ld_q; const void* k; long long ld_k; const void* v; long long ld_v;
   void* q_out; long long ld_o;
   void* cache; long long num_pages;
-  const int *batch_idx, *positions, *page_ids, *page_indptr, *num_tokens;
+  const int *batch_idx, *positions, *slots, *page_ids, *page_indptr, *num_tokens;
   const float* table;
   int* status; cudaStream_t stream;
   int nnz, H, Hkv, D, B, page_size, num_page_ids, table_rows, R, interleaved, is_bf16, num_sms;
@@ -141,7 +142,7 @@ RB_API int rb_kv_append_rotary(const void* call) {
   RotaryArgs p;
   p.q = (const uint16_t*)c.q; p.k = (const uint16_t*)c.k; p.v = (const uint16_t*)c.v; p.ld_q = c.ld_q; p.ld_k = c.ld_k; p.ld_v = c.ld_v;
   p.q_out = (uint16_t*)c.q_out; p.ld_o = c.ld_o; p.cache = (uint16_t*)c.cache; p.batch_idx = c.batch_idx; p.positions = c.positions;
-  p.page_ids = c.page_ids; p.page_indptr = c.page_indptr; p.num_tokens = c.num_tokens; p.nnz = c.nnz; p.H = c.H; p.Hkv = c.Hkv; p.D = c.D;
+  p.slots = c.slots; p.page_ids = c.page_ids; p.page_indptr = c.page_indptr; p.num_tokens = c.num_tokens; p.nnz = c.nnz; p.H = c.H; p.Hkv = c.Hkv; p.D = c.D;
   p.B = c.B; p.page_size = c.page_size; p.num_page_ids = c.num_page_ids; p.num_pages = c.num_pages; p.table = c.table;
   p.table_rows = c.table_rows; p.R = c.R; p.interleaved = c.interleaved; p.status = c.status;
   const long long work = static_cast<long long>(c.nnz) * ((c.H + 2 * c.Hkv + HPT - 1) / HPT) * (c.D / 16);

@@ -24,7 +24,7 @@ from . import _lib
 
 _HEAD_DIMS = (64, 128)
 # the launchers' argument records (KvAppendCall, SoftmaxAttnCall): 8-byte fields, ints, floats
-_APPEND_CALL = struct.Struct("@18q12i")
+_APPEND_CALL = struct.Struct("@19q12i")
 _ATTEND_CALL = struct.Struct("@20q12if")
 
 
@@ -96,14 +96,16 @@ def _rotate_ref(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, interleav
 def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor, batch_indices: torch.Tensor,
                      positions: torch.Tensor, page_ids: torch.Tensor, page_indptr: torch.Tensor, page_size: int,
                      table: torch.Tensor, interleaved: bool = False, num_tokens: Optional[torch.Tensor] = None,
-                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     out: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Turn the new tokens' queries and keys by their positions, write keys and values into their pages, return the queries.
 
     ``q [n, heads, head_dim]``, ``k`` / ``v [n, kv_heads, head_dim]`` (token stride free, e.g. slices of one projection);
     token ``i`` is token ``positions[i]`` of request ``batch_indices[i]``, whose pages are
     ``page_ids[page_indptr[b]:page_indptr[b + 1]]``.  ``table`` is :func:`rotary_table`'s ``[max_positions, rotary_dim]``
     (or any cosines and sines); the first ``rotary_dim`` elements of a head turn, element ``i`` with ``i + rotary_dim / 2``
-    or, ``interleaved``, ``2i`` with ``2i + 1``.  No two tokens of a call may name the same position of a request.
+    or, ``interleaved``, ``2i`` with ``2i + 1``.  ``slots``: where a token goes among its request's keys if not at its
+    position - behind a shared prefix, whose tokens the request's pages do not hold.  No two tokens of a call may go to the same
+    place.
 
     ``num_tokens``: optional device int32 ``[1]`` (``new_history_nnz_npu``): only that many tokens are there, the rows
     behind them are neither appended nor written to the result - for static buffers under a captured graph.  ``out``: where the
@@ -126,6 +128,8 @@ def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache
     page_ids, page_indptr = _ints("page_ids", page_ids, index), _ints("page_indptr", page_indptr, index)
     if num_tokens is not None:
         num_tokens = _ints("num_tokens", num_tokens, index, 1)
+    if slots is not None:
+        slots = _ints("slots", slots, index, n)
     if page_indptr.shape[0] < 1:
         raise ValueError("page_indptr must be [requests + 1]")
     if out is None:
@@ -139,20 +143,21 @@ def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache
         m = n if num_tokens is None else min(n, int(num_tokens))
         pos, b = positions[:m].long(), batch_indices[:m].long()
         cos, sin = table[pos][:, None, :].chunk(2, dim=-1)
-        at = page_ids.long()[page_indptr.long()[b] + pos // page_size]
+        to = pos if slots is None else slots[:m].long()
+        at = page_ids.long()[page_indptr.long()[b] + to // page_size]
         out[:m] = _rotate_ref(q[:m], cos, sin, interleaved)
-        cache[at, 0, pos % page_size] = _rotate_ref(k[:m], cos, sin, interleaved)
-        cache[at, 1, pos % page_size] = v[:m]
+        cache[at, 0, to % page_size] = _rotate_ref(k[:m], cos, sin, interleaved)
+        cache[at, 1, to % page_size] = v[:m]
         return out
     if not _lib.is_current(index):
         with torch.cuda.device(index):
             return append_kv_rotary(q, k, v, cache, batch_indices, positions, page_ids, page_indptr, page_size, table, interleaved,
-                                    num_tokens, out)
+                                    num_tokens, out, slots)
     lib, sms, status = _lib.launch_env(index)
     rc = lib.rb_kv_append_rotary(_APPEND_CALL.pack(
         q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0),
-        cache.data_ptr(), pages, batch_indices.data_ptr(), positions.data_ptr(), page_ids.data_ptr(), page_indptr.data_ptr(),
-        0 if num_tokens is None else num_tokens.data_ptr(), table.data_ptr(), status, _lib.raw_stream(index), n, H, Hkv, D,
+        cache.data_ptr(), pages, batch_indices.data_ptr(), positions.data_ptr(), 0 if slots is None else slots.data_ptr(),
+        page_ids.data_ptr(), page_indptr.data_ptr(), 0 if num_tokens is None else num_tokens.data_ptr(), table.data_ptr(), status, _lib.raw_stream(index), n, H, Hkv, D,
         page_indptr.shape[0] - 1, page_size, page_ids.shape[0], table.shape[0], table.shape[1], interleaved, q.dtype is torch.bfloat16, sms))
     _lib.check(rc, "rb_kv_append_rotary")
     return out
@@ -252,6 +257,8 @@ def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size,
         raise ValueError("page_size must be a multiple of 16, got %d" % page_size)
     if T and B == 0:
         raise ValueError("q holds %d tokens but there are no requests" % T)
+    if pages == 0:
+        raise ValueError("kv_cache holds no pages")
     if not _lib.is_current(index):
         with torch.cuda.device(index):
             return _attend(q, cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks, return_lse, prefix)

@@ -119,3 +119,38 @@ def test_the_draws_follow_the_distribution():
     ids, _ = S.sample_scores(x.to(DEV).expand(n, 300), u, temperature=0.8)
     want = torch.softmax(x.double() / torch.tensor(0.8, dtype=torch.float32).double(), 0) * n
     assert ((torch.bincount(ids.cpu(), minlength=300) - want).abs() <= 1.01).all()
+
+
+def test_more_rows_than_blocks_and_long_jagged_rows():
+    g = torch.Generator(device=DEV).manual_seed(9)
+    x = torch.randn(70001, 6, generator=g, device=DEV)
+    u = torch.rand(70001, generator=g, device=DEV)
+    ids, _ = S.sample_scores(x, u, top_k=3)
+    pick = torch.tensor([0, 1, 65535, 65536, 69999, 70000])
+    assert torch.equal(ids[pick], S.sample_scores_ref(x[pick], u[pick], top_k=3)[0])
+    # a row far longer than the average, beyond what shared memory holds
+    lens = [700001, 3, 100, 2000]
+    x = torch.randn(sum(lens), generator=g, device=DEV).half()
+    o = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), device=DEV)
+    for kw in (dict(top_p=0.9), dict(top_k=5000, top_p=0.99), dict(min_p=0.01), dict(temperature=0.0)):
+        _same(x, torch.rand(4, generator=g, device=DEV), o, **kw)
+
+
+def test_the_ranker_draws_from_its_scores():
+    from recsdk_b200.inference import KVCacheConfig, KVCacheManager
+    from recsdk_b200.models.hstu import HSTU, HSTUConfig
+    from recsdk_b200.models.hstu_inference import HSTURanker
+
+    torch.manual_seed(0)
+    cfg = HSTUConfig(num_layers=2, d_model=128, num_heads=2, head_dim=64, max_seq_len=1024, num_time_buckets=16)
+    model = HSTU(cfg, torch.nn.Identity(), DEV, torch.bfloat16).eval()
+    make = lambda: HSTURanker(model, KVCacheManager.from_config(KVCacheConfig(  # noqa: E731
+        num_layers=2, num_heads=2, head_dim=64, page_size=32, offload_chunksize=64, num_primary_cache_pages=64, num_buffer_pages=16,
+        host_capacity_per_layer=1 << 22, max_batch_size=4, max_seq_len=1024, dtype=torch.bfloat16, device=DEV)))
+    users, hist, cands = torch.tensor([3, 5, 8]), torch.tensor([100, 60, 30]), torch.tensor([20, 0, 300])
+    x = (torch.randn(510, 128, device=DEV) * 0.5).bfloat16()
+    u = torch.tensor([0.3, 0.1, 0.95], device=DEV)
+    scores = make().rank(users, hist, cands, x)
+    ids, lp = make().recommend(users, hist, cands, x, u, temperature=0.5, top_p=0.9)
+    want, want_lp = S.sample_scores_ref(scores, u, torch.tensor([0, 20, 20, 320]), temperature=0.5, top_p=0.9)
+    assert torch.equal(ids, want) and ids[1] == -1 and torch.allclose(lp[[0, 2]], want_lp[[0, 2]], rtol=1e-6)

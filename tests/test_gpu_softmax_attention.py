@@ -271,3 +271,131 @@ def test_one_step_in_a_graph():
         got = out.clone()
         assert torch.equal(got, step())
     _lib.check_status()
+
+
+def test_many_requests_and_wide_groups():
+    g = torch.Generator().manual_seed(6)
+    # more requests than threads that count them, some without tokens, some without keys
+    new = torch.randint(0, 3, (3000,), generator=g).tolist()
+    keys = [n + k for n, k in zip(new, torch.randint(0, 40, (3000,), generator=g).tolist())]
+    _run(new, keys, 4, 2, 64, 16, torch.bfloat16, seed=6)
+    new = torch.randint(0, 90, (700,), generator=g).tolist()
+    keys = [n + k for n, k in zip(new, torch.randint(0, 100, (700,), generator=g).tolist())]
+    _run(new, keys, 2, 2, 64, 32, torch.float16, 50, 3, seed=7)
+    # 160 and 64 query heads on one key head
+    _run([1, 3], [70, 500], 160, 1, 64, 16, torch.bfloat16, seed=8)
+    _run([5, 33], [70, 300], 64, 1, 128, 16, torch.bfloat16, seed=9)
+
+
+def test_long_offsets_and_uneven_lengths():
+    """One very long request among short ones; the other offset type."""
+    _run([1] * 9, [40001, 1, 2, 3, 64, 65, 100, 7, 9], 8, 2, 128, 64, torch.float16, seed=1)
+    _run([150] + [1] * 5, [9000, 3, 2, 700, 1, 65], 4, 1, 64, 64, torch.bfloat16, 0, 0, seed=2)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    cache, ids, ptr = _cache([100, 70], 16, 2, 64, torch.bfloat16, g)
+    q = torch.randn(2, 4, 64, generator=g, device=DEV).bfloat16()
+    a = SA.softmax_attention_paged(q, cache, _off([1, 1]), _off([100, 70]), ids, ptr, 16)
+    b = SA.softmax_attention_paged(q, cache, _off([1, 1]).long(), _off([100, 70]).long(), ids.long(), ptr.long(), 16)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("new", [1, 200])
+def test_a_broken_query_stays_alone(new):
+    g = torch.Generator(device=DEV).manual_seed(3)
+    cache, ids, ptr = _cache([300, 400], 16, 2, 64, torch.bfloat16, g)
+    q = torch.randn(2 * new, 4, 64, generator=g, device=DEV).bfloat16()
+    args = (cache, _off([new, new]), _off([300, 400]), ids, ptr, 16)
+    want = SA.softmax_attention_paged(q, *args)
+    q[0, 1] = math.nan
+    got = SA.softmax_attention_paged(q, *args)
+    assert torch.isnan(got[0, 1]).all()
+    got[0, 1] = want[0, 1]
+    assert torch.equal(got, want)
+
+
+def test_calls_on_two_streams():
+    g = torch.Generator(device=DEV).manual_seed(5)
+    cache, ids, ptr = _cache([5000, 60, 900], 64, 2, 128, torch.bfloat16, g)
+    few, many = torch.randn(3, 8, 128, generator=g, device=DEV).bfloat16(), torch.randn(300, 8, 128, generator=g, device=DEV).bfloat16()
+    calls = [lambda: SA.softmax_attention_paged(few, cache, _off([1, 1, 1]), _off([5000, 60, 900]), ids, ptr, 64),
+             lambda: SA.softmax_attention_paged(many, cache, _off([200, 50, 50]), _off([5000, 60, 900]), ids, ptr, 64, window=700)]
+    want = [c() for c in calls]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(calls[i]())
+    torch.cuda.synchronize()
+    assert all(torch.equal(want[i], o) for i in (0, 1) for o in got[i])
+
+
+def test_refusals_on_the_gpu():
+    g = torch.Generator(device=DEV).manual_seed(2)
+    cache, ids, ptr = _cache([20], 16, 2, 64, torch.bfloat16, g)
+    q = torch.randn(1, 4, 64, generator=g, device=DEV).bfloat16()
+    ok = dict(q=q, kv_cache=cache, q_offsets=_off([1]), k_offsets=_off([20]), page_ids=ids, page_indptr=ptr, page_size=16)
+    SA.softmax_attention_paged(**ok)
+    c32 = torch.zeros(3, 2, 16, 2, 32, dtype=torch.bfloat16, device=DEV)
+    c24 = torch.zeros(3, 2, 24, 2, 64, dtype=torch.bfloat16, device=DEV)
+    for kw in (dict(kv_cache=cache.float(), q=q.float()), dict(kv_cache=c32, q=q[..., :32]), dict(kv_cache=c24, page_size=24),
+               dict(q_offsets=_off([1]).cpu()), dict(page_ids=ids.cpu()), dict(kv_cache=cache[:0]), dict(q=q.half())):
+        with pytest.raises(ValueError):
+            SA.softmax_attention_paged(**{**ok, **kw})
+
+
+def test_decoding_with_beams():
+    """Two users, three beams each: the prompt goes into shared pages, every step appends to the beams' own pages, attends
+    behind the shared prefix and draws the next item; each call against its own statement on the same inputs."""
+    from recsdk_b200.ops import sampling
+
+    g = torch.Generator(device=DEV).manual_seed(12)
+    H, Hkv, D, page, V, steps = 8, 2, 64, 16, 211, 20
+    prompt, beams = [45, 30], 3
+    emb = torch.randn(V, (H + 2 * Hkv) * D, generator=g, device=DEV).bfloat16()
+    head = (torch.randn(V, H * D, generator=g, device=DEV) / 8).bfloat16()
+    table = SA.rotary_table(100, D, device=DEV)
+    cache = torch.full((20, 2, page, Hkv, D), math.nan, dtype=torch.bfloat16, device=DEV)
+    split = lambda x: (t.unflatten(1, (-1, D)) for t in x.split([H * D, Hkv * D, Hkv * D], dim=1))  # noqa: E731
+    # the prompts
+    items = torch.randint(0, V, (75,), generator=g, device=DEV)
+    b = torch.tensor([0] * 45 + [1] * 30, dtype=torch.int32, device=DEV)
+    pos = torch.cat([torch.arange(45), torch.arange(30)]).int().to(DEV)
+    p_ids, p_ptr = torch.tensor([7, 3, 11, 0, 9], dtype=torch.int32, device=DEV), torch.tensor([0, 3, 5], dtype=torch.int32, device=DEV)
+    q, k, v = split(emb[items])
+    q = SA.append_kv_rotary(q, k, v, cache, b, pos, p_ids, p_ptr, page, table)
+    o = SA.softmax_attention_paged(q, cache, _off(prompt), _off(prompt), p_ids, p_ptr, page, window=32, num_sinks=4)
+    want, _ = SA.softmax_attention_ref(q, cache, _off(prompt), _off(prompt), p_ids, p_ptr, page, window=32, num_sinks=4, dtype=torch.float64)
+    assert (o.double() - want).abs().max() < 0.05
+    # the beams
+    n = 2 * beams
+    own_ids = torch.tensor([1, 2, 4, 5, 6, 8, 10, 12, 13, 14, 15, 16], dtype=torch.int32, device=DEV)
+    own_ptr, bi = torch.arange(0, 13, 2, dtype=torch.int32, device=DEV), torch.arange(n, dtype=torch.int32, device=DEV)
+    groups = torch.tensor([0, beams, n], dtype=torch.int32, device=DEV)
+    start = torch.tensor(prompt, dtype=torch.int32, device=DEV).repeat_interleave(beams)
+    items = torch.randint(0, V, (n,), generator=g, device=DEV)
+    for step in range(steps):
+        q, k, v = split(emb[items])
+        # positions count from the prompt, slots from the beam's own pages
+        slots = torch.full_like(bi, step)
+        before = k.clone()
+        q0, q = q, SA.append_kv_rotary(q, k, v, cache, bi, start + step, own_ids, own_ptr, page, table, slots=slots)
+        cos, sin = table[(start + step).long()][:, None].chunk(2, dim=-1)
+        assert (q.double() - SA._rotate_ref(q0.double(), cos.double(), sin.double(), False)).abs().max() < 0.02
+        at = own_ids.long()[own_ptr[:-1].long() + step // page]
+        turned = SA._rotate_ref(before.double(), cos.double(), sin.double(), False)
+        assert (cache[at, 0, step % page].double() - turned).abs().max() < 0.02 and torch.equal(cache[at, 1, step % page], v)
+        kw = dict(group_offsets=groups)
+        args = (q, cache, _off([1] * n), _off([step + 1] * n), own_ids, own_ptr)
+        pre = (_off(prompt), p_ids, p_ptr)
+        o = SA.softmax_attention_shared_prefix(*args, *pre, page, **kw)
+        want, _ = SA.softmax_attention_ref(*args, page, prefix_offsets=pre[0], prefix_page_ids=p_ids, prefix_page_indptr=p_ptr,
+                                           dtype=torch.float64, **kw)
+        assert torch.isfinite(o).all() and (o.double() - want).abs().max() < 0.05
+        scores = o.flatten(1).float() @ head.float().t()
+        u = torch.rand(n, generator=g, device=DEV)
+        items, lp = sampling.sample_scores(scores, u, temperature=0.9, top_k=40, top_p=0.9, min_p=0.01)
+        ref, _ = sampling.sample_scores_ref(scores, u, temperature=0.9, top_k=40, top_p=0.9, min_p=0.01)
+        assert torch.equal(items, ref) and (lp <= 0).all()
+    _lib.check_status()

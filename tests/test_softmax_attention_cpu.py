@@ -169,3 +169,17 @@ def test_ranker_recommends_from_its_scores():
     ids, lp = make().recommend(users, hist, cands, x, u, temperature=0.5, top_p=0.9)
     want, want_lp = S.sample_scores(scores, u, torch.tensor([0, 6, 6, 10]), temperature=0.5, top_p=0.9)
     assert torch.equal(ids, want) and torch.equal(lp, want_lp) and ids[1] == -1
+
+
+def test_slots_are_where_keys_go():
+    cache, ids, ptr, g = _paged([20], 16, 2, 64)
+    q, k, v = torch.randn(2, 4, 64, generator=g), torch.randn(2, 2, 64, generator=g), torch.randn(2, 2, 64, generator=g)
+    table = SA.rotary_table(64, 64)
+    z, pos = torch.zeros(2, dtype=torch.int32), torch.tensor([40, 41], dtype=torch.int32)
+    SA.append_kv_rotary(q, k, v, cache, z, pos, ids, ptr, 16, table, slots=torch.tensor([15, 16]))
+    cos, sin = table[pos.long()][:, None].chunk(2, dim=-1)
+    turned = SA._rotate_ref(k, cos, sin, False)
+    assert torch.equal(cache[ids[0].long(), 0, 15], turned[0]) and torch.equal(cache[ids[1].long(), 0, 0], turned[1])
+    assert torch.equal(cache[ids[0].long(), 1, 15], v[0])
+    with pytest.raises(ValueError):
+        SA.append_kv_rotary(q, k, v, cache, z, pos, ids, ptr, 16, table, slots=torch.tensor([15]))
