@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
   long long* found_base = reinterpret_cast<long long*>(tail + 320);            // [NW]
   int* found = reinterpret_cast<int*>(tail + 384);                             // [NW]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 416);
+  long long* starts = reinterpret_cast<long long*>(tail + 448);                // [NW + 1] where the workers' shares begin
   float* ml = reinterpret_cast<float*>(tail + 1024);                           // [NW][RT][2]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nb = p.a.B + p.b.B;
@@ -113,22 +114,29 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
     total += sums[i];
   }
   const Shares sh(total, gridDim.x * PER_CTA);
-  for (int x = 0; x < PER_CTA; ++x) {
-    const int c = blockIdx.x * PER_CTA + x;
-    const long long at = c < sh.n ? sh.begin(c) : -1;
-    if (at >= before && at < before + mine) {
-      long long base = before;
-      for (int i = tid * per;; ++i) {
-        const long long n = units_of(items_of<KT, W>(p, seq_of(p, i)));
-        if (at < base + n) { found[x] = i; found_base[x] = base; break; }
-        base += n;
-      }
+  if (tid <= PER_CTA) {
+    const int c = blockIdx.x * PER_CTA + tid;
+    starts[tid] = c <= sh.n ? sh.begin(c) : -1;
+  }
+  __syncthreads();
+  // the sequences that the CTA's workers begin with: those of the threads that counted them
+  long long last = -1;
+#pragma unroll
+  for (int x = 0; x < PER_CTA; ++x) if (starts[x + 1] >= 0) last = starts[x];
+  if (mine > 0 && starts[0] < before + mine && last >= before) {
+    long long base = before;
+    for (int i = tid * per; i < min((tid + 1) * per, nb); ++i) {
+      const long long n = per == 1 ? mine : units_of(items_of<KT, W>(p, seq_of(p, i)));
+#pragma unroll
+      for (int x = 0; x < PER_CTA; ++x)
+        if (starts[x + 1] >= 0 && starts[x] >= base && starts[x] < base + n) { found[x] = i; found_base[x] = base; }
+      base += n;
     }
   }
   __syncthreads();
   const int me = W == 1 ? warp : 0, turn = W == 1 ? 0 : warp;                  // worker of the CTA, this warp's turn in it
   const int wk = blockIdx.x * PER_CTA + me;
-  const long long p0 = wk < sh.n ? sh.begin(wk) : 0, p1 = wk < sh.n ? sh.begin(wk + 1) : 0;
+  const long long p0 = starts[me + 1] >= 0 ? starts[me] : 0, p1 = max(starts[me + 1], 0LL);
   Meta m;
   m.valid = 0;
   if (p0 < p1) {
@@ -146,7 +154,8 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
       const Items it = items_of<KT, W>(p, s);
       const long long n_b = units_of(it);
       if (pos >= base + n_b) { base += n_b; ++b; continue; }
-      const int item = static_cast<int>((pos - base) / it.units);
+      const unsigned long long at = static_cast<unsigned long long>(pos - base);
+      const int item = static_cast<int>(at >> 32 ? at / it.units : static_cast<uint32_t>(at) / static_cast<uint32_t>(it.units));
       const int off = static_cast<int>(pos - base - static_cast<long long>(item) * it.units);
       const int qt = item / p.Hkv, h0 = item - qt * p.Hkv;
       const int rows = min(s.len_q * p.G - qt * RT, RT);
