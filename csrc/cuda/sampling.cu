@@ -15,9 +15,10 @@
 // polynomial of degree 3 (relative error (ln2/512)^4 / 24 = 1.4e-13).  Sums inside the histograms are whole numbers (2^-44 of the largest weight for
 // rows up to 2^18 items, coarser beyond), so atomics in any order give the same bits.
 //
-// Bound: the row is read from memory once, into the shared memory of a cluster of CTAs (1 to 8 by its size and by how many
-// rows there are), which then exchange histograms and sums through distributed shared memory; what remains is the 64-bit
-// arithmetic, about ten operations per item and pass.  Rows that do not fit are read again from L2.
+// A row is read from memory once, into the shared memory of a cluster of CTAs (1 to 8 by its size and by how many rows there
+// are), which then exchange histograms and sums through distributed shared memory; rows that do not fit are read again from
+// L2.  Bound: for many long rows the histogram's shared-memory atomics (a third of the time) and the 64-bit arithmetic, ten
+// operations per item and pass, not the memory; for few or short rows the exchanges between the passes.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -134,7 +135,7 @@ __device__ __forceinline__ void for_each(const T* x, int n, F&& f) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
+__global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
   T* store = reinterpret_cast<T*>(smem + (sizeof(Shared) + 15) / 16 * 16);
@@ -564,9 +565,12 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       const int nv = b1 > b0 ? (b1 - b0 - head) / V : 0, tail = b0 + max(head, 0) + nv * V;
       if (b1 > b0) {
         take(lane < head ? to_f<T>(x[b0 + lane]) : NAN);
+        const uint4* xv = reinterpret_cast<const uint4*>(x + b0 + head);
+        uint4 next = make_uint4(0, 0, 0, 0);
+        if (lane < nv) next = xv[lane];
         for (int i = 0; i < nv; i += 32) {
-          uint4 u = make_uint4(0, 0, 0, 0);
-          if (i + lane < nv) u = reinterpret_cast<const uint4*>(x + b0 + head)[i + lane];
+          const uint4 u = next;
+          if (i + 32 + lane < nv) next = xv[i + 32 + lane];
           const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
           for (int j = 0; j < V; ++j) take(i + lane < nv ? to_f<T>(e[j]) : NAN);
@@ -669,17 +673,17 @@ template <typename T>
 int launch(SampleArgs p, int num_sms, cudaStream_t st) {
   constexpr int fixed_bytes = (sizeof(Shared) + 15) / 16 * 16 + 16;
   constexpr int max_bytes = 227 * 1024;
-  constexpr int half_bytes = 113 * 1024;                           // two CTAs per SM
   // The most a row can have (of jagged rows: all but never, so assume twice the average).
   long long longest = p.width;
   if (p.offsets) longest = min(p.width, 2 * p.width / p.rows + 1024);
-  // CTAs per row: enough to hold it in shared memory at two CTAs per SM, and more while SMs would stay idle and a CTA keeps
-  // some thousand items
+  // CTAs per row: as many as run at once (one per SM: its 16 warps need 128 registers a thread to keep eight items' arithmetic in
+  // flight; two per SM at 64 took 226 instead of 205 us for 256 rows of 131071 bf16), while each keeps some thousand
+  // items.  More than that in turns, each with its own exchanges, cost more than reading a row again from L2 where it does
+  // not fit (256 rows of 131071 fp32: 593 us with eight CTAs a row, 281 us with one).
   int c = 1;
-  while (c < MAX_CLUSTER && (longest + c - 1) / c * static_cast<long long>(sizeof(T)) + fixed_bytes > half_bytes) c *= 2;
   while (c < MAX_CLUSTER && 2LL * c * p.rows <= num_sms && longest / c > 4096) c *= 2;
   const long long slice = (((longest + c - 1) / c + 31) / 32 * 32) * static_cast<long long>(sizeof(T));
-  const long long room = slice + fixed_bytes <= half_bytes ? slice : min(slice, static_cast<long long>(max_bytes - fixed_bytes));
+  const long long room = min(slice, static_cast<long long>(max_bytes - fixed_bytes));
   p.cap = static_cast<int>(room / sizeof(T));
   const int bytes = fixed_bytes + static_cast<int>(room);
   static std::atomic<unsigned long long> done{0};
