@@ -4,21 +4,25 @@
 //     the first k;  of those, up to the first whose running sum reaches p times their sum;  of those, w_i >= min_p
 //   -> the smallest index i whose running sum over the kept items, in index order, exceeds u times their sum.
 //
-// Every filter keeps a beginning of the same order, so no sort is needed: a histogram over 1/64 octaves of the weight and a
-// radix descent inside the bin that the cut falls into find the last kept value (by count for k, by weight for p) and how
-// many of the items that share it are kept.  Where at most LIST items can be kept (short rows, small k), one CTA sorts
-// those instead.
+// Every filter keeps a beginning of the same order, so no sort is needed: histograms find the last kept value (by count for k,
+// by weight for p) and how many of the items that share it are kept.
+//   16-bit scores: the histogram has a bin for each of the 65536 patterns, 16-bit counts (a row where one passes 65535 is noticed
+//     by their sum and done the other way).  The weights of the patterns that occur, some hundreds, are all that is computed;
+//     afterwards they take the counts' place as a table, and the draw reads them from there.
+//   fp32: bins of 1/64 octave of the weight, and a radix descent inside the bin that the cut falls into.
+// Where at most LIST items can be kept (short rows, small k), one CTA sorts those instead.
 //
 // Weights are computed and summed in 64 bits: with N kept items each of the N borders can go either way with the sums'
 // relative error as its chance, and 32-bit exponentials (1e-7 each) would draw a neighbour in every hundredth row of 10^5
 // items.  The exponential is table-driven (Tang, ACM TOMS 15, 1989): 2^(n/256) from a table, 2^(f/256), |f| <= 1/2, as a
-// polynomial of degree 3 (relative error (ln2/512)^4 / 24 = 1.4e-13).  Sums inside the histograms are whole numbers (2^-44 of the largest weight for
-// rows up to 2^18 items, coarser beyond), so atomics in any order give the same bits.
+// polynomial of degree 3 (relative error (ln2/512)^4 / 24 = 1.4e-13).  Sums inside the histograms are whole numbers (2^-44 of
+// the largest weight for rows up to 2^18 items, coarser beyond), so atomics in any order give the same bits.
 //
 // A row is read from memory once, into the shared memory of a cluster of CTAs (1 to 8 by its size and by how many rows there
 // are), which then exchange histograms and sums through distributed shared memory; rows that do not fit are read again from
-// L2.  Bound: for many long rows the histogram's shared-memory atomics (a third of the time) and the 64-bit arithmetic, ten
-// operations per item and pass, not the memory; for few or short rows the exchanges between the passes.
+// L2.  Bound: for many long rows shared memory (one CTA, 131071 bf16 items, cycles: counting 19000, the draw's sums out of the
+// table 27000, everything else 25000), not the memory; in fp32 the histogram's atomics and the 64-bit arithmetic, ten
+// operations per item and pass; for few or short rows the chain of short steps between the passes.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -32,12 +36,16 @@ constexpr int BINS = 2048, PB = BINS / NT;
 constexpr int MAX_CLUSTER = 8;
 constexpr int TABLE = 256;
 constexpr int LIST = 1024;                      // items that are sorted, or kept aside for a descent
+constexpr int GROUP = 64, GROUPS = 65536 / GROUP;   // 16-bit patterns are looked through in groups
+constexpr int COUNT_BYTES = 65536 * 2;
+constexpr int SLOTS = COUNT_BYTES / 8 / GROUP;  // groups whose weights fit where the counts were; the first holds zeros
 
 struct SampleArgs {
   const void* scores; long long ld;             // dense: rows of `width`, `ld` elements apart
   const void* offsets; int offsets64;           // jagged: [rows + 1] into scores (then `width` is its length), or null
   long long width; int rows;
   int cap;                                      // elements of a slice that shared memory holds
+  int counted;                                  // count the patterns (16-bit scores, one CTA per row)
   const float* uniform;
   const float* temperature; const int* top_k; const float* top_p; const float* min_p;   // per row, or null: the values below
   float temperature_v; int top_k_v; float top_p_v, min_p_v;
@@ -57,6 +65,17 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 constexpr uint32_t KEY_NONE = 0x007fffffu;                         // -inf: never drawn
+
+// The same for the patterns of a 16-bit type, two at a time; NaN are the patterns outside (-inf, inf], -0 is next to 0.
+__device__ __forceinline__ uint32_t patterns_of(uint32_t two) { return two ^ (((two >> 15) & 0x00010001u) * 0xffffu | 0x80008000u); }
+template <typename T> __device__ __forceinline__ float pattern_value(uint32_t k) {
+  const unsigned short b = static_cast<unsigned short>(k ^ ((k >> 15) ? 0x8000u : 0xffffu));
+  return to_f<T>(*reinterpret_cast<const T*>(&b));
+}
+template <typename T> constexpr uint32_t INF16 = 0;                // the pattern of inf; its group holds no other number
+template <> constexpr uint32_t INF16<__nv_bfloat16> = 0xff80u;
+template <> constexpr uint32_t INF16<__half> = 0xfc00u;
+constexpr uint32_t ZERO16 = 0x8000u;
 
 // What the CTAs of a cluster read of one another
 struct __align__(16) Shared {
@@ -79,19 +98,18 @@ struct __align__(16) Shared {
 // exp((x - top) / T), 64 bits
 struct Weigher {
   const double* table;
-  double scale;                                 // 1/256 octaves per unit of score
+  double rate;                                  // 1 / T
   float top;
   // with its binary exponent raised by `up`; x is not NaN and at most top
   __device__ __forceinline__ double operator()(float x, int up = 0) const {
-    const double t = x == top ? 0.0 : (static_cast<double>(x) - static_cast<double>(top)) * scale;
+    const double t = x == top ? 0.0 : (static_cast<double>(x) - static_cast<double>(top)) * rate;
     const double magic = 6755399441055744.0;                       // 1.5 * 2^52: the sum's low word is the nearest whole number
-    const double nd = t + magic;
+    const double nd = fma(t, TABLE * 1.4426950408889634, magic);
     const int n = __double2loint(nd);
-    const double f = t - (nd - magic);
-    constexpr double c1 = 0.6931471805599453 / TABLE, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3;
-    const double q = fma(fma(fma(c3, f, c2), f, c1), f, 1.0) * table[n & (TABLE - 1)];
+    const double f = fma(nd - magic, -0.6931471805599453 / TABLE, t);              // (next to 0 it is t itself: 1 - t is rounded once)
+    const double q = fma(fma(fma(1.0 / 6.0, f, 0.5), f, 1.0), f, 1.0) * table[n & (TABLE - 1)];
     const double w = __hiloint2double(__double2hiint(q) + (((n >> 8) + up) << 20), __double2loint(q));
-    return t > -260000.0 ? w : 0.0;                                // (2^-1015; also for -inf)
+    return t > -700.0 ? w : 0.0;                                   // (2^-1010; also for -inf)
   }
   // the weight in units of 2^-shift, rounded (up <= 44)
   __device__ __forceinline__ unsigned long long fixed(float x, int up) const {
@@ -138,7 +156,8 @@ template <typename T>
 __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
-  T* store = reinterpret_cast<T*>(smem + (sizeof(Shared) + 15) / 16 * 16);
+  unsigned int* counts = reinterpret_cast<unsigned int*>(smem + (sizeof(Shared) + 15) / 16 * 16);   // two to a word
+  T* store = reinterpret_cast<T*>(smem + (sizeof(Shared) + 15) / 16 * 16 + (p.counted ? COUNT_BYTES : 0));
   cg::cluster_group cluster = cg::this_cluster();
   const int c = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -170,38 +189,216 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
     const float uf = p.uniform[row];
     const double u = uf > 0.f ? static_cast<double>(uf) : 0.0;
 
-    // ---- bring the slice in; its largest score (fmaxf passes over NaN)
-    float most = -INFINITY;
-    if (n <= p.cap) {
-      // at the same offset from a 16-byte border, so that both sides move in vectors
-      T* y = store + (reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T);
+    // ---- bring the slice in, with a look at each 16 bytes (`vec`) and at the ends (`one`)
+    auto bring = [&](auto&& vec, auto&& one) {
       constexpr int V = 16 / sizeof(T);
       const int head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T)));
       const int nv = (n - head) / V;
-      for (int i = tid; i < head; i += NT) { y[i] = x[i]; most = fmaxf(most, to_f<T>(x[i])); }
+      const bool keep = n <= p.cap;
+      // at the same offset from a 16-byte border, so that both sides move in vectors
+      T* y = store + (reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T);
       const uint4* xv = reinterpret_cast<const uint4*>(x + head);
       uint4* yv = reinterpret_cast<uint4*>(y + head);
 #pragma unroll 4
       for (int i = tid; i < nv; i += NT) {
         const uint4 v = __ldg(xv + i);
-        yv[i] = v;
+        if (keep) yv[i] = v;
+        vec(v);
+      }
+      const int ends = n - nv * V;
+      if (tid < ends) {
+        const int i = tid < head ? tid : nv * V + tid;
+        if (keep) y[i] = x[i];
+        one(x[i]);
+      }
+      if (keep) x = y;
+    };
+
+    // ---- 16-bit scores: how often each pattern occurs is all that the cuts need
+    uint32_t top_key = 0, top16 = 0, cut16 = 0;
+    Cut cut = {KEY_NONE, 0};
+    bool counted = false;
+    unsigned short* slot = reinterpret_cast<unsigned short*>(s.lo + GROUPS);       // by group: where its weights are
+    unsigned short* group = slot + GROUPS;                         // those that are not empty, from the highest down
+    int groups = 0;
+    if constexpr (sizeof(T) == 2) {
+      if (p.counted && temp > 0.f && n_row > LIST && !(top_k > 0 && top_k <= LIST / 2)) {
+        unsigned int* in_group = s.lo;
+        unsigned long long* mass = reinterpret_cast<unsigned long long*>(s.hi);    // of a group
+        for (int i = tid; i < COUNT_BYTES / 16; i += NT) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        auto count = [&](uint32_t k) { atomicAdd(counts + (k >> 1), (k & 1) ? 0x10000u : 1u); };
+        auto count2 = [&](uint32_t two) {
+          const uint32_t k = patterns_of(two);
+          count(k & 0xffffu);
+          count(k >> 16);
+        };
+        bring([&](const uint4& v) { count2(v.x); count2(v.y); count2(v.z); count2(v.w); },
+              [&](const T& v) { count(patterns_of(*reinterpret_cast<const unsigned short*>(&v)) & 0xffffu); });
+        __syncthreads();
+        if (tid == 0) {
+          s.u0 = 0; s.u1 = 0;
+          // -0 is 0
+          const unsigned int minus = counts[ZERO16 / 2 - 1] >> 16;
+          if (minus + (counts[ZERO16 / 2] & 0xffffu) > 0xffffu) {
+            s.u1 = 1;
+          } else {
+            counts[ZERO16 / 2 - 1] &= 0xffffu;
+            counts[ZERO16 / 2] += minus;
+          }
+        }
+        __syncthreads();
+        constexpr int g_inf = INF16<T> / GROUP, g_none = (0xffffu - INF16<T>) / GROUP;
+        unsigned int seen = 0;
+        int g_top = 0;
+#pragma unroll 4
+        for (int i = tid; i < COUNT_BYTES / 16; i += NT) {         // 8 threads per group
+          uint4 w = reinterpret_cast<const uint4*>(counts)[i];
+          const int g = i / (GROUP / 8);
+          seen += (w.x & 0xffffu) + (w.x >> 16) + (w.y & 0xffffu) + (w.y >> 16) + (w.z & 0xffffu) + (w.z >> 16) + (w.w & 0xffffu) + (w.w >> 16);
+          if (g >= g_inf || g <= g_none) {
+            w = make_uint4(g == g_inf && i % (GROUP / 8) == 0 ? w.x & 0xffffu : 0, 0, 0, 0);
+            reinterpret_cast<uint4*>(counts)[i] = w;
+          }
+          unsigned int m = (w.x & 0xffffu) + (w.x >> 16) + (w.y & 0xffffu) + (w.y >> 16) + (w.z & 0xffffu) + (w.z >> 16) + (w.w & 0xffffu) + (w.w >> 16);
+          m += __shfl_xor_sync(0xffffffffu, m, 1);
+          m += __shfl_xor_sync(0xffffffffu, m, 2);
+          m += __shfl_xor_sync(0xffffffffu, m, 4);
+          if (i % (GROUP / 8) == 0) in_group[g] = m;
+          if (m) g_top = max(g_top, g);
+        }
+        seen = __reduce_add_sync(0xffffffffu, seen);
+        g_top = __reduce_max_sync(0xffffffffu, g_top);
+        if (lane == 0) { s.wcnt[warp] = seen; atomicMax(&s.u0, g_top); }
+        __syncthreads();
+        seen = 0;
+        for (int i = 0; i < NWARP; ++i) seen += s.wcnt[i];
+        // A count that passed 16 bits took 65535 or 65536 from the sum: such a row is done by weight, below.
+        counted = seen == static_cast<unsigned int>(n_row) && !s.u1;
+        g_top = s.u0;
+        __syncthreads();
+        if (counted) {
+          const unsigned int wt_ = counts[g_top * 32 + lane];
+          top16 = g_top * GROUP + __reduce_max_sync(0xffffffffu, (wt_ >> 16) ? 2 * lane + 1 : wt_ ? 2 * lane : 0);
+          if (in_group[g_top] == 0) {
+            if (tid == 0) { p.ids[row] = -1; p.logprobs[row] = -INFINITY; }
+            __syncthreads();
+            continue;
+          }
+          const float top_f = pattern_value<T>(top16);
+          top_key = key_of(top_f);
+          Weigher wt;
+          wt.table = s.table; wt.top = top_f;
+          wt.rate = 1.0 / static_cast<double>(temp);
+          const int shift_fx = 62 - max(18, 32 - __clz(n_row));
+          // list the groups, two per thread (and always -0's, for its weight)
+          static_assert(GROUPS == 2 * NT, "two groups per thread");
+          {
+            const int g = GROUPS - 1 - 2 * tid;
+            const bool f0 = in_group[g] || g == ZERO16 / GROUP - 1, f1 = in_group[g - 1] != 0;
+            const unsigned int b0 = __ballot_sync(0xffffffffu, f0), b1 = __ballot_sync(0xffffffffu, f1);
+            if (lane == 0) s.wcnt[warp] = __popc(b0) + __popc(b1);
+            __syncthreads();
+            int at = __popc(b0 & ((1u << lane) - 1)) + __popc(b1 & ((1u << lane) - 1));
+            for (int i = 0; i < NWARP; ++i) {
+              if (i < warp) at += s.wcnt[i];
+              groups += s.wcnt[i];
+            }
+            if (f0) group[at++] = g;
+            if (f1) group[at] = g - 1;
+            __syncthreads();
+          }
+          for (int by_mass = 0; by_mass < 2; ++by_mass) {
+            if (by_mass ? !(top_p < 1.f) : !(top_k > 0 && top_k < n_row)) continue;
+            auto value = [&](uint32_t k, unsigned int m) -> unsigned long long {
+              if (k <= cut16) m = k == cut16 ? cut.ties : 0;
+              return m * (by_mass ? wt.fixed(pattern_value<T>(k), shift_fx) : 1ULL);
+            };
+            // eight threads per group, eight patterns each
+            for (int i = tid; i < (groups * (GROUP / 8) + 31) / 32 * 32; i += NT) {
+              const int at = i / (GROUP / 8);
+              const int k = group[min(at, groups - 1)] * GROUP + i % (GROUP / 8) * 8;
+              const uint4 w = *reinterpret_cast<const uint4*>(counts + k / 2);
+              const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+              unsigned long long v = 0;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v += value(k + j, j & 1 ? ws[j / 2] >> 16 : ws[j / 2] & 0xffffu);
+              v += __shfl_xor_sync(0xffffffffu, v, 1);
+              v += __shfl_xor_sync(0xffffffffu, v, 2);
+              v += __shfl_xor_sync(0xffffffffu, v, 4);
+              if (i % (GROUP / 8) == 0 && at < groups) mass[at] = v;
+            }
+            if (tid == 0) s.u2 = 0;
+            __syncthreads();
+            const unsigned long long v0 = 2 * tid < groups ? mass[2 * tid] : 0, v1 = 2 * tid + 1 < groups ? mass[2 * tid + 1] : 0;
+            unsigned long long incl = v0 + v1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o);
+              if (lane >= o) incl += y;
+            }
+            if (lane == 31) s.wmass[warp] = incl;
+            __syncthreads();
+            unsigned long long before = incl - v0 - v1, all = 0, target;
+            for (int i = 0; i < NWARP; ++i) {
+              if (i < warp) before += s.wmass[i];
+              all += s.wmass[i];
+            }
+            if (by_mass) {
+              const double t = ceil(static_cast<double>(top_p) * static_cast<double>(all));
+              target = t > 1.0 ? static_cast<unsigned long long>(t) : 1ULL;        // at least the first item
+            } else {
+              target = all <= static_cast<unsigned int>(top_k) ? ~0ULL : static_cast<unsigned long long>(top_k);
+            }
+            if (before < target && before + v0 >= target) { s.u0 = group[2 * tid]; s.m0 = before; s.u2 = 1; }
+            before += v0;
+            if (before < target && before + v1 >= target) { s.u0 = group[2 * tid + 1]; s.m0 = before; s.u2 = 1; }
+            __syncthreads();
+            if (s.u2) {
+              // its patterns, two per lane from the highest down
+              const int at = s.u0 * 32 + 31 - lane;
+              const unsigned int w = counts[at], k = 2 * at;
+              const unsigned long long a1 = value(k + 1, w >> 16), a0 = value(k, w & 0xffffu);
+              unsigned long long run = a0 + a1;
+#pragma unroll
+              for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long y = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += y;
+              }
+              unsigned long long above = s.m0 + run - a0 - a1;
+              const int who = __ffs(__ballot_sync(0xffffffffu, s.m0 + run >= target)) - 1;
+              const bool second = above + a1 < target;
+              if (second) above += a1;
+              const unsigned int key = k + (second ? 0 : 1);
+              unsigned long long kept = target - above;
+              if (by_mass) {
+                const unsigned long long one = wt.fixed(pattern_value<T>(key), shift_fx);
+                const unsigned int most = key == cut16 ? cut.ties : 0xffffffffu;
+                kept = one ? min((kept + one - 1) / one, static_cast<unsigned long long>(most)) : most;
+              }
+              cut.ties = __shfl_sync(0xffffffffu, static_cast<unsigned int>(kept), who);
+              cut16 = __shfl_sync(0xffffffffu, key, who);
+              cut.key = key_of(pattern_value<T>(cut16));
+            }
+            __syncthreads();
+          }
+        }
+      }
+    }
+    if (!counted) {
+      float most = -INFINITY;                                      // (fmaxf passes over NaN)
+      bring([&](const uint4& v) {
         const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-        for (int j = 0; j < V; ++j) most = fmaxf(most, to_f<T>(e[j]));
-      }
-      for (int i = head + nv * V + tid; i < n; i += NT) { y[i] = x[i]; most = fmaxf(most, to_f<T>(x[i])); }
-      x = y;
-    } else {
-      for_each<T>(x, n, [&](auto& v, int) {
-        for (float e : v) most = fmaxf(most, e);
-      });
+        for (int j = 0; j < static_cast<int>(16 / sizeof(T)); ++j) most = fmaxf(most, to_f<T>(e[j]));
+      }, [&](const T& v) { most = fmaxf(most, to_f<T>(v)); });
+      top_key = __reduce_max_sync(0xffffffffu, key_of(most));
+      if (lane == 0) s.wcnt[warp] = top_key;
     }
-    uint32_t top_key = __reduce_max_sync(0xffffffffu, key_of(most));
-    if (lane == 0) s.wcnt[warp] = top_key;
     if (tid == 0) { s.listed = 0; s.first = 0xffffffffu; }
     __syncthreads();
     if (tid == 0) {
-      for (int i = 0; i < NWARP; ++i) top_key = max(top_key, s.wcnt[i]);
+      if (!counted) for (int i = 0; i < NWARP; ++i) top_key = max(top_key, s.wcnt[i]);
       s.best = top_key;
     }
     sync();
@@ -230,16 +427,16 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
     const float top_f = value_of(top_key);
     Weigher wt;
     wt.table = s.table; wt.top = top_f;
-    wt.scale = TABLE * 1.4426950408889634 / static_cast<double>(temp);
+    wt.rate = 1.0 / static_cast<double>(temp);
     auto wk = [&](uint32_t k) { return wt(value_of(k)); };
-    Cut cut = {KEY_NONE, 0};
-    float cut_f = -INFINITY;                                       // its value
+    float cut_f = value_of(cut.key);
     // bins of 1/64 octave of the weight, the last one open: all that matters is that they are monotone in the score
     const float bin_scale = 64.f * 1.44269504f / temp, bin_shift = top_f * bin_scale;
     auto place_of = [&](float x) { return fmaxf(fminf(fmaf(x, -bin_scale, bin_shift), BINS - 1.f), 0.f); };
     auto bin_of = [&](float x) { return static_cast<int>(place_of(x)); };
     const int shift_fx = 62 - max(18, 32 - __clz(n_row));
     const double mp = static_cast<double>(min_p);
+    auto enough = [&](double w) { return w >= mp && mp < 1.0; };   // next to the largest score the weight rounds to 1, but is less
 
     // ---- the first CTA's list holds everything that can be kept: sort, cut, draw
     auto draw_listed = [&]() {
@@ -302,7 +499,7 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
       const double before = scan(w0, w1, all);
       const double limit = top_p < 1.f ? static_cast<double>(top_p) * all : INFINITY;
       auto kept = [&](int i, double w, double b) {
-        return i < m && (top_k <= 0 || i < top_k) && (i == 0 || b < limit) && (w >= mp || static_cast<uint32_t>(s.list[i] >> 32) == top_key);
+        return i < m && (top_k <= 0 || i < top_k) && (i == 0 || b < limit) && (enough(w) || static_cast<uint32_t>(s.list[i] >> 32) == top_key);
       };
       const bool k0 = kept(i0, w0, before), k1 = kept(i1, w1, before + w0);
       const unsigned int at0 = k0 ? 0xffffffffu - static_cast<unsigned int>(s.list[i0]) : 0xffffffffu;
@@ -345,7 +542,7 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
     }
     bool drawn = false;
 
-    for (int by_mass = 0; by_mass < 2 && !drawn; ++by_mass) {
+    for (int by_mass = 0; by_mass < 2 && !drawn && !counted; ++by_mass) {
       if (by_mass ? !(top_p < 1.f) : !(top_k > 0 && top_k < n_row)) continue;
       // Finds, from the top, the bin where the running sum reaches the target.  -> u2: found, u0: the bin, u1 / m0: what is above it
       unsigned long long target = 0, above = 0, in_bin = 0, all = 0;
@@ -515,28 +712,66 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
       continue;
     }
     // ---- draw: which CTA, which warp, ... holds the item where the running sum passes u * total
+    // where patterns were counted, the kept ones' weights take the counts' place, if their groups fit
+    bool tabled = false;
+    double* weights = reinterpret_cast<double*>(counts);
+    uint32_t tie16 = 0x10000u, tie16b = 0x10000u, low16 = 0;       // (0x10000: no pattern)
+    if constexpr (sizeof(T) == 2) {
+      if (counted) {
+        auto in = [&](int i) { return i < groups && group[i] >= cut16 / GROUP; };      // the first of the list
+        reinterpret_cast<uint32_t*>(slot)[tid] = 0;
+        if (tid == 0) s.u2 = 0xffffu;
+        const int used = 1 + __syncthreads_count(in(tid)) + __syncthreads_count(in(tid + NT));
+        tabled = used <= SLOTS;
+        if (tabled) {
+          if (tid + 1 < used) slot[group[tid]] = tid + 1;
+          uint32_t low = 0xffffu;
+          for (int i = tid; i < used * GROUP; i += NT) {
+            double w = 0.0;
+            if (i >= GROUP) {
+              const uint32_t k = group[i / GROUP - 1] * GROUP + i % GROUP;
+              if (k > cut16 && k <= top16) {
+                w = wt(pattern_value<T>(k));
+                if (enough(w) || pattern_value<T>(k) == top_f) low = min(low, k); else w = 0.0;
+              }
+            }
+            weights[i] = w;
+          }
+          low = __reduce_min_sync(0xffffffffu, low);
+          if (lane == 0) atomicMin(&s.u2, low);
+          __syncthreads();
+          low16 = s.u2;
+          if (cut.ties) {
+            tie16 = cut16;
+            tie16b = cut16 == ZERO16 ? ZERO16 - 1 : cut16;
+          }
+        }
+      }
+    }
+    auto weight16 = [&](uint32_t k) { return weights[slot[k / GROUP] * GROUP + k % GROUP]; };
     // min-p as a key: the smallest one with enough weight, by 32 tries at a time
     uint32_t lim = cut.key;                                        // kept: keys above it, and the cut's ties
-    if (mp > 0.0) {
-      uint32_t below = KEY_NONE, enough = top_key;                 // w(below) < mp <= w(enough)
+    if (mp > 0.0 && !tabled) {
+      uint32_t below = mp < 1.0 ? KEY_NONE : top_key - 1, most = top_key;            // w(below) < mp <= w(most)
       if (mp < 1.0 && !isinf(top_f)) {
         // where it should be, give or take: a bracket that is checked before it is used
         const float guess = top_f + temp * __logf(min_p), slack = 1e-3f * (fabsf(temp) + 1e-3f * fabsf(guess));
         const float g0 = guess - slack, g1 = fminf(guess + slack, top_f);
-        if (g0 > -INFINITY && g0 < g1 && wt(g0) < mp && wt(g1) >= mp) { below = key_of(g0); enough = key_of(g1); }
+        if (g0 > -INFINITY && g0 < g1 && wt(g0) < mp && wt(g1) >= mp) { below = key_of(g0); most = key_of(g1); }
       }
-      while (enough - below > 1) {
-        const uint32_t step = (enough - below - 1) / 32 + 1, k = below + step * (lane + 1);
-        const unsigned int yes = __ballot_sync(0xffffffffu, k < enough && k > below && wk(k) >= mp);
-        const uint32_t tried = (enough - below - 1) / step;        // tries below `enough`; from the f-th on they have enough weight
+      while (most - below > 1) {
+        const uint32_t step = (most - below - 1) / 32 + 1, k = below + step * (lane + 1);
+        const unsigned int yes = __ballot_sync(0xffffffffu, k < most && k > below && wk(k) >= mp);
+        const uint32_t tried = (most - below - 1) / step;        // tries below `most`; from the f-th on they have enough weight
         const uint32_t f = yes ? __ffs(yes) - 1 : tried;
-        if (yes) enough = below + step * (f + 1);
+        if (yes) most = below + step * (f + 1);
         below += step * f;
       }
-      lim = max(lim, enough - 1);
+      lim = max(lim, most - 1);
+      if (lim == 0x7fffffffu) --lim;                               // -0's key, which no score has: as a number it is 0 itself
     }
     const double w_tie = cut.ties ? wt(cut_f) : 0.0;
-    const unsigned int ties_kept = cut.ties && (w_tie >= mp || cut.key == top_key) ? cut.ties : 0u;
+    const unsigned int ties_kept = cut.ties && (enough(w_tie) || cut.key == top_key) ? cut.ties : 0u;
     // sums of the warps' segments of [a, a + len): kept keys are queued so that every lane of the 64-bit arithmetic has one
     auto segments = [&](int a, int len, int seg) {
       double sum = 0.0;
@@ -563,7 +798,30 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
       constexpr int V = 16 / sizeof(T);
       const int head = min(b1 - b0, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x + b0) & 15)) & 15) / static_cast<int>(sizeof(T)));
       const int nv = b1 > b0 ? (b1 - b0 - head) / V : 0, tail = b0 + max(head, 0) + nv * V;
-      if (b1 > b0) {
+      if (tabled) {
+        if constexpr (sizeof(T) == 2) {
+          double more = 0.0;
+          auto add = [&](uint32_t k, double& to) {
+            to += weight16(k >= low16 ? k : 0);                    // (dropped ones all read one zero: no bank is asked twice)
+            ties += k == tie16 || k == tie16b;
+          };
+          auto add2 = [&](uint32_t two) {
+            const uint32_t k = patterns_of(two);
+            add(k & 0xffffu, sum);
+            add(k >> 16, more);
+          };
+          const unsigned short* xb = reinterpret_cast<const unsigned short*>(x);
+          if (lane < head) add(patterns_of(xb[b0 + lane]) & 0xffffu, sum);
+          const uint4* xv = reinterpret_cast<const uint4*>(x + b0 + head);
+#pragma unroll 2
+          for (int i = lane; i < nv; i += 32) {
+            const uint4 v = xv[i];
+            add2(v.x); add2(v.y); add2(v.z); add2(v.w);
+          }
+          if (tail + lane < b1) add(patterns_of(xb[tail + lane]) & 0xffffu, sum);
+          sum += more;
+        }
+      } else if (b1 > b0) {
         take(lane < head ? to_f<T>(x[b0 + lane]) : NAN);
         const uint4* xv = reinterpret_cast<const uint4*>(x + b0 + head);
         uint4 next = make_uint4(0, 0, 0, 0);
@@ -623,22 +881,28 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
     if (rank == owner) {
       target -= before;
       for (;;) {
-        // every thread walks the 16 sums alike
-        double run = 0.0, pick_run = 0.0;
-        unsigned int left = ties_left, pick_left = 0;
-        int pick = 0;
-        for (int i = 0; i < NWARP; ++i) {
-          const unsigned int t = min(s.wcnt[i], left);
-          const double m = s.wsum[i] + t * w_tie;
-          if (m > 0.0) {
-            pick = i; pick_run = run; pick_left = left;
-            if (run + m > target) break;
-          }
-          run += m;
-          left -= t;
+        // every warp walks the sums alike, one per lane
+        static_assert(NWARP <= 32, "one sum per lane");
+        unsigned int tied = lane < NWARP ? s.wcnt[lane] : 0;
+        const unsigned int own_ties = tied;
+#pragma unroll
+        for (int o = 1; o < NWARP; o <<= 1) {
+          const unsigned int y = __shfl_up_sync(0xffffffffu, tied, o);
+          if (lane >= o) tied += y;
         }
-        target -= pick_run;
-        ties_left = pick_left;
+        const unsigned int used_before = min(tied - own_ties, ties_left);
+        const double m = lane < NWARP ? s.wsum[lane] + (min(tied, ties_left) - used_before) * w_tie : 0.0;
+        double run = m;
+#pragma unroll
+        for (int o = 1; o < NWARP; o <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, run, o);
+          if (lane >= o) run += y;
+        }
+        const unsigned int over = __ballot_sync(0xffffffffu, m > 0.0 && run > target), any = __ballot_sync(0xffffffffu, m > 0.0);
+        const int pick = over ? __ffs(over) - 1 : 31 - __clz(any);
+        const double to_pick = __shfl_sync(0xffffffffu, run, max(pick - 1, 0));
+        if (pick > 0) target -= to_pick;
+        ties_left -= __shfl_sync(0xffffffffu, used_before, pick);
         len = min(seg, len - pick * seg);
         a += pick * seg;
         if (len <= 32) break;
@@ -649,7 +913,14 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
         const uint32_t k = lane < len ? key_of(to_f<T>(x[a + lane])) : 0u;
         const bool tie = lane < len && k == cut.key;
         const unsigned int tied = __ballot_sync(0xffffffffu, tie);
-        double w = lane < len && k > lim ? wk(k) : 0.0;
+        double w = 0.0;
+        if constexpr (sizeof(T) == 2) {
+          if (tabled && lane < len) {
+            const uint32_t k16 = patterns_of(reinterpret_cast<const unsigned short*>(x)[a + lane]) & 0xffffu;
+            if (k16 >= low16) w = weight16(k16);
+          }
+        }
+        if (!tabled && lane < len && k > lim) w = wk(k);
         if (tie && __popc(tied & ((1u << lane) - 1)) < static_cast<int>(min(ties_left, 32u))) w = w_tie;
         double run = w;
 #pragma unroll
@@ -676,16 +947,23 @@ int launch(SampleArgs p, int num_sms, cudaStream_t st) {
   // The most a row can have (of jagged rows: all but never, so assume twice the average).
   long long longest = p.width;
   if (p.offsets) longest = min(p.width, 2 * p.width / p.rows + 1024);
-  // CTAs per row: as many as run at once (one per SM: its 16 warps need 128 registers a thread to keep eight items' arithmetic in
-  // flight; two per SM at 64 took 226 instead of 205 us for 256 rows of 131071 bf16), while each keeps some thousand
-  // items.  More than that in turns, each with its own exchanges, cost more than reading a row again from L2 where it does
-  // not fit (256 rows of 131071 fp32: 593 us with eight CTAs a row, 281 us with one).
+  // 16-bit scores are counted by one CTA per row, however few rows there are: its fixed part (zeroing, listing and weighing the
+  // patterns) is 10 us, its two passes 20 us for 131071 items; by weight it took 17 against 14 us at 1500 items a row, 21 against
+  // 15 at 8192, 105 against 40 at 131071, and shared by four CTAs still 46.  Small k are left to the list (256 x 131071, k = 50: 81
+  // against 112 us), and the largest score needs no counts.
+  p.counted = sizeof(T) == 2 && longest > LIST && (p.temperature || p.temperature_v > 0.f) && (p.top_k || p.top_k_v <= 0 || p.top_k_v > LIST / 2);
+  // Otherwise CTAs per row: as many as run at once (one per SM: its 16 warps need 128 registers a thread to keep several items'
+  // arithmetic in flight), while each keeps some thousand items.  131071 fp32 items with one / two / four CTAs: 114 / 70 /
+  // 45 us; 8192: 19 / 20 / 23.  Clusters that do not all run at once cost more than they save: 36 rows by four took 86 us, since
+  // clusters of four leave an eighth of the SMs over; of eight, more (16 rows by eight 86 us, by four 44).
   int c = 1;
-  while (c < MAX_CLUSTER && 2LL * c * p.rows <= num_sms && longest / c > 4096) c *= 2;
+  auto fits = [&](int by) { return by * p.rows <= (by < 4 ? num_sms : by == 4 ? num_sms - num_sms / 8 : num_sms / 2); };
+  if (!p.counted) while (c < MAX_CLUSTER && fits(2 * c) && longest / c > (c < 4 ? 8192 : 65536)) c *= 2;
   const long long slice = (((longest + c - 1) / c + 31) / 32 * 32) * static_cast<long long>(sizeof(T));
-  const long long room = min(slice, static_cast<long long>(max_bytes - fixed_bytes));
+  const int count_bytes = p.counted ? COUNT_BYTES : 0;
+  const long long room = min(slice, static_cast<long long>(max_bytes - fixed_bytes - count_bytes));
   p.cap = static_cast<int>(room / sizeof(T));
-  const int bytes = fixed_bytes + static_cast<int>(room);
+  const int bytes = fixed_bytes + count_bytes + static_cast<int>(room);
   static std::atomic<unsigned long long> done{0};
   const int rc = rb_host::allow_smem(sample_kernel<T>, max_bytes, done);
   if (rc) return rc;

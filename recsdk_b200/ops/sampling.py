@@ -118,7 +118,8 @@ def sample_scores_ref(scores, uniform, offsets=None, temperature: Param = 1.0, t
             run = torch.cumsum(w, 0)
             n = 1 + int((run[:-1] < at(top_p, r) * run[-1]).sum())
             order, w = order[:n], w[:n]
-        keep = w >= at(min_p, r)
+        # (next to the largest score a weight rounds to 1, but is less)
+        keep = w >= at(min_p, r) if at(min_p, r) < 1.0 else x[order] == top
         keep[0] = True
         order, w = order[keep], w[keep]
         order, back = torch.sort(order)

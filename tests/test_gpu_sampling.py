@@ -154,3 +154,56 @@ def test_the_ranker_draws_from_its_scores():
     ids, lp = make().recommend(users, hist, cands, x, u, temperature=0.5, top_p=0.9)
     want, want_lp = S.sample_scores_ref(scores, u, torch.tensor([0, 20, 20, 320]), temperature=0.5, top_p=0.9)
     assert torch.equal(ids, want) and ids[1] == -1 and torch.allclose(lp[[0, 2]], want_lp[[0, 2]], rtol=1e-6)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("width", [1025, 5003, 65536, 131071])
+def test_patterns_of_16_bits(dtype, width):
+    """Rows whose values are few, all, or more often the same than 16 bits count; zeros of both signs, infinities, NaN."""
+    g = torch.Generator(device=DEV).manual_seed(width)
+    n = (12, width + 3)
+    x = (torch.randn(*n, generator=g, device=DEV) * 2.0).to(dtype)[:, 3:]     # 16-byte borders fall anywhere
+    x[1] = -1.5
+    x[2] = 0.0
+    x[2, ::2] = -0.0
+    x[3] = torch.where(torch.rand(width, generator=g, device=DEV) < 0.9, 0.0, -0.0).to(dtype)
+    x[3, 5] = 1e-3
+    x[4] = torch.randint(-32768, 32768, (width,), generator=g, device=DEV).to(torch.int16).view(dtype)        # every pattern
+    x[5] = torch.where(x[4].isfinite(), x[4], torch.zeros_like(x[4]))
+    x[6, ::3] = -math.inf
+    x[6, 1::3] = math.nan
+    x[7] = -math.inf
+    x[7, 1::2] = -math.nan
+    x[8] = x[0].abs() * -1e-4
+    x[9, width // 2] = math.inf
+    x[10] = -x[5].abs()
+    x[11] = -math.inf
+    x[11, width - 1] = -3.0
+    filters = FILTERS + [dict(top_k=513), dict(top_k=900, top_p=0.9), dict(top_k=width - 1, top_p=0.999), dict(top_p=0.9, min_p=0.002),
+                         dict(temperature=3e4), dict(temperature=3e4, top_p=0.9, min_p=0.3), dict(temperature=1e-3, top_p=0.99)]
+    for kw in filters:
+        _same(x, torch.rand(12, generator=g, device=DEV), **kw)
+    per_row = dict(top_k=torch.tensor([0, 1, 600, 0, 512, 513, 1024, 0, 5000, 0, 77, 0], dtype=torch.int32, device=DEV),
+                   temperature=torch.tensor([0.0, 1.0, 2.0, 0.5] * 3, device=DEV))
+    _same(x, torch.rand(12, generator=g, device=DEV), **per_row)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 9, 10, 33, 75])
+def test_few_long_rows(dtype, rows):
+    """One to eight CTAs a row."""
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    x = torch.randn(rows, 300007 if rows < 20 else 70001, generator=g, device=DEV).to(dtype)
+    for kw in (dict(), dict(top_p=0.9, min_p=0.002), dict(top_k=40), dict(top_k=5000, top_p=0.8), dict(temperature=0.0)):
+        _same(x, torch.rand(rows, generator=g, device=DEV), **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_min_p_keeps_down_to_zero(dtype):
+    """The lowest kept score is 0, whose neighbour below is -0."""
+    x = -torch.rand(4, 3001, device=DEV).to(dtype) - 0.5
+    x[:, 5::7] = 0.0
+    x[1, 5::14] = -0.0
+    x[2, 100] = 0.25
+    for kw in (dict(min_p=1.0), dict(min_p=0.7), dict(min_p=0.7, top_p=0.99), dict(min_p=0.65, top_k=2000)):
+        _same(x, torch.rand(4, device=DEV), **kw)
