@@ -18,6 +18,9 @@
 // anything else - and a CTA of eight otherwise, whose warps take turns at the tiles of an item and are joined in shared
 // memory.  Every warp feeds its own ring by TMA (128-byte swizzle, read with ldmatrix), the page rows of 32 boxes looked up
 // at a time.
+//
+// 128 single tokens of 32 heads over 8 key heads of 128, a window of 4096 and uneven histories: 1.9 GB in 320 us, nine tenths of a
+// copy's bandwidth.  Heads of 64 halve the bytes of a tile but not its instructions, and reach six tenths.
 #include "softmax_attention.cuh"
 
 namespace {
@@ -508,17 +511,19 @@ Space space_of(int n_cta, int D, long long rows, bool with_rows, bool with_tiles
 }
 
 // Which kernel a list of sequences takes, by the average number of rows that share a key head: the rows kernel reads
-// K and V once for 16 of them, the tiles kernel once for 256 with at least 128 computed.
-bool by_tiles(long long Tq, int G, int sequences, float scale) {
-  return G <= 128 && scale > 0.f && sequences > 0 && Tq * G >= 48LL * sequences;
+// K and V once for 16 of them, the tiles kernel once for 256 with at least 128 computed.  Heads of 128, 32 sequences of 4000
+// keys, 16 / 24 / 48 / 128 rows: by rows 96 / 177 / 234 / 626 us, by tiles 98 / 101 / 102 / 111; heads of 64, 200 sequences
+// of 1000 keys, 16 / 32 / 48 / 64 rows: by rows 118 / 116 / 153 / 230 us, by tiles 132 / 132 / 133 / 133.
+bool by_tiles(long long Tq, int G, int D, int sequences, float scale) {
+  return G <= 128 && scale > 0.f && sequences > 0 && Tq * G * D > 2048LL * sequences;
 }
 
 struct Plan { bool tiles_a, tiles_b; };
 
-Plan plan_of(long long Tq, int G, int B, int groups, float scale) {
-  const bool own = by_tiles(Tq, G, B, scale);
+Plan plan_of(long long Tq, int G, int D, int B, int groups, float scale) {
+  const bool own = by_tiles(Tq, G, D, B, scale);
   Plan r;
-  r.tiles_a = groups > 0 ? by_tiles(Tq, G, groups, scale) : own;
+  r.tiles_a = groups > 0 ? by_tiles(Tq, G, D, groups, scale) : own;
   r.tiles_b = groups > 0 && own;
   return r;
 }
@@ -558,8 +563,10 @@ int launch(const Batch& p, Outs w, const Plan& plan, const Space& sp, char* ws, 
       int rc = rb_host::make_map_2d(&tm, cache, p.total_rows, static_cast<long long>(p.Hkv) * D, static_cast<long long>(p.Hkv) * D, 64,
                                     q.box_rows, BF16);
       if (rc) return rc;
-      // a worker per warp where the items (at least one per sequence and key head) go round at least a quarter of them
-      const bool single = static_cast<long long>(q.a.B + q.b.B) * p.Hkv * 4 >= static_cast<long long>(n_cta) * NW;
+      // a worker per warp where there are more items (at least one per sequence and key head) than CTAs.  8000 keys each, heads of
+      // 64, 128 / 192 / 1184 items: by warps 63 / 85 / 390 us, by CTAs 52 / 95 / 564; 100 keys: 9.9 / 10.2 / 12.9 and 8.1 / 11.2 /
+      // 30.1; heads of 128, 8000 keys: 96 / 138 / 779 and 93 / 135 / 782.
+      const bool single = static_cast<long long>(q.a.B + q.b.B) * p.Hkv > n_cta;
       if (single) shares = n_cta * NW;
       rc = single ? launch_rows<D, BF16, 1>(tm, q, w, n_cta, after, st) : launch_rows<D, BF16, NW>(tm, q, w, n_cta, after, st);
       if (rc) return rc;
@@ -582,7 +589,7 @@ int launch(const Batch& p, Outs w, const Plan& plan, const Space& sp, char* ws, 
 // Bytes of workspace that rb_softmax_attn_paged needs.
 RB_API long long rb_softmax_attn_workspace(int num_sms, long long Tq, int H, int Hkv, int D, int B, int groups, float scale) {
   if (Hkv <= 0 || H % Hkv) return 0;
-  const Plan plan = plan_of(Tq, H / Hkv, B, groups, scale);
+  const Plan plan = plan_of(Tq, H / Hkv, D, B, groups, scale);
   return space_of(num_sms > 0 ? num_sms : 148, D, Tq * H, !plan.tiles_a || (groups > 0 && !plan.tiles_b), plan.tiles_a || plan.tiles_b,
                   groups > 0).total;
 }
@@ -614,7 +621,7 @@ RB_API int rb_softmax_attn_paged(const void* call) {
   const long long rows = c.num_pages * 2 * c.page_size;
   if (c.Tq * c.H > 0x7fffffffLL || rows + c.page_size > 0x7fffffffLL) return -4;
   const int n_cta = c.num_sms > 0 ? c.num_sms : 148;
-  const Plan plan = plan_of(c.Tq, c.H / c.Hkv, c.B, c.groups, c.scale);
+  const Plan plan = plan_of(c.Tq, c.H / c.Hkv, c.D, c.B, c.groups, c.scale);
   const Space sp = space_of(n_cta, c.D, c.Tq * c.H, !plan.tiles_a || (c.groups > 0 && !plan.tiles_b), plan.tiles_a || plan.tiles_b, c.groups > 0);
   if (c.workspace_bytes < sp.total) return -5;
   Batch p;

@@ -2,21 +2,26 @@
 // group of requests behind a common prefix), forward, on tcgen05 / TMEM (sm_100a).  The mathematics is that of
 // softmax_attention.cu: one pass over K and V with a running maximum and sum in fp32.
 //
-// Bound: the matrix rate and, equally, the exponentials: a 128 x 128 block costs 2 x 128 x 128 x D multiply-adds (1024
-// cycles of the tensor core for D = 128) and 16384 exponentials (1024 cycles of the special function units).  So two
-// blocks are always in flight, one in the tensor core while the other is in the softmax warps:
+// Bound: the matrix rate and, equally, the exponentials: 128 rows of a key tile of 64 cost 2 x 128 x 64 x D multiply-adds
+// (512 cycles of the tensor core for D = 128) and 8192 exponentials (512 cycles of the special function units).  So two row
+// tiles are always in flight, one in the tensor core while the other is in the softmax warps:
 //   * 256 rows (two row tiles of 128: 128 / G tokens x the G query heads that share a key head) walk the same key tiles, or
 //   * where a block has 128 rows or fewer, one row tile takes even key tiles with one set of warps and odd ones with
 //     the other; the two results are joined from TMEM at the end.
-// Roles: one warp issues TMA loads (Q once per block, then K and V tiles of 128 keys through a ring, box by box through the page
-// table), two warps issue tcgen05.mma, one for each row tile, and clear V of keys that nobody sees (0 x NaN), one thread
-// works the pieces of the share out ahead, eight warps do the softmax, a
-// thread per row: S from TMEM, maximum, exponentials, P back to TMEM over S as the A operand of O += P V.  O stays in TMEM
-// and is rescaled only when a row's maximum has grown by more than 2^8 since the value its weights refer to, which fp32
-// sums and 16-bit weights (a floating-point type: no precision lost) bear and which is rare after the first tiles.
+// Roles: warp 0 issues TMA loads (Q once per block, then a K and a V tile a slot through a ring, box by box through the page
+// table), warps 1 and 2 issue tcgen05.mma, one for each row tile, and clear V of keys that nobody sees (0 x NaN), warp 3
+// works the pieces of the share out ahead, eight warps do the softmax, a thread per row: S from TMEM, maximum, exponentials, P
+// back to TMEM over S as the A operand of O += P V.  A row tile's S is two key tiles ahead of its P (two buffers; with tiles of
+// 128 keys and one buffer the tensor core waited: 8192 tokens causal 1547 us, so 632).  O stays in TMEM and is rescaled only
+// when a row's maximum has grown by more than 2^8 since the value its weights refer to, which fp32 sums and 16-bit
+// weights (a floating-point type: no precision lost) bear and which is rare after the first tiles.
 //
 // The CTAs are persistent, one per SM, and share the work as in softmax_attention.cu: equal, contiguous pieces of all
-// (block, key head) items laid end to end, in units of two 128 x 128 blocks.
+// (block, key head) items laid end to end, in units of a key tile (of two where a block has one row tile).
+//
+// 16384 tokens causal, 32 heads over 8 of 128: 1.8 ms, 1.23 PFLOP/s, three quarters of a large matrix product's rate; 8192: 0.49
+// ms.  What is left: S of 64 keys is held up by shared memory (58 cycles a product instead of 32), and the two row tiles fall into
+// step; a block costs 4 us to finish and begin, which short histories (1000 keys, 17 tiles) feel as a third of their time.
 #include "softmax_attention.cuh"
 
 namespace {
@@ -133,6 +138,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+// one lane of a converged warp, which the compiler takes as issuing for it (a test of the lane's number made a loop of it)
 __device__ __forceinline__ bool elect() {
   uint32_t ok;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
@@ -280,11 +286,9 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const uint32_t tmem = *tmem_slot;                                           // S / P of row tile w at w * 128, O at 256 + w * 128
   bool gave_up = false;
   int n_piece = 0;
-  // A warp waits and arrives as one: lane 0 does it.  (Every thread's own arrival and polling on the same word is served
-  // one after another: with 128 of each per step that was most of a step's time.)
+  // A warp gives up as one, and arrives as one by lane 0 (arrivals on one word are served one after another).
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    int ok = 0;
-    ok = !gave_up && spin_wait(bar, parity, abort_flag, p.status);
+    const int ok = !gave_up && spin_wait(bar, parity, abort_flag, p.status);
     if (!__all_sync(0xffffffffu, ok)) gave_up = true;
     return !gave_up;
   };
