@@ -35,7 +35,7 @@ def sample_scores(scores: torch.Tensor, uniform: torch.Tensor, offsets: Optional
     after another ``[T]``.  ``uniform [B]`` fp32: numbers in ``[0, 1)``.  In the order (score descending, index ascending)
     the filters keep the first ``top_k`` items (0: all); of those, up to and with the one at which the running sum of
     ``exp(score / temperature)`` reaches ``top_p`` of their sum; of those, the ones with at least ``min_p`` times the
-    largest weight.  The item drawn is the first one, in index order, whose running sum over the kept items exceeds
+    largest weight.  (``min_p = 1``: the largest scores only.)  The item drawn is the first one, in index order, whose running sum over the kept items exceeds
     ``uniform`` times their sum.  ``temperature = 0`` takes the largest score (the first of equals).  Every parameter is a
     number or a ``[B]`` tensor on the scores' device; in a tensor ``top_k <= 0`` and ``top_p >= 1`` are off and
     ``temperature <= 0`` takes the largest score.
