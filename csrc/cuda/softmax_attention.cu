@@ -408,19 +408,28 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
   if (tid == 0) wait_before();                                                 // what ran before is done when this kernel is
 }
 
-// Joins the pieces of the items that borders cut: blocks (c, y) look after the item whose first border is share c's begin,
+// One kernel's cut items, `split` blocks for each share; a call has those of the rows kernel, of the tiles kernel or of both.
+struct Join { Batch p; Outs w; int shares, split, block_rows; };
+struct Joins { Join of[2]; };
+
+// Joins the pieces of the items that borders cut: a share's blocks look after the item whose first border is its begin,
 // 16 rows at a time and four columns per thread.  Items have up to `block_rows` rows.  (Few blocks: most of them find nothing to
 // do, and it is their number that this kernel's time goes by.)
 template <int D, bool BF16>
-__global__ void __launch_bounds__(RT * D / 4) attn_join_kernel(const Batch p, const Outs w, int block_rows) {
+__global__ void __launch_bounds__(RT * D / 4) attn_join_kernel(const __grid_constant__ Joins j) {
   launch_dependents();
   wait_before();
-  const Meta m = w.meta[blockIdx.x];
+  const bool second = static_cast<int>(blockIdx.x) >= j.of[0].shares * j.of[0].split;
+  const Join& of = j.of[second];
+  const int b = blockIdx.x - (second ? j.of[0].shares * j.of[0].split : 0), block_rows = of.block_rows;
+  const Batch& p = of.p;
+  const Outs& w = of.w;
+  const Meta m = w.meta[b / of.split];
   if (!m.valid) return;
   constexpr int STEP = 8;                                                      // pieces in flight
   const int col = threadIdx.x % (D / 4) * 4;
   const Seq s = seq_of(p, m.seq);
-  for (int r = blockIdx.y * RT + threadIdx.x / (D / 4); r < m.rows; r += gridDim.y * RT) {
+  for (int r = b % of.split * RT + threadIdx.x / (D / 4); r < m.rows; r += of.split * RT) {
     auto place = [&](int c) { return static_cast<long long>(c == m.c0 ? m.first : 2 * c) * block_rows + r; };
     float mm = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
     for (int c = m.c0; c <= m.c1; c += STEP) {
@@ -528,11 +537,6 @@ Plan plan_of(long long Tq, int G, int D, int B, int groups, float scale) {
   return r;
 }
 
-template <int D, bool BF16>
-int join(const Batch& p, const Outs& w, int shares, int block_rows, cudaStream_t st) {
-  return launch_kernel(true, attn_join_kernel<D, BF16>, dim3(shares, block_rows > RT ? 8 : 1), dim3(RT * D / 4), 0, st, p, w, block_rows);
-}
-
 template <int D, bool BF16, int W>
 int launch_rows(const CUtensorMap& tm, const Batch& p, const Outs& w, int n_cta, bool after, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
@@ -545,6 +549,7 @@ template <int D, bool BF16>
 int launch(const Batch& p, Outs w, const Plan& plan, const Space& sp, char* ws, const void* cache, int n_cta, cudaStream_t st) {
   const bool parts = p.b.B > 0;
   bool after = false;
+  Joins joins = {};
   for (int tiles = 0; tiles < 2; ++tiles) {
     Batch q = p;
     if (plan.tiles_a != (tiles != 0)) q.a.B = 0;
@@ -571,10 +576,14 @@ int launch(const Batch& p, Outs w, const Plan& plan, const Space& sp, char* ws, 
       rc = single ? launch_rows<D, BF16, 1>(tm, q, w, n_cta, after, st) : launch_rows<D, BF16, NW>(tm, q, w, n_cta, after, st);
       if (rc) return rc;
     }
-    const int rc = join<D, BF16>(q, w, shares, tiles ? TILE_ROWS : RT, st);
-    if (rc) return rc;
+    joins.of[after] = {q, w, shares, tiles ? 8 : 1, tiles ? TILE_ROWS : RT};
+    if (!after) joins.of[1].split = 1;
     after = true;
   }
+  if (!after) return 0;
+  const int rc = launch_kernel(true, attn_join_kernel<D, BF16>, dim3(joins.of[0].shares * joins.of[0].split + joins.of[1].shares * joins.of[1].split),
+                               dim3(RT * D / 4), 0, st, joins);
+  if (rc) return rc;
   if (parts) {
     const long long rows = static_cast<long long>(p.Tq) * p.H;
     const int per = 256 / (D / 4);
