@@ -9,7 +9,7 @@
 // Bound: memory.  A unit of work is 16 elements of a head (two 16-byte loads whose elements turn with each other, so no
 // exchange between threads), and one thread takes the same unit of up to four heads of a token: the eight loads are in
 // flight together and the unit's cosines and sines (64 bytes of the fp32 table) are read once for them.
-// 20011 tokens, 32 + 2 x 8 heads of 128: 0.5 GB in 89 us, 85 % of a copy's bandwidth; a single token: 3.6 us in a graph, the launch.
+// 20011 tokens, 32 + 2 x 8 heads of 128: 0.5 GB in 89 to 94 us, 81 to 85 % of a copy's bandwidth; a single token: 3.6 us in a graph, the launch.
 #include "common.cuh"
 
 namespace {

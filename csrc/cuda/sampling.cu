@@ -626,18 +626,24 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
         static_assert(PB == 4, "a thread's bins are one vector");
         unsigned long long v[PB] = {0, 0, 0, 0}, mine = 0;
         const int at = upwards ? tid : BINS / PB - 1 - tid;
-        auto add4 = [&](const uint4& l, const uint4& h) {
-          const uint32_t ls[4] = {l.x, l.y, l.z, l.w}, hs[4] = {h.x, h.y, h.z, h.w};
+        auto add4 = [&](const uint4& l, int shift) {
+          const uint32_t ls[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] += (static_cast<unsigned long long>(hs[i]) << 32) + ls[i];
+          for (int i = 0; i < 4; ++i) v[i] += static_cast<unsigned long long>(ls[i]) << shift;
         };
-        for (int r = 0; r < c; r += 2) {                           // two peers' loads in flight
-          const Shared& a = peer(r);
-          const Shared& b = peer(min(r + 1, c - 1));
-          const uint4 la = reinterpret_cast<const uint4*>(a.lo)[at], ha = reinterpret_cast<const uint4*>(a.hi)[at];
-          const uint4 lb = reinterpret_cast<const uint4*>(b.lo)[at], hb = reinterpret_cast<const uint4*>(b.hi)[at];
-          add4(la, ha);
-          if (r + 1 < c) add4(lb, hb);
+        for (int r = 0; r < c; r += 4) {                           // four peers' loads in flight; counts have no high words
+          uint4 l[4], h[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            l[i] = h[i] = make_uint4(0, 0, 0, 0);
+            if (r + i < c) {
+              const Shared& a = peer(r + i);
+              l[i] = reinterpret_cast<const uint4*>(a.lo)[at];
+              if (by_mass) h[i] = reinterpret_cast<const uint4*>(a.hi)[at];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { add4(l[i], 0); add4(h[i], 32); }
         }
         if (!upwards) {
           unsigned long long y = v[0]; v[0] = v[3]; v[3] = y;
@@ -1057,25 +1063,32 @@ int launch(SampleArgs p, int num_sms, cudaStream_t st) {
 
 }  // namespace
 
+// The arguments of rb_sample_scores, 8-byte fields first (packed by the caller).
 // scores: fp32 / fp16 / bf16 (dtype 0 / 1 / 2), dense rows of `width` elements `ld` apart, or - with offsets (int32 or int64
 // device array [rows + 1]) - jagged in a vector of `width` elements.  uniform [rows] in [0, 1).  Per-row parameters, where
 // given, replace the scalar ones: temperature <= 0 takes the largest score, top_k <= 0 and top_p >= 1 are off, min_p is
 // relative to the largest weight.  ids [rows] int64 (index within the row, -1: nothing to draw), logprobs [rows]: log of
 // the drawn item's share of the kept weights.
-RB_API int rb_sample_scores(const void* scores, long long ld, const void* offsets, int offsets64, long long width, int rows,
-                            const float* uniform, const float* temperature, const int* top_k, const float* top_p,
-                            const float* min_p, float temperature_v, int top_k_v, float top_p_v, float min_p_v, long long* ids,
-                            float* logprobs, int dtype, int num_sms, cudaStream_t st) {
-  if (rows == 0) return 0;
-  if (width > 0x7fffffffLL - 64) return -1;
+struct SampleCall {
+  const void* scores; long long ld; const void* offsets; long long width;
+  const float *uniform, *temperature; const int* top_k; const float *top_p, *min_p;
+  long long* ids; float* logprobs; cudaStream_t stream;
+  int offsets64, rows, top_k_v, dtype, num_sms;
+  float temperature_v, top_p_v, min_p_v;
+};
+
+RB_API int rb_sample_scores(const void* call) {
+  const SampleCall& c = *static_cast<const SampleCall*>(call);
+  if (c.rows == 0) return 0;
+  if (c.width > 0x7fffffffLL - 64) return -1;
   SampleArgs p;
-  p.scores = scores; p.ld = ld; p.offsets = offsets; p.offsets64 = offsets64; p.width = width; p.rows = rows; p.cap = 0;
-  p.uniform = uniform; p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
-  p.temperature_v = temperature_v; p.top_k_v = top_k_v; p.top_p_v = top_p_v; p.min_p_v = min_p_v;
-  p.ids = ids; p.logprobs = logprobs;
-  const int sms = num_sms > 0 ? num_sms : 148;
-  if (dtype == 0) return launch<float>(p, sms, st);
-  if (dtype == 1) return launch<__half>(p, sms, st);
-  if (dtype == 2) return launch<__nv_bfloat16>(p, sms, st);
+  p.scores = c.scores; p.ld = c.ld; p.offsets = c.offsets; p.offsets64 = c.offsets64; p.width = c.width; p.rows = c.rows; p.cap = 0;
+  p.uniform = c.uniform; p.temperature = c.temperature; p.top_k = c.top_k; p.top_p = c.top_p; p.min_p = c.min_p;
+  p.temperature_v = c.temperature_v; p.top_k_v = c.top_k_v; p.top_p_v = c.top_p_v; p.min_p_v = c.min_p_v;
+  p.ids = c.ids; p.logprobs = c.logprobs;
+  const int sms = c.num_sms > 0 ? c.num_sms : 148;
+  if (c.dtype == 0) return launch<float>(p, sms, c.stream);
+  if (c.dtype == 1) return launch<__half>(p, sms, c.stream);
+  if (c.dtype == 2) return launch<__nv_bfloat16>(p, sms, c.stream);
   return -2;
 }

@@ -4,6 +4,7 @@ uniform numbers.  Rows are dense ``[B, V]`` or jagged (the scores of every user'
 from __future__ import annotations
 
 import math
+import struct
 from typing import Optional, Tuple, Union
 
 import torch
@@ -12,15 +13,21 @@ from . import _lib
 
 Param = Union[float, int, torch.Tensor]
 
+_SAMPLE_CALL = struct.Struct("@12q5i3f")                # SampleCall of sampling.cu
+_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_BIG = torch.finfo(torch.float32).max
 
-def _param(name: str, value: Param, rows: int, dtype: torch.dtype, device, lo: float, hi: float, open_lo: bool = False):
+
+def _param(name: str, value: Param, rows: int, dtype: torch.dtype, like: torch.Tensor, lo: float, hi: float, open_lo: bool = False):
     """-> (per-row tensor or None, scalar).  Scalars are checked; what tensors hold is taken as it is."""
     if isinstance(value, torch.Tensor):
-        if value.shape != (rows,) or value.device != device:
+        if value.shape != (rows,) or value.device != like.device:
             raise ValueError("%s must be a scalar or a [%d] tensor on %s, got %s on %s"
-                             % (name, rows, device, tuple(value.shape), value.device))
+                             % (name, rows, like.device, tuple(value.shape), value.device))
         if dtype is torch.int32 and value.dtype not in (torch.int32, torch.int64):
             raise ValueError("%s must hold integers, got %s" % (name, value.dtype))
+        if value.dtype is torch.int64 and dtype is torch.int32:
+            value = value.clamp(-1, (1 << 31) - 1)
         return value.to(dtype).contiguous(), 0
     if not (value >= lo and value <= hi) or (open_lo and value == lo):
         raise ValueError("%s = %r is outside %s%g, %g]" % (name, value, "(" if open_lo else "[", lo, hi))
@@ -35,10 +42,10 @@ def sample_scores(scores: torch.Tensor, uniform: torch.Tensor, offsets: Optional
     after another ``[T]``.  ``uniform [B]`` fp32: numbers in ``[0, 1)``.  In the order (score descending, index ascending)
     the filters keep the first ``top_k`` items (0: all); of those, up to and with the one at which the running sum of
     ``exp(score / temperature)`` reaches ``top_p`` of their sum; of those, the ones with at least ``min_p`` times the
-    largest weight.  (``min_p = 1``: the largest scores only.)  The item drawn is the first one, in index order, whose running sum over the kept items exceeds
-    ``uniform`` times their sum.  ``temperature = 0`` takes the largest score (the first of equals).  Every parameter is a
-    number or a ``[B]`` tensor on the scores' device; in a tensor ``top_k <= 0`` and ``top_p >= 1`` are off and
-    ``temperature <= 0`` takes the largest score.
+    largest weight (``min_p = 1``: the largest scores only).  The item drawn is the first one, in index order, whose running
+    sum over the kept items exceeds ``uniform`` times their sum.  ``temperature = 0`` takes the largest score (the first
+    of equals).  Every parameter is a number or a ``[B]`` tensor on the scores' device; in a tensor ``top_k <= 0`` and
+    ``top_p >= 1`` are off and ``temperature <= 0`` takes the largest score.
 
     ``ids`` count within the row; ``logprobs`` is the log of the drawn item's share of what was kept (0 for
     ``temperature = 0``) - the propensity to log.  NaN and ``-inf`` are never drawn; a row with nothing else, or with
@@ -51,41 +58,43 @@ def sample_scores(scores: torch.Tensor, uniform: torch.Tensor, offsets: Optional
         if scores.dim() != 1 or offsets.dim() != 1 or offsets.numel() < 1:
             raise ValueError("jagged scores must be [T] with offsets [B + 1]; got %s and %s"
                              % (tuple(scores.shape), tuple(offsets.shape)))
-        if offsets.dtype not in (torch.int32, torch.int64) or offsets.device != scores.device:
+        if offsets.dtype not in (torch.int32, torch.int64) or offsets.get_device() != scores.get_device():
             raise ValueError("offsets must be int32 or int64 on the scores' device")
         rows, width = offsets.numel() - 1, scores.shape[0]
-    dev = scores.device
-    if uniform.shape != (rows,) or uniform.dtype != torch.float32 or uniform.device != dev:
-        raise ValueError("uniform must be [%d] fp32 on %s" % (rows, dev))
-    if scores.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    index = scores.get_device()                                         # (-1: CPU)
+    if uniform.shape != (rows,) or uniform.dtype is not torch.float32 or uniform.get_device() != index:
+        raise ValueError("uniform must be [%d] fp32 on %s" % (rows, scores.device))
+    code = _CODES.get(scores.dtype)
+    if code is None:
         raise ValueError("scores must be fp32, fp16 or bf16, got %s" % (scores.dtype,))
+    if scores.requires_grad and torch.is_grad_enabled():
+        raise ValueError("scores require a gradient, which this operator does not have (use torch.no_grad())")
     if width > (1 << 31) - 65:
         raise ValueError("2^31 - 64 and more scores in a row (or in all jagged rows) are not supported")
-    big = torch.finfo(torch.float32).max
-    t_t, t_v = _param("temperature", temperature, rows, torch.float32, dev, 0.0, big)
-    k_t, k_v = _param("top_k", top_k, rows, torch.int32, dev, 0, (1 << 31) - 1)
-    p_t, p_v = _param("top_p", top_p, rows, torch.float32, dev, 0.0, 1.0, open_lo=True)
-    m_t, m_v = _param("min_p", min_p, rows, torch.float32, dev, 0.0, 1.0)
+    t_t, t_v = _param("temperature", temperature, rows, torch.float32, scores, 0.0, _BIG)
+    k_t, k_v = _param("top_k", top_k, rows, torch.int32, scores, 0, (1 << 31) - 1)
+    p_t, p_v = _param("top_p", top_p, rows, torch.float32, scores, 0.0, 1.0, open_lo=True)
+    m_t, m_v = _param("min_p", min_p, rows, torch.float32, scores, 0.0, 1.0)
     if not scores.is_cuda:
         return sample_scores_ref(scores, uniform, offsets, temperature, top_k, top_p, min_p)
-    index = scores.get_device()
     if not _lib.is_current(index):
         with torch.cuda.device(index):
             return sample_scores(scores, uniform, offsets, temperature, top_k, top_p, min_p)
     if width > 1 and scores.stride(-1) != 1:
         scores = scores.contiguous()
     uniform = uniform.contiguous()
-    off_ptr, off_64 = None, False
-    if offsets is not None:
+    ld = off_ptr = off_64 = 0
+    if offsets is None:
+        ld = scores.stride(0)
+    else:
         offsets = offsets.contiguous()
         off_ptr, off_64 = offsets.data_ptr(), offsets.dtype is torch.int64
-    ids = torch.empty(rows, dtype=torch.int64, device=dev)
-    logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
+    ids, logprobs = uniform.new_empty(rows, dtype=torch.int64), torch.empty_like(uniform)
     lib, sms, _ = _lib.launch_env(index)
-    rc = lib.rb_sample_scores(scores.data_ptr(), scores.stride(0) if offsets is None else 0, off_ptr, off_64, width, rows,
-                              uniform.data_ptr(), _lib.ptr(t_t), _lib.ptr(k_t), _lib.ptr(p_t), _lib.ptr(m_t), float(t_v), int(k_v),
-                              float(p_v), float(m_v), ids.data_ptr(), logprobs.data_ptr(), _lib.dtype_code(scores.dtype), sms,
-                              _lib.raw_stream(index))
+    rc = lib.rb_sample_scores(_SAMPLE_CALL.pack(
+        scores.data_ptr(), ld, off_ptr, width, uniform.data_ptr(), 0 if t_t is None else t_t.data_ptr(), 0 if k_t is None else k_t.data_ptr(),
+        0 if p_t is None else p_t.data_ptr(), 0 if m_t is None else m_t.data_ptr(), ids.data_ptr(), logprobs.data_ptr(),
+        _lib.raw_stream(index), off_64, rows, int(k_v), code, sms, t_v, p_v, m_v))
     _lib.check(rc, "rb_sample_scores")
     return ids, logprobs
 

@@ -207,3 +207,20 @@ def test_min_p_keeps_down_to_zero(dtype):
     x[2, 100] = 0.25
     for kw in (dict(min_p=1.0), dict(min_p=0.7), dict(min_p=0.7, top_p=0.99), dict(min_p=0.65, top_k=2000)):
         _same(x, torch.rand(4, device=DEV), **kw)
+
+
+def test_more_long_rows_than_blocks():
+    """Rows of patterns that a CTA works through one after another."""
+    g = torch.Generator(device=DEV).manual_seed(11)
+    x = torch.randn(66001, 1100, generator=g, device=DEV).bfloat16()
+    u = torch.rand(66001, generator=g, device=DEV)
+    pick = torch.tensor([0, 1, 464, 465, 65535, 65536, 66000])
+    for kw in (dict(top_p=0.9), dict(top_k=600, top_p=0.9, min_p=0.01)):
+        ids, _ = S.sample_scores(x, u, **kw)
+        assert torch.equal(ids[pick], S.sample_scores_ref(x[pick], u[pick], **kw)[0])
+
+
+def test_counts_past_32_bits():
+    x = torch.randn(4, 2000, device=DEV)
+    k = torch.tensor([1 << 40, (1 << 32) + 1, -(1 << 32) + 3, 2], device=DEV)
+    _same(x, torch.rand(4, device=DEV), top_k=k, temperature=2.0)

@@ -183,3 +183,17 @@ def test_slots_are_where_keys_go():
     assert torch.equal(cache[ids[0].long(), 1, 15], v[0])
     with pytest.raises(ValueError):
         SA.append_kv_rotary(q, k, v, cache, z, pos, ids, ptr, 16, table, slots=torch.tensor([15]))
+
+
+def test_sampling_refuses_what_wants_a_gradient():
+    x, u = torch.randn(3, 5, requires_grad=True), torch.rand(3)
+    with pytest.raises(ValueError, match="gradient"):
+        S.sample_scores(x, u)
+    with torch.no_grad():
+        S.sample_scores(x, u)
+
+
+def test_min_p_of_one_keeps_the_largest_only():
+    x = torch.tensor([[0.0, -1e-30, 0.0, -1e-17, -1.0]])
+    ids = {int(S.sample_scores(x, torch.tensor([v]), min_p=1.0)[0]) for v in (0.0, 0.3, 0.49, 0.51, 0.7, 0.99)}
+    assert ids == {0, 2}
