@@ -40,7 +40,7 @@ template <int D> struct Cfg {
   static constexpr int CH = D / 64;
   static constexpr int TILE = KT * D * 2, Q_TILE = MT * D * 2;  // bytes of a K or V tile, of a Q tile
   static constexpr int STAGES = D == 64 ? 8 : 5;                // a K and a V tile each
-  static constexpr int TAIL = 3072;               // shared memory is full to the last byte for D = 128
+  static constexpr int TAIL = 3 * 1024;              // shared memory is full to the last byte for D = 128
   static constexpr int SMEM = 2 * Q_TILE + STAGES * 2 * TILE + TAIL;
 };
 
