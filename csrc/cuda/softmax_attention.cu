@@ -5,7 +5,9 @@
 // over the keys that the row sees: up to its own position, of those the last `window` and the first `sinks`.  One pass
 // over K and V with a running maximum and sum; both are kept in fp32, as is o.  w is rounded to the inputs' type for the
 // product with V (the sum takes it unrounded): a rounding of at most half a step per weight, which averages out over the
-// keys to about the rounding of the result itself.
+// keys to about the rounding of the result itself.  fp16 has no exponents below 2^-14 and nothing below 2^-24, and keys whose
+// weights are smaller than that can be many enough to matter, so w is held 2^15 times as large there (`WeightTop`): off by half a step
+// down to 2^-29 of the largest weight and by 2^-40 of it below.
 //
 // Bound: the bytes of K and V.  The G query heads that share a key head are the rows of one 16-row mma.sync tile (a
 // 128-row tcgen05 tile would be mostly padding here and the matrix rate does not matter), so K and V are read once for all
@@ -229,7 +231,7 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
         float o[D / 8][4];
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+        float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};               // mx: the maximum less WeightTop
         for (int v = begin(ih); v < end(ih) && !dead; v += W) {
           const bool ok = rb::mbar_wait(&bar[st_out], par, abort_flag, p.status);
           if (!__all_sync(0xffffffffu, ok)) { dead = true; break; }
@@ -254,7 +256,7 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
               mma16816<BF16>(sc[2 * i + 1], qf[kk], b2, b3);
             }
           }
-          float mn[2] = {mx[0], mx[1]};
+          float mn[2] = {-INFINITY, -INFINITY};
           uint32_t seen[2] = {~0u, ~0u};                                       // bit j: the row sees key j0 + (lane & 3) * 2 + j
           if (!full) {
 #pragma unroll
@@ -275,6 +277,7 @@ __global__ void __launch_bounds__(NW * 32, 1) attn_rows_kernel(const __grid_cons
           for (int e = 0; e < 2; ++e) {
             mn[e] = fmaxf(mn[e], __shfl_xor_sync(0xffffffffu, mn[e], 1));
             mn[e] = fmaxf(mn[e], __shfl_xor_sync(0xffffffffu, mn[e], 2));
+            mn[e] = fmaxf(mx[e], __fsub_ru(mn[e], WeightTop<BF16>));              // (up: x - mn is never above WeightTop)
             base_m[e] = mn[e] == -INFINITY ? 0.f : mn[e];
             corr[e] = exp2_approx(mx[e] - base_m[e]);
             mx[e] = mn[e];

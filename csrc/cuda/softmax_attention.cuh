@@ -112,6 +112,10 @@ __device__ __forceinline__ int box_row(const Batch& p, const Seq& s, const Span&
   return p.total_rows;
 }
 
+// log2 of the largest weight that is handed to the product with V, which takes weights in the inputs' type: bf16 has fp32's
+// exponents and may have it anywhere, fp16's range ends just above 2^15.
+template <bool BF16> constexpr float WeightTop = BF16 ? 0.f : 15.f;
+
 template <bool BF16> __device__ __forceinline__ uint32_t pack16(float a, float b) { return BF16 ? rb::pack_bf16(a, b) : rb::pack_f16(a, b); }
 
 __device__ __forceinline__ float exp2_approx(float x) {

@@ -13,8 +13,9 @@
 // works the pieces of the share out ahead, eight warps do the softmax, a thread per row: S from TMEM, maximum, exponentials, P
 // back to TMEM over S as the A operand of O += P V.  A row tile's S is two key tiles ahead of its P (two buffers; with tiles of
 // 128 keys and one buffer the tensor core waited: 8192 tokens causal 1547 us, so 632).  O stays in TMEM and is rescaled only
-// when a row's maximum has grown by more than 2^8 since the value its weights refer to, which fp32 sums and 16-bit
-// weights (a floating-point type: no precision lost) bear and which is rare after the first tiles.
+// when a row's maximum has grown by more than GROWTH octaves since the value its weights refer to, which is rare after the first
+// tiles.  bf16 weights bear that like fp32 sums; fp16 weights begin at 2^(15 - GROWTH), so that the largest of its range is
+// never passed and the small ones lose nothing above 2^-(29 - GROWTH) of the largest.
 //
 // The CTAs are persistent, one per SM, and share the work as in softmax_attention.cu: equal, contiguous pieces of all
 // (block, key head) items laid end to end, in units of a key tile (of two where a block has one row tile).
@@ -34,6 +35,7 @@ constexpr int MT = 128;                 // rows per row tile
 // us a unit): without them the shares with many short items would run half as long again as the others.
 constexpr int FIXED = 4;
 constexpr int THREADS = 384;            // 4 service warps, 2 x 4 softmax warps
+template <bool BF16> constexpr float GROWTH = BF16 ? 8.f : 4.f;
 constexpr uint32_t WAIT = 1u << 24;     // tries of a wait: some tenths of a second
 
 template <int D> struct Cfg {
@@ -598,11 +600,13 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             for (int e = 1; e < 15; e += 2) mx[c] = fmaxf(mx[c], fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
           }
           const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;   // scale > 0 in this kernel
-          // O and the sum refer to m_ref; only a row that outgrows it by 2^8 (or its first weight) moves it
-          const bool grow = m_new > m_ref + 8.f || (m_ref == -INFINITY && m_new > -INFINITY);
+          // O and the sum refer to m_ref; only a row whose weights would pass 2^TOP (or its first weight) moves it
+          constexpr float START = BF16 ? 0.f : WeightTop<BF16> - GROWTH<BF16>, TOP = START + GROWTH<BF16>;
+          const bool grow = m_new > __fadd_rd(m_ref, TOP) || (m_ref == -INFINITY && m_new > -INFINITY);
           if (__any_sync(0xffffffffu, grow)) {
-            const float f = grow ? (m_ref == -INFINITY ? 0.f : exp2_approx(m_ref - m_new)) : 1.f;
-            if (grow) m_ref = m_new;
+            const float m_next = __fsub_ru(m_new, START);
+            const float f = grow ? (m_ref == -INFINITY ? 0.f : exp2_approx(m_ref - m_next)) : 1.f;
+            if (grow) m_ref = m_next;
             sum *= f;
             if (any) {
               // once the product with the tile before is done, O is at rest until this tile's P is there
