@@ -20,6 +20,7 @@ enum RbStatus : int {
   RB_ERR_PEER_TIMEOUT = 2,   // a peer flag wait ran out of iterations
   RB_ERR_BOUNDS = 3,         // an index was outside its table
   RB_ERR_CAPACITY = 4,       // a fixed-size buffer was too small
+  RB_ERR_RANGE = 5,          // a number was too large to be computed with
 };
 
 namespace rb {

@@ -36,6 +36,10 @@ constexpr int MT = 128;                 // rows per row tile
 constexpr int FIXED = 4;
 constexpr int THREADS = 384;            // 4 service warps, 2 x 4 softmax warps
 template <bool BF16> constexpr float GROWTH = BF16 ? 8.f : 4.f;
+// A row whose largest score (log2) is beyond this, on either side of 0, is reported: fp32 has no digit behind the point left there, and
+// further out the fused operation that makes the exponents, whose product is not rounded as the maximum's was, loses the largest
+// weight itself.  (Out to any size: the difference first, then its product, in a loop of its own: 2 to 3 % of a prompt's time.)
+constexpr float FAR = 8388608.f;        // 2^23
 constexpr uint32_t WAIT = 1u << 24;     // tries of a wait: some tenths of a second
 
 template <int D> struct Cfg {
@@ -697,6 +701,7 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           lse = lse2 * LN2;
         }
         if (live && c_lo == 0 && dst_lse) *dst_lse = lse;
+        if (live && fabsf(m_ref) >= FAR && fabsf(m_ref) < INFINITY && p.status) atomicCAS(p.status, 0, RB_ERR_RANGE);
 #pragma unroll 1
         for (int c = c_lo; c < c_hi; c += 32) {
           uint32_t a[32];

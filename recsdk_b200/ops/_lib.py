@@ -174,7 +174,7 @@ def num_sms(device: Optional[torch.device] = None) -> int:
 _status: Dict[int, torch.Tensor] = {}
 
 STATUS_NAMES = {0: "ok", 1: "mbarrier wait timed out", 2: "peer flag wait timed out",
-                3: "index out of bounds", 4: "fixed-size buffer overflow"}
+                3: "index out of bounds", 4: "fixed-size buffer overflow", 5: "number too large to be computed with"}
 
 
 class KernelStatusError(RuntimeError):

@@ -295,7 +295,9 @@ def softmax_attention_paged(q: torch.Tensor, kv_cache: torch.Tensor, q_offsets: 
     query that sees no key gives 0 and ``-inf``; rows of ``q`` behind the last request are undefined in the result.  bf16 or
     fp16, head_dim 64 or 128, page_size a multiple of 16.  Stale values in slots that a block of queries does not see do no
     harm; a non-finite VALUE that one query sees can spread to neighbouring queries of the same request that do not.  A
-    missing page reads as zeros and is reported by ``_lib.check_status``."""
+    missing page reads as zeros and is reported by ``_lib.check_status``; so is, where requests
+    have many queries, one whose largest score (``scale`` times the product) lies beyond 5 * 10^6 on either side of 0: its result is
+    undefined."""
     return _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks, return_lse)
 
 

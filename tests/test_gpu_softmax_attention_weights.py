@@ -90,3 +90,36 @@ def test_behind_a_shared_prefix(new):
         tol = 2 * 2.0 ** -11 * own + 40000 * 2.0 ** -36 * 1.6 + 48 * 2.0 ** -16 * own
         assert ((got.double() - own).abs() <= tol).all()
     _lib.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new", [1, 140])
+def test_very_large_scores(dtype, new):
+    """One key stands out by more than any weight can show, at sizes where fp32 has no digits behind the point: the result is that
+    key's value, to within the rounding of its weight and of the result (half a step each); or the score is reported."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    D, page = 64, 16
+    cache = torch.randn(25, 2, page, 2, D, generator=g, device=DEV)
+    cache[:, 0] *= 0.01
+    cache[3, 0, 5] = 30000.0
+    cache = cache.to(dtype)
+    q = torch.full((new, 4, D), 3000.0, device=DEV).to(dtype)
+    want = cache[3, 1, 5].repeat_interleave(2, 0).double()
+    for scale in (1e-4, 1e-3, 1.9e-3, 1.0, 30.0):                   # scores of 5.76e9 times that
+        got = SA.softmax_attention_paged(q, cache, _off([new]), _off([400]), torch.arange(25, device=DEV), _off([25]), page, scale=scale)
+        if new > 1 and scale > 1e-3:
+            with pytest.raises(_lib.KernelStatusError, match="too large"):
+                _lib.check_status()
+            continue
+        _lib.check_status()
+        assert ((got.double() - want).abs() <= 1.01 * torch.finfo(dtype).eps * want.abs()).all()
+    if new > 1:                                                       # nothing but scores far below 0
+        low = cache.clone()
+        low[:, 0] = -30000.0
+        SA.softmax_attention_paged(q, low, _off([new]), _off([400]), torch.arange(25, device=DEV), _off([25]), page, scale=1.0)
+        with pytest.raises(_lib.KernelStatusError, match="too large"):
+            _lib.check_status()
+    q[0, 1, 3] = math.inf                                             # infinities are not sizes
+    got = SA.softmax_attention_paged(q, cache, _off([new]), _off([400]), torch.arange(25, device=DEV), _off([25]), page, scale=1e-3)
+    assert torch.isnan(got[0, 1]).all() and torch.isfinite(got[:, 2:]).all()
+    _lib.check_status()
