@@ -41,7 +41,7 @@ def rotary_table(max_positions: int, rotary_dim: int, base: float = 10000.0, dev
 
 # ----------------------------------------------------------------------------- checks
 def _rows(name: str, x: torch.Tensor, heads: Optional[int], dim: int, like: torch.Tensor) -> torch.Tensor:
-    """[T, heads, dim] with adjacent heads and 16-byte aligned rows (others are copied)."""
+    """[T, heads, dim] with adjacent heads and 16-byte aligned rows (others are copied; a single row has no stride to mind)."""
     shape = x.shape
     if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
         raise ValueError("%s must be [tokens, %s, %d], got %s" % (name, "heads" if heads is None else heads, dim, tuple(shape)))
@@ -51,6 +51,9 @@ def _rows(name: str, x: torch.Tensor, heads: Optional[int], dim: int, like: torc
         raise ValueError("%s requires a gradient, which this operator does not have (use torch.no_grad())" % name)
     if x.is_cuda:
         st = x.stride()
+        if shape[0] == 1 and st[0] != shape[1] * dim:
+            x = x.as_strided(shape, (shape[1] * dim,) + st[1:])
+            st = x.stride()
         if (st[2] != 1 or st[1] != dim or st[0] & 7 or st[0] < 0 or x.data_ptr() & 15) and x.numel():
             x = x.contiguous()
             if x.data_ptr() & 15:
@@ -135,7 +138,8 @@ def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != cache.device or (out.numel() and (
-            out.stride(2) != 1 or out.stride(1) != D or out.stride(0) % 8 or out.stride(0) < H * D or out.data_ptr() % 16)):
+            out.stride(2) != 1 or (H > 1 and out.stride(1) != D) or (n > 1 and (out.stride(0) % 8 or out.stride(0) < H * D))
+            or out.data_ptr() % 16)):
         raise ValueError("out must be %s %s on %s with adjacent heads and 16-byte aligned rows" % (tuple(q.shape), q.dtype, cache.device))
     if n == 0:
         return out
@@ -155,7 +159,7 @@ def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache
                                     num_tokens, out, slots)
     lib, sms, status = _lib.launch_env(index)
     rc = lib.rb_kv_append_rotary(_APPEND_CALL.pack(
-        q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0),
+        q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0) if n > 1 else H * D,
         cache.data_ptr(), pages, batch_indices.data_ptr(), positions.data_ptr(), 0 if slots is None else slots.data_ptr(),
         page_ids.data_ptr(), page_indptr.data_ptr(), 0 if num_tokens is None else num_tokens.data_ptr(), table.data_ptr(), status, _lib.raw_stream(index), n, H, Hkv, D,
         page_indptr.shape[0] - 1, page_size, page_ids.shape[0], table.shape[0], table.shape[1], interleaved, q.dtype is torch.bfloat16, sms))
