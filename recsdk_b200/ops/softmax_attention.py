@@ -231,6 +231,8 @@ def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size,
     index = cache.get_device()
     q = _rows("q", q, None, D, cache)
     T, H, _ = q.shape
+    if q.is_cuda and T > 1 and (q.stride(0) < H * D or q.stride(0) % D):
+        q = q.contiguous()                                              # a tensor map's strides are whole multiples, and do not overlap
     if H == 0 or H % Hkv:
         raise ValueError("%d query heads cannot share %d key heads" % (H, Hkv))
     B = q_offsets.numel() - 1

@@ -34,3 +34,31 @@ def test_a_single_token_has_no_stride(dist):
     want = SA.append_kv_rotary(q.clone(), k.clone(), v.clone(), c2, zero, zero + 33, ids, ptr, 16, table)
     assert got is out and torch.equal(got, want) and torch.equal(c1, c2) and not torch.equal(c1, cache)
     _lib.check_status()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("page", [48, 128])
+@pytest.mark.parametrize("new,keys", [([1, 1, 1], [70, 300, 9]), ([150, 1, 300], [150, 700, 333])])
+def test_slices_of_many_tokens(new, keys, page, D):
+    """A projection's slice, rows with padding behind them, every other token, one token for all, heads that are not adjacent."""
+    g = torch.Generator(device=DEV).manual_seed(page + D)
+    H, Hkv, T = 4, 2, sum(new)
+    cache, ids, ptr = _cache(keys, page, Hkv, D, g)
+    kw = dict(q_offsets=_off(new), k_offsets=_off(keys), page_ids=ids, page_indptr=ptr, page_size=page, window=200, num_sinks=3)
+    base = torch.randn(2 * T, (H + 2 * Hkv) * D + 8, generator=g, device=DEV).bfloat16()
+    slices = [base[:T, : (H + 2 * Hkv) * D].contiguous()[:, 2 * D:(2 + H) * D].unflatten(1, (H, D)),      # stride 8 D, a head's offset
+              base[:T, : H * D].unflatten(1, (H, D)), base[::2, : H * D].unflatten(1, (H, D)),            # odd multiples of 16 bytes
+              base[:1, : H * D].unflatten(1, (H, D)).expand(T, H, D),
+              base.flatten()[: (T + H) * D].as_strided((T, H, D), (D, D, 1)),                             # tokens overlap
+              base[:T, : 2 * H * D].unflatten(1, (H, 2 * D))[..., :D], base[:T, 1:1 + H * D].unflatten(1, (H, D))]
+    for q in slices:
+        want, want_lse = SA.softmax_attention_paged(q.clone(memory_format=torch.contiguous_format), cache, return_lse=True, **kw)
+        got, lse = SA.softmax_attention_paged(q, cache, return_lse=True, **kw)
+        assert torch.equal(got, want) and torch.equal(lse, want_lse)
+        ref, _ = SA.softmax_attention_ref(q, cache, kw["q_offsets"], kw["k_offsets"], ids, ptr, page, window=200, num_sinks=3, dtype=torch.float64)
+        mag = cache.clone()
+        mag[:, 1] = mag[:, 1].abs()
+        avg, _ = SA.softmax_attention_ref(q, mag, kw["q_offsets"], kw["k_offsets"], ids, ptr, page, window=200, num_sinks=3, dtype=torch.float64)
+        # half a step of the weights and of the result, 2^-12 for scores that are fp32 sums of sum |q_i k_i| * scale <= 8 in 128 terms
+        assert ((got.double() - ref).abs() <= 2.0 ** -8 * (avg + ref.abs()) + 2.0 ** -12 * avg).all()
+    _lib.check_status()
