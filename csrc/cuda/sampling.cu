@@ -185,7 +185,8 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
     const float temp = p.temperature ? p.temperature[row] : p.temperature_v;
     const int top_k = p.top_k ? p.top_k[row] : p.top_k_v;
     const float top_p = p.top_p ? p.top_p[row] : p.top_p_v;
-    const float min_p = p.min_p ? p.min_p[row] : p.min_p_v;
+    const float min_pv = p.min_p ? p.min_p[row] : p.min_p_v;
+    const float min_p = min_pv == min_pv ? min_pv : 1.f;           // NaN: no weight is known to be enough but the largest
     const float uf = p.uniform[row];
     const double u = uf > 0.f ? static_cast<double>(uf) : 0.0;
 

@@ -45,7 +45,8 @@ def sample_scores(scores: torch.Tensor, uniform: torch.Tensor, offsets: Optional
     largest weight (``min_p = 1``: the largest scores only).  The item drawn is the first one, in index order, whose running
     sum over the kept items exceeds ``uniform`` times their sum.  ``temperature = 0`` takes the largest score (the first
     of equals).  Every parameter is a number or a ``[B]`` tensor on the scores' device; in a tensor ``top_k <= 0`` and
-    ``top_p >= 1`` are off and ``temperature <= 0`` takes the largest score.
+    ``top_p >= 1`` are off and ``temperature <= 0`` takes the largest score (NaN: ``top_p`` is off, ``temperature`` takes the
+    largest score, ``min_p`` keeps the largest scores only).
 
     ``ids`` count within the row; ``logprobs`` is the log of the drawn item's share of what was kept (0 for
     ``temperature = 0``) - the propensity to log.  NaN and ``-inf`` are never drawn; a row with nothing else, or with
