@@ -15,8 +15,9 @@
 // Weights are computed and summed in 64 bits: with N kept items each of the N borders can go either way with the sums'
 // relative error as its chance, and 32-bit exponentials (1e-7 each) would draw a neighbour in every hundredth row of 10^5
 // items.  The exponential is table-driven (Tang, ACM TOMS 15, 1989): 2^(n/256) from a table, 2^(f/256), |f| <= 1/2, as a
-// polynomial of degree 3 (relative error (ln2/512)^4 / 24 = 1.4e-13).  Sums inside the histograms are whole numbers (2^-44 of
-// the largest weight for rows up to 2^18 items, coarser beyond), so atomics in any order give the same bits.
+// polynomial of degree 3 (relative error (ln2/512)^4 / 24 = 1.4e-13).  Sums inside the histograms are whole numbers, so atomics in
+// any order give the same bits: units of 2^-44 of the largest weight for rows up to 2^18 items, of about 2^-61 of the row's sum of weights
+// beyond, which takes a rough look at that sum first.
 //
 // A row is read from memory once, into the shared memory of a cluster of CTAs (1 to 8 by its size and by how many rows there
 // are), which then exchange histograms and sums through distributed shared memory; rows that do not fit are read again from
@@ -111,12 +112,24 @@ struct Weigher {
     const double w = __hiloint2double(__double2hiint(q) + (((n >> 8) + up) << 20), __double2loint(q));
     return t > -700.0 ? w : 0.0;                                   // (2^-1010; also for -inf)
   }
-  // the weight in units of 2^-shift, rounded (up <= 44)
+  // the weight in units of 2^-up, rounded (up <= 61)
   __device__ __forceinline__ unsigned long long fixed(float x, int up) const {
+    if (up > 51) return __double2ull_rn((*this)(x, up));
     const double w = (*this)(x, up) + 4503599627370496.0;          // + 2^52
     return static_cast<unsigned long long>(__double_as_longlong(w)) & 0xfffffffffffffULL;
   }
 };
+
+// In which units a row's weights are summed: 64 bits hold the sum.  Rows of up to SHORT items fit whatever their weights are; the
+// sum of a longer one may be far below its number of items, and many weights that are nothing in units made for the latter can
+// matter together.
+constexpr int SHORT = 1 << 18;
+__device__ __forceinline__ float rough_weight(float x, float top, float temp) {
+  return x == top ? 1.f : x > -INFINITY ? exp2f((x - top) * (1.44269504f / temp)) : 0.f;
+}
+__device__ __forceinline__ int shift_for(double rough_sum) {      // (an upper bound of it, as a power of two)
+  return 62 - max(1, (__double2hiint(rough_sum * 1.01) >> 20) - 1022);
+}
 
 // Where the order is cut: everything above `key` is kept and the first `ties` items (in index order) that equal it.
 struct Cut { uint32_t key; unsigned int ties; };
@@ -215,6 +228,20 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
       if (keep) x = y;
     };
 
+    int shift_fx = 62 - 18;
+    // of the CTA, the same bits for all
+    auto sum_of_all = [&](double v) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      __syncthreads();
+      if (lane == 0) s.wsum[warp] = v;
+      __syncthreads();
+      v = 0.0;
+      for (int i = 0; i < NWARP; ++i) v += s.wsum[i];
+      __syncthreads();
+      return v;
+    };
+
     // ---- 16-bit scores: how often each pattern occurs is all that the cuts need
     uint32_t top_key = 0, top16 = 0, cut16 = 0;
     Cut cut = {KEY_NONE, 0};
@@ -291,7 +318,6 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
           Weigher wt;
           wt.table = s.table; wt.top = top_f;
           wt.rate = 1.0 / static_cast<double>(temp);
-          const int shift_fx = 62 - max(18, 32 - __clz(n_row));
           // list the groups, two per thread (and always -0's, for its weight)
           static_assert(GROUPS == 2 * NT, "two groups per thread");
           {
@@ -311,6 +337,16 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
           }
           for (int by_mass = 0; by_mass < 2; ++by_mass) {
             if (by_mass ? !(top_p < 1.f) : !(top_k > 0 && top_k < n_row)) continue;
+            if (by_mass && n_row > SHORT) {
+              double rough = 0.0;
+              for (int i = tid; i < groups * (GROUP / 2); i += NT) {
+                const int at = group[i / (GROUP / 2)] * (GROUP / 2) + i % (GROUP / 2);
+                const unsigned int w = counts[at];
+                if (w & 0xffffu) rough += static_cast<double>(w & 0xffffu) * rough_weight(pattern_value<T>(2 * at), top_f, temp);
+                if (w >> 16) rough += static_cast<double>(w >> 16) * rough_weight(pattern_value<T>(2 * at + 1), top_f, temp);
+              }
+              shift_fx = shift_for(sum_of_all(rough));
+            }
             auto value = [&](uint32_t k, unsigned int m) -> unsigned long long {
               if (k <= cut16) m = k == cut16 ? cut.ties : 0;
               return m * (by_mass ? wt.fixed(pattern_value<T>(k), shift_fx) : 1ULL);
@@ -435,7 +471,6 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
     const float bin_scale = 64.f * 1.44269504f / temp, bin_shift = top_f * bin_scale;
     auto place_of = [&](float x) { return fmaxf(fminf(fmaf(x, -bin_scale, bin_shift), BINS - 1.f), 0.f); };
     auto bin_of = [&](float x) { return static_cast<int>(place_of(x)); };
-    const int shift_fx = 62 - max(18, 32 - __clz(n_row));
     const double mp = static_cast<double>(min_p);
     auto enough = [&](double w) { return w >= mp && mp < 1.0; };   // next to the largest score the weight rounds to 1, but is less
 
@@ -693,6 +728,18 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
       };
       // items equal to an earlier cut count as many times as they are kept: one thread adds them
       const bool lump = by_mass && cut.ties && rank == 0 && tid == 0;
+      if (by_mass && n_row > SHORT) {
+        double rough = 0.0;
+        for_each<T>(x, n, [&](auto& v, int) {
+          for (float e : v) rough += rough_weight(e, top_f, temp);
+        });
+        rough = sum_of_all(rough);
+        if (tid == 0) s.sum = rough;
+        sync();
+        rough = 0.0;
+        for (int r = 0; r < c; ++r) rough += peer(r).sum;
+        shift_fx = shift_for(rough);
+      }
       sync();                                                      // earlier histograms have been read
       clear();
       if (by_mass) {

@@ -50,7 +50,12 @@ def sample_scores(scores: torch.Tensor, uniform: torch.Tensor, offsets: Optional
 
     ``ids`` count within the row; ``logprobs`` is the log of the drawn item's share of what was kept (0 for
     ``temperature = 0``) - the propensity to log.  NaN and ``-inf`` are never drawn; a row with nothing else, or with
-    nothing at all, gives ``-1`` and ``-inf``.  Sums are in 64 bits and the result does not depend on the launch."""
+    nothing at all, gives ``-1`` and ``-inf``.
+
+    Weights carry 1.4e-13 of themselves; what ``top_p`` compares is summed in units of 2^-44 of the largest weight (rows of up to
+    2^18 items, longer ones 2^-61 of their sum), the draw's sums in 64 bits.  A border that close to ``top_p`` or ``uniform`` can
+    fall on either side, and on another one where the row's alignment or the number of rows has its parts summed in another
+    order; the same call always gives the same."""
     if offsets is None:
         if scores.dim() != 2:
             raise ValueError("scores must be [B, V], or [T] with offsets; got %s" % (tuple(scores.shape),))
