@@ -906,7 +906,7 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
       double sum = 0.0;
       unsigned int ties = 0, queued = 0;
       float* q = s.queue[warp];
-      const int b0 = a + warp * seg, b1 = min(b0 + seg, a + len);
+      const int at = min(warp * seg, len), b0 = a + at, b1 = b0 + min(seg, len - at);   // (16 segments can pass 2^31)
       const float lim_f = value_of(lim);
       auto take = [&](float e) {                                   // NaN for lanes without an item
         ties += e == cut_f;

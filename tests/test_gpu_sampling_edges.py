@@ -99,3 +99,34 @@ def test_weights_past_the_short_rows_units(dtype):
     x[0, 5] = math.inf
     x[1, 7::5] = math.nan
     _same(x, torch.rand(2, generator=g, device=DEV), top_p=0.9)
+
+
+def test_a_row_of_almost_two_to_the_31():
+    """As long as a row may be, among many empty ones (one CTA a row): its last item is the only one that can be drawn."""
+    n = (1 << 31) - 65
+    x = torch.full((n,), -math.inf, device=DEV)
+    x[n - 1] = -2.0
+    off = torch.zeros(101, dtype=torch.int64, device=DEV)
+    off[43:] = n
+    u = torch.full((100,), 0.5, device=DEV)
+    for kw in (dict(), dict(top_p=0.9)):
+        ids, lp = S.sample_scores(x, u, off, **kw)
+        assert int(ids[42]) == n - 1 and float(lp[42]) == 0.0
+        ids[42] = -1
+        assert (ids == -1).all()
+    del x
+    torch.cuda.empty_cache()
+    with pytest.raises(ValueError, match="2\\^31"):
+        S.sample_scores(torch.empty(1, device=DEV).expand(1, (1 << 31) - 64), u[:1])
+
+
+@pytest.mark.parametrize("lens", [[1, 700, 0, 300000], [1024, 1025, 33, 0, 1, 200001], [1000, 3, 90000]])
+def test_short_rows_shared_by_several_ctas(lens):
+    """Jagged rows that one CTA could sort, in clusters that the longest row is given."""
+    g = torch.Generator(device=DEV).manual_seed(sum(lens))
+    x = torch.randn(sum(lens), generator=g, device=DEV)
+    o = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=torch.int32, device=DEV)
+    for kw in (dict(), dict(top_k=1), dict(top_k=7), dict(top_k=10 ** 6), dict(top_p=0.3), dict(top_p=0.95), dict(min_p=0.05), dict(min_p=1.0),
+               dict(temperature=0.0), dict(temperature=0.3, top_k=50, top_p=0.9), dict(temperature=2.5, top_k=300, top_p=0.5, min_p=0.01)):
+        for _ in range(3):
+            _same(x, torch.rand(len(lens), generator=g, device=DEV), o, **kw)
