@@ -76,8 +76,8 @@ __global__ void __launch_bounds__(256) kv_append_rotary_kernel(const RotaryArgs 
       const uint16_t* src = h < p.H ? p.q + i * p.ld_q + h * p.D
                             : h < p.H + p.Hkv ? p.k + i * p.ld_k + (h - p.H) * p.D
                                               : p.v + i * p.ld_v + (h - p.H - p.Hkv) * p.D;
-      a[t] = __ldg(reinterpret_cast<const uint4*>(src) + va);
-      b[t] = __ldg(reinterpret_cast<const uint4*>(src) + vb);
+      a[t] = reinterpret_cast<const uint4*>(src)[va];                        // (no __ldg: q_out may be q)
+      b[t] = reinterpret_cast<const uint4*>(src)[vb];
     }
     const int pos = p.positions[i], at_token = p.slots ? p.slots[i] : pos, bi = p.batch_idx[i];
     bool ok = pos >= 0 && pos < p.table_rows && at_token >= 0 && bi >= 0 && bi < p.B;

@@ -62,3 +62,21 @@ def test_slices_of_many_tokens(new, keys, page, D):
         # half a step of the weights and of the result, 2^-12 for scores that are fp32 sums of sum |q_i k_i| * scale <= 8 in 128 terms
         assert ((got.double() - ref).abs() <= 2.0 ** -8 * (avg + ref.abs()) + 2.0 ** -12 * avg).all()
     _lib.check_status()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("T,H,Hkv,D,R", [(1, 4, 2, 64, 64), (3001, 32, 8, 128, 64), (777, 5, 1, 64, 16)])
+def test_queries_turned_in_place(T, H, Hkv, D, R, interleaved):
+    """The result goes where the queries are, a slice of the projection that keys and values are slices of, too."""
+    g = torch.Generator(device=DEV).manual_seed(T)
+    cache, ids, ptr = _cache([T], 16, Hkv, D, g)
+    qkv = torch.randn(T, (H + 2 * Hkv) * D, generator=g, device=DEV).bfloat16()
+    q, k, v = (x.unflatten(1, (-1, D)) for x in qkv.split([H * D, Hkv * D, Hkv * D], dim=1))
+    rest = qkv[:, H * D:].clone()
+    zero, pos = torch.zeros(T, dtype=torch.int32, device=DEV), torch.arange(T, dtype=torch.int32, device=DEV)
+    table = SA.rotary_table(T, R, device=DEV)
+    c1, c2 = cache.clone(), cache.clone()
+    want = SA.append_kv_rotary(q, k, v, c1, zero, pos, ids, ptr, 16, table, interleaved=interleaved)
+    got = SA.append_kv_rotary(q, k, v, c2, zero, pos, ids, ptr, 16, table, interleaved=interleaved, out=q)
+    assert got is q and torch.equal(q, want) and torch.equal(c1, c2) and torch.equal(qkv[:, H * D:], rest)
+    _lib.check_status()
