@@ -21,7 +21,7 @@ import torch
 from ..inference.kvcache_manager import HostKVTaskStatus, KVCacheManager, KVIndexMeta
 from ..ops import gemm, hstu_ops
 from ..ops.hstu_attention import hstu_attention_paged, hstu_attention_ref
-from ..ops.sampling import sample_scores
+from ..ops.sampling import check_parameters, sample_scores
 from .hstu import HSTU
 
 
@@ -103,7 +103,9 @@ class HSTURanker:
                   min_p=0.0) -> Tuple[torch.Tensor, torch.Tensor]:
         """:meth:`rank`, then one of every user's candidates drawn from their scores
         (:func:`~recsdk_b200.ops.sampling.sample_scores` with the given ``uniform [B]``): its index among the user's
-        candidates (-1: none) and the log of its probability, the propensity of off-policy training."""
+        candidates (-1: none) and the log of its probability, the propensity of off-policy training.  What is wrong with the
+        parameters is refused before the cache is touched."""
+        check_parameters(num_candidates.numel(), x_new.device, uniform, temperature, top_k, top_p, min_p)
         scores = self.rank(user_ids, history_lengths, num_candidates, x_new, timestamps)
         offsets = torch.zeros(num_candidates.numel() + 1, dtype=torch.int64)
         torch.cumsum(num_candidates, 0, out=offsets[1:])

@@ -18,12 +18,12 @@ _CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _BIG = torch.finfo(torch.float32).max
 
 
-def _param(name: str, value: Param, rows: int, dtype: torch.dtype, like: torch.Tensor, lo: float, hi: float, open_lo: bool = False):
+def _param(name: str, value: Param, rows: int, dtype: torch.dtype, device: torch.device, lo: float, hi: float, open_lo: bool = False):
     """-> (per-row tensor or None, scalar).  Scalars are checked; what tensors hold is taken as it is."""
     if isinstance(value, torch.Tensor):
-        if value.shape != (rows,) or value.device != like.device:
+        if value.shape != (rows,) or value.device != device:
             raise ValueError("%s must be a scalar or a [%d] tensor on %s, got %s on %s"
-                             % (name, rows, like.device, tuple(value.shape), value.device))
+                             % (name, rows, device, tuple(value.shape), value.device))
         if dtype is torch.int32 and value.dtype not in (torch.int32, torch.int64):
             raise ValueError("%s must hold integers, got %s" % (name, value.dtype))
         if value.dtype is torch.int64 and dtype is torch.int32:
@@ -32,6 +32,18 @@ def _param(name: str, value: Param, rows: int, dtype: torch.dtype, like: torch.T
     if not (value >= lo and value <= hi) or (open_lo and value == lo):
         raise ValueError("%s = %r is outside %s%g, %g]" % (name, value, "(" if open_lo else "[", lo, hi))
     return None, value
+
+
+def check_parameters(rows: int, device: torch.device, uniform: torch.Tensor, temperature: Param = 1.0, top_k: Param = 0,
+                     top_p: Param = 1.0, min_p: Param = 0.0):
+    """Refuses what :func:`sample_scores` refuses of its parameters for ``rows`` rows on ``device``, for callers that have work to
+    do before they have scores.  -> (per-row tensor or None, scalar) of temperature, top_k, top_p, min_p."""
+    if uniform.shape != (rows,) or uniform.dtype is not torch.float32 or uniform.device != device:
+        raise ValueError("uniform must be [%d] fp32 on %s" % (rows, device))
+    return (_param("temperature", temperature, rows, torch.float32, device, 0.0, _BIG),
+            _param("top_k", top_k, rows, torch.int32, device, 0, (1 << 31) - 1),
+            _param("top_p", top_p, rows, torch.float32, device, 0.0, 1.0, open_lo=True),
+            _param("min_p", min_p, rows, torch.float32, device, 0.0, 1.0))
 
 
 def sample_scores(scores: torch.Tensor, uniform: torch.Tensor, offsets: Optional[torch.Tensor] = None, temperature: Param = 1.0,
@@ -68,8 +80,6 @@ def sample_scores(scores: torch.Tensor, uniform: torch.Tensor, offsets: Optional
             raise ValueError("offsets must be int32 or int64 on the scores' device")
         rows, width = offsets.numel() - 1, scores.shape[0]
     index = scores.get_device()                                         # (-1: CPU)
-    if uniform.shape != (rows,) or uniform.dtype is not torch.float32 or uniform.get_device() != index:
-        raise ValueError("uniform must be [%d] fp32 on %s" % (rows, scores.device))
     code = _CODES.get(scores.dtype)
     if code is None:
         raise ValueError("scores must be fp32, fp16 or bf16, got %s" % (scores.dtype,))
@@ -77,10 +87,7 @@ def sample_scores(scores: torch.Tensor, uniform: torch.Tensor, offsets: Optional
         raise ValueError("scores require a gradient, which this operator does not have (use torch.no_grad())")
     if width > (1 << 31) - 65:
         raise ValueError("2^31 - 64 and more scores in a row (or in all jagged rows) are not supported")
-    t_t, t_v = _param("temperature", temperature, rows, torch.float32, scores, 0.0, _BIG)
-    k_t, k_v = _param("top_k", top_k, rows, torch.int32, scores, 0, (1 << 31) - 1)
-    p_t, p_v = _param("top_p", top_p, rows, torch.float32, scores, 0.0, 1.0, open_lo=True)
-    m_t, m_v = _param("min_p", min_p, rows, torch.float32, scores, 0.0, 1.0)
+    (t_t, t_v), (k_t, k_v), (p_t, p_v), (m_t, m_v) = check_parameters(rows, scores.device, uniform, temperature, top_k, top_p, min_p)
     if not scores.is_cuda:
         return sample_scores_ref(scores, uniform, offsets, temperature, top_k, top_p, min_p)
     if not _lib.is_current(index):
