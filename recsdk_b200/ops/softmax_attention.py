@@ -96,6 +96,18 @@ def _rotate_ref(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, interleav
     return y.to(x.dtype)
 
 
+def _pages_of(b, to, page_ids, page_indptr, page_size: int, pages: int) -> torch.Tensor:
+    """The page of every token (place ``to`` of request ``b``), -1 where it does not exist."""
+    known = (b >= 0) & (b < page_indptr.shape[0] - 1) & (to >= 0)
+    b = torch.where(known, b, 0)
+    if page_indptr.shape[0] < 2 or page_ids.shape[0] == 0:
+        return torch.full_like(to, -1)
+    at = page_indptr[b] + to // page_size
+    known = known & (at >= 0) & (at < page_indptr[b + 1]) & (at < page_ids.shape[0])
+    page = page_ids[torch.where(known, at, 0)]
+    return torch.where(known & (page >= 0) & (page < pages), page, -1)
+
+
 def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor, batch_indices: torch.Tensor,
                      positions: torch.Tensor, page_ids: torch.Tensor, page_indptr: torch.Tensor, page_size: int,
                      table: torch.Tensor, interleaved: bool = False, num_tokens: Optional[torch.Tensor] = None,
@@ -113,7 +125,7 @@ def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache
     ``num_tokens``: optional device int32 ``[1]`` (``new_history_nnz_npu``): only that many tokens are there, the rows
     behind them are neither appended nor written to the result - for static buffers under a captured graph.  ``out``: where the
     queries go (may be ``q``).  A token whose position or page does not exist is left out and reported by
-    ``_lib.check_status``."""
+    ``_lib.check_status``; on CPU tensors it is refused, before anything is written."""
     cache = _cache(kv_cache, page_size)
     pages, _, _, Hkv, D = cache.shape
     index = cache.get_device()
@@ -144,11 +156,13 @@ def append_kv_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache
     if n == 0:
         return out
     if not cache.is_cuda:
-        m = n if num_tokens is None else min(n, int(num_tokens))
+        m = n if num_tokens is None else max(0, min(n, int(num_tokens)))
         pos, b = positions[:m].long(), batch_indices[:m].long()
-        cos, sin = table[pos][:, None, :].chunk(2, dim=-1)
         to = pos if slots is None else slots[:m].long()
-        at = page_ids.long()[page_indptr.long()[b] + to // page_size]
+        at = _pages_of(b, to, page_ids.long(), page_indptr.long(), page_size, pages)
+        if ((pos < 0) | (pos >= table.shape[0]) | (at < 0)).any():
+            raise IndexError("a token's position is not in the table, or its page does not exist")
+        cos, sin = table[pos][:, None, :].chunk(2, dim=-1)
         out[:m] = _rotate_ref(q[:m], cos, sin, interleaved)
         cache[at, 0, to % page_size] = _rotate_ref(k[:m], cos, sin, interleaved)
         cache[at, 1, to % page_size] = v[:m]

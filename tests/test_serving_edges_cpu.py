@@ -4,6 +4,7 @@ import torch
 
 from recsdk_b200.inference import KVCacheConfig, KVCacheManager
 from recsdk_b200.ops import sampling as S
+from recsdk_b200.ops import softmax_attention as SA
 
 
 def test_recommend_refuses_before_the_cache_is_touched():
@@ -34,3 +35,28 @@ def test_parameters_are_checked_without_scores():
                   ((3, u.device, u), dict(top_k=torch.rand(3)))):
         with pytest.raises(ValueError):
             S.check_parameters(*a, **kw)
+
+
+def test_append_refuses_what_does_not_exist():
+    """Two requests of two pages each; a token past its request's pages must not land in the neighbour's."""
+    g = torch.Generator().manual_seed(1)
+    cache = torch.randn(5, 2, 16, 2, 64, generator=g)
+    ids, ptr, table = torch.tensor([3, 0, 4, 1]), torch.tensor([0, 2, 4]), SA.rotary_table(64, 64)
+    q, k, v = torch.randn(2, 4, 64, generator=g), torch.randn(2, 2, 64, generator=g), torch.randn(2, 2, 64, generator=g)
+    add = lambda b, pos, ids=ids, **kw: SA.append_kv_rotary(q, k, v, cache, torch.tensor(b), torch.tensor(pos), ids, ptr, 16, table, **kw)  # noqa: E731
+    before = cache.clone()
+    for args, kw in ((([0, 0], [0, 32]), {}), (([1, 0], [31, 32]), {}), (([0, 1], [0, 64]), {}), (([0, 1], [-1, 0]), {}), (([0, 2], [0, 0]), {}),
+                     (([0, -1], [0, 0]), {}), (([0, 0], [0, 16], torch.tensor([3, -1, 4, 1])), {}), (([0, 1], [0, 16], torch.tensor([3, 0, 4, 5])), {}),
+                     (([0, 1], [0, 16], torch.tensor([3, 0, 4])), {}), (([0, 0], [0, 1]), dict(slots=torch.tensor([0, 40]))),
+                     (([0, 0], [0, 1]), dict(slots=torch.tensor([0, -1])))):
+        with pytest.raises(IndexError):
+            add(*args, **kw)
+        assert torch.equal(cache, before)
+    # padding is not looked at
+    out = torch.full_like(q, 7.0)
+    add([0, 9], [3, 999], num_tokens=torch.tensor([1], dtype=torch.int32), out=out)
+    assert (out[1] == 7.0).all() and torch.equal(cache[3, 1, 3], v[0])
+    cache.copy_(before)
+    for n in (0, -1):
+        add([0, 0], [0, 1], num_tokens=torch.tensor([n], dtype=torch.int32), out=out)
+        assert torch.equal(cache, before)
