@@ -198,7 +198,8 @@ def _attention_ref(q, keys, values, sees, scale: float):
 def softmax_attention_ref(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size: int, scale: Optional[float] = None,
                           window: int = 0, num_sinks: int = 0, prefix_offsets=None, prefix_page_ids=None, prefix_page_indptr=None,
                           group_offsets=None, dtype: torch.dtype = torch.float32):
-    """``(o [T, H, D] in dtype, lse [T, H])`` of the two attention operators, request by request in ``dtype``."""
+    """``(o [T, H, D] in dtype, lse [T, H])`` of the two attention operators, request by request in ``dtype``.  A page of keys
+    that some query sees has to be there; the others' may be gone."""
     H, D = q.shape[1], q.shape[2]
     scale = 1.0 / math.sqrt(D) if scale is None else scale
     qo, ko, ip = q_offsets.tolist(), k_offsets.tolist(), page_indptr.tolist()
@@ -208,9 +209,15 @@ def softmax_attention_ref(q, kv_cache, q_offsets, k_offsets, page_ids, page_indp
         go = [0, len(qo) - 1] if group_offsets is None else group_offsets.tolist()
         group = {b: g for g in range(len(go) - 1) for b in range(go[g], go[g + 1])}
 
-    def fetch(ids, n):
-        c = kv_cache[ids.long()]
-        return [c[:, i].reshape(-1, c.shape[3], D)[:n].to(dtype) for i in (0, 1)]
+    def fetch(ids, n, seen):
+        """K and V of a sequence's first n keys, of which ``seen [n]`` are needed."""
+        L, pages = (n + page_size - 1) // page_size, kv_cache.shape[0]
+        ids = torch.nn.functional.pad(ids[:L].long(), (0, max(L - ids.numel(), 0)), value=-1)
+        there = (ids >= 0) & (ids < pages)
+        if (torch.nn.functional.pad(seen, (0, L * page_size - n)).view(L, page_size).any(dim=1) & ~there).any():
+            raise IndexError("a page of keys that a query sees does not exist")
+        c = kv_cache[torch.where(there, ids, 0)] if pages else kv_cache.new_zeros(L, *kv_cache.shape[1:])
+        return [c[:, i].reshape(L * page_size, c.shape[3], D)[:n].to(dtype) for i in (0, 1)]
 
     out = torch.zeros(q.shape[0], H, D, dtype=dtype, device=q.device)
     lse = torch.full((q.shape[0], H), -math.inf, dtype=dtype, device=q.device)
@@ -218,15 +225,15 @@ def softmax_attention_ref(q, kv_cache, q_offsets, k_offsets, page_ids, page_indp
         n, m = qo[b + 1] - qo[b], ko[b + 1] - ko[b]
         if n == 0:
             continue
-        k, v = fetch(page_ids[ip[b]:ip[b + 1]], m)
         i = torch.arange(m - n, m, device=q.device)[:, None]
         j = torch.arange(m, device=q.device)[None, :]
         sees = j <= i
         if window > 0:
             sees = sees & ((j > i - window) | (j < num_sinks))
+        k, v = fetch(page_ids[ip[b]:ip[b + 1]], m, sees.any(dim=0))
         if group is not None and b in group:
             g = group[b]
-            kp, vp = fetch(prefix_page_ids[pp[g]:pp[g + 1]], po[g + 1] - po[g])
+            kp, vp = fetch(prefix_page_ids[pp[g]:pp[g + 1]], po[g + 1] - po[g], torch.ones(po[g + 1] - po[g], dtype=torch.bool, device=q.device))
             k, v = torch.cat([kp, k]), torch.cat([vp, v])
             sees = torch.cat([torch.ones(n, kp.shape[0], dtype=torch.bool, device=q.device), sees], dim=1)
         if k.shape[0]:
@@ -315,9 +322,9 @@ def softmax_attention_paged(q: torch.Tensor, kv_cache: torch.Tensor, q_offsets: 
     query that sees no key gives 0 and ``-inf``; rows of ``q`` behind the last request are undefined in the result.  bf16 or
     fp16, head_dim 64 or 128, page_size a multiple of 16.  Stale values in slots that a block of queries does not see do no
     harm; a non-finite VALUE that one query sees can spread to neighbouring queries of the same request that do not.  A
-    missing page reads as zeros and is reported by ``_lib.check_status``; so is, where requests
-    have many queries, one whose largest score (``scale`` times the product) lies beyond 5 * 10^6 on either side of 0: its result is
-    undefined."""
+    missing page reads as zeros and is reported by ``_lib.check_status`` (on CPU tensors it is refused).  Where requests
+    have many queries, one whose largest score (``scale`` times the product) lies beyond 5 * 10^6 on either side of 0 is reported
+    in the same way; its result is undefined."""
     return _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks, return_lse)
 
 

@@ -60,3 +60,30 @@ def test_append_refuses_what_does_not_exist():
     for n in (0, -1):
         add([0, 0], [0, 1], num_tokens=torch.tensor([n], dtype=torch.int32), out=out)
         assert torch.equal(cache, before)
+
+
+def test_attention_refuses_missing_pages_that_are_seen():
+    g = torch.Generator().manual_seed(2)
+    cache, off = torch.randn(6, 2, 16, 2, 64, generator=g), torch.tensor
+    q = torch.randn(2, 4, 64, generator=g)
+    ids, ptr = off([4, 1, 3, 0, 5]), off([0, 4, 5])
+    attend = lambda ids, ptr=ptr, k=off([0, 60, 70]), **kw: SA.softmax_attention_paged(q, cache, off([0, 1, 2]), k, ids, ptr, 16, **kw)  # noqa: E731
+    want = attend(ids)
+    for bad in (-1, 6, 10 ** 9):
+        for at in range(5):
+            hurt = ids.clone()
+            hurt[at] = bad
+            with pytest.raises(IndexError):
+                attend(hurt)
+    with pytest.raises(IndexError):                                    # fewer pages than keys
+        attend(ids, ptr=off([0, 3, 5]))
+    with pytest.raises(IndexError):
+        SA.softmax_attention_shared_prefix(q, cache, off([0, 1, 2]), off([0, 0, 10]), ids[4:], off([0, 0, 1]), off([0, 32]), off([4, -1]),
+                                           off([0, 2]), 16)
+    # what lies before the window and behind the sinks may be gone, and there may be no page for it
+    window = attend(ids, window=12, num_sinks=2)
+    for bad in (-1, 6, 10 ** 9):
+        hurt = ids.clone()
+        hurt[1] = hurt[2] = bad
+        assert torch.equal(attend(hurt, window=12, num_sinks=2), window)
+    assert torch.equal(attend(torch.cat([ids, off([-3])]), ptr=off([0, 4, 6])), want)       # more pages than keys
