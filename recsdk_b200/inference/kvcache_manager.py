@@ -416,6 +416,8 @@ class GPUKVCacheManager:
         which are returned) are turned by the tokens' positions on the way (:func:`~recsdk_b200.ops.softmax_attention.append_kv_rotary`).
         Rows behind ``md.new_history_nnz_npu`` (the padding of preallocated metadata) are left alone."""
         n = q.shape[0]
+        if n < md.new_history_nnz:
+            raise ValueError("q, k and v must hold all %d new tokens, got %d" % (md.new_history_nnz, n))
         return append_kv_rotary(q, k, v, self.cache[layer], md.batch_indices[:n], md.position[:n], md.kv_indices, md.kv_indptr,
                                 self.cfg.page_size, table, interleaved, num_tokens=md.new_history_nnz_npu, out=out)
 

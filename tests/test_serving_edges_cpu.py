@@ -87,3 +87,16 @@ def test_attention_refuses_missing_pages_that_are_seen():
         hurt[1] = hurt[2] = bad
         assert torch.equal(attend(hurt, window=12, num_sinks=2), window)
     assert torch.equal(attend(torch.cat([ids, off([-3])]), ptr=off([0, 4, 6])), want)       # more pages than keys
+
+
+def test_manager_wants_all_new_tokens():
+    m = KVCacheManager.from_config(KVCacheConfig(
+        num_layers=1, num_heads=2, head_dim=64, page_size=16, offload_chunksize=64, num_primary_cache_pages=32, num_buffer_pages=8,
+        host_capacity_per_layer=1 << 20, max_batch_size=4, max_seq_len=512, dtype=torch.float32, device="cpu"))
+    md = m.gpu.allocate(torch.tensor([3, 9]), torch.tensor([20, 33], dtype=torch.int32), torch.zeros(2, dtype=torch.int32))
+    q, k, table = torch.randn(53, 4, 64), torch.randn(53, 2, 64), SA.rotary_table(512, 64)
+    for n in (0, 20, 52):
+        with pytest.raises(ValueError, match="all 53 new tokens"):
+            m.gpu.append_kvcache_rotary(0, q[:n], k[:n], k[:n], md, table)
+    assert not m.gpu.cache.any()
+    m.gpu.append_kvcache_rotary(0, q, k, k, md, table)
