@@ -606,6 +606,13 @@ RB_API long long rb_softmax_attn_workspace(int num_sms, long long Tq, int H, int
                   groups > 0).total;
 }
 
+// How many kernels it launches.
+RB_API int rb_softmax_attn_kernels(long long Tq, int H, int Hkv, int D, int B, int groups, float scale) {
+  if (Tq == 0 || B == 0 || Hkv <= 0 || H % Hkv) return 0;
+  const Plan plan = plan_of(Tq, H / Hkv, D, B, groups, scale);
+  return 2 + (groups > 0 ? 1 + (plan.tiles_a != plan.tiles_b) : 0);            // rows or tiles or both, join, merge
+}
+
 // The arguments of rb_softmax_attn_paged, 8-byte fields first (the caller packs them: by far cheaper than 33 arguments).
 // q [Tq][H][D] (token stride ld_q), cache [num_pages][2][page_size][Hkv][D], bf16 or fp16; int32 offsets and page tables on
 // the device.  B requests own the queries q_offsets[b]..q_offsets[b+1] and k_offsets[b+1] - k_offsets[b] keys, the last of which are

@@ -242,8 +242,9 @@ def softmax_attention_ref(q, kv_cache, q_offsets, k_offsets, page_ids, page_indp
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(*sizes) -> int:
-    return _lib.lib().rb_softmax_attn_workspace(*sizes)
+def _plan(sms: int, *sizes):
+    """-> (bytes of workspace, kernels launched)."""
+    return _lib.lib().rb_softmax_attn_workspace(sms, *sizes), _lib.lib().rb_softmax_attn_kernels(*sizes)
 
 
 def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks, return_lse, prefix=None):
@@ -252,8 +253,10 @@ def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size,
     index = cache.get_device()
     q = _rows("q", q, None, D, cache)
     T, H, _ = q.shape
-    if q.is_cuda and T > 1 and (q.stride(0) < H * D or q.stride(0) % D):
+    ld_q = q.stride(0)
+    if (ld_q < H * D or ld_q % D) and index >= 0:
         q = q.contiguous()                                              # a tensor map's strides are whole multiples, and do not overlap
+        ld_q = H * D
     if H == 0 or H % Hkv:
         raise ValueError("%d query heads cannot share %d key heads" % (H, Hkv))
     B = q_offsets.numel() - 1
@@ -293,16 +296,17 @@ def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size,
     lse = torch.empty((T, H), dtype=torch.float32, device=cache.device) if return_lse else None
     if T:
         lib, sms, status = _lib.launch_env(index)
-        nbytes = _workspace_bytes(sms, T, H, Hkv, D, B, groups, scale)
+        nbytes, kernels = _plan(sms, T, H, Hkv, D, B, groups, scale)
         ws = q.new_empty(nbytes // 2)                                   # (16-bit elements)
         rc = lib.rb_softmax_attn_paged(_ATTEND_CALL.pack(
-            q.data_ptr(), q.stride(0), T, cache.data_ptr(), pages, q_offsets.data_ptr(), k_offsets.data_ptr(), page_ids.data_ptr(),
+            q.data_ptr(), ld_q, T, cache.data_ptr(), pages, q_offsets.data_ptr(), k_offsets.data_ptr(), page_ids.data_ptr(),
             page_indptr.data_ptr(), 0 if g_off is None else g_off.data_ptr(), p_off.data_ptr() if groups else 0,
             p_ids.data_ptr() if groups else 0, p_ptr.data_ptr() if groups else 0, out.data_ptr(), H * D,
             0 if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes, status, _lib.raw_stream(index), H, Hkv, D, page_size,
             page_ids.shape[0], B, p_ids.shape[0] if groups else 0, groups, min(window, 1 << 30), min(num_sinks, 1 << 30),
             q.dtype is torch.bfloat16, sms, scale))
         _lib.check(rc, "rb_softmax_attn_paged")
+        _lib.launch_count += kernels
     return (out, lse) if return_lse else out
 
 

@@ -80,3 +80,34 @@ def test_queries_turned_in_place(T, H, Hkv, D, R, interleaved):
     got = SA.append_kv_rotary(q, k, v, c2, zero, pos, ids, ptr, 16, table, interleaved=interleaved, out=q)
     assert got is q and torch.equal(q, want) and torch.equal(c1, c2) and torch.equal(qkv[:, H * D:], rest)
     _lib.check_status()
+
+
+def test_the_launch_counter_counts_every_kernel():
+    """Against the nodes of a captured graph, which are the call's kernels."""
+    import ctypes
+
+    rt = ctypes.CDLL("libcudart.so.12")
+    g = torch.Generator(device=DEV).manual_seed(1)
+    cache, ids, ptr = _cache([100, 100], 16, 2, 64, g)
+    two = (_off([100, 100]), ids, ptr)
+
+    def count(call):
+        call()
+        graph = torch.cuda.CUDAGraph(keep_graph=True)
+        with torch.cuda.graph(graph):
+            before = _lib.launch_count
+            call()
+            counted = _lib.launch_count - before
+        n = ctypes.c_size_t(0)
+        assert rt.cudaGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(n)) == 0
+        assert counted == n.value
+        return counted
+
+    seen = set()
+    for new in (1, 12, 90):                                            # by rows; prefix by tiles and own keys by rows; all by tiles
+        q = torch.randn(2 * new, 4, 64, generator=g, device=DEV).bfloat16()
+        qo, one, go = _off([new, new]), _off([100]), _off([2])
+        p_ids, p_ptr = ids[:7].contiguous(), _off([7])
+        seen.add(count(lambda: SA.softmax_attention_paged(q, cache, qo, *two, 16)))
+        seen.add(count(lambda: SA.softmax_attention_shared_prefix(q, cache, qo, *two, one, p_ids, p_ptr, 16, group_offsets=go)))
+    assert seen == {2, 3, 4}
