@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(256) kv_append_rotary_kernel(const RotaryArgs 
     bool ok = pos >= 0 && pos < p.table_rows && at_token >= 0 && bi >= 0 && bi < p.B;
     long long page = 0;
     if (ok) {
-      const int at = p.page_indptr[bi] + at_token / p.page_size;
+      const long long at = static_cast<long long>(p.page_indptr[bi]) + at_token / p.page_size;
       ok = at >= 0 && at < p.page_indptr[bi + 1] && at < p.num_page_ids;
       if (ok) {
         page = p.page_ids[at];

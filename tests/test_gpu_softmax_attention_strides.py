@@ -111,3 +111,28 @@ def test_the_launch_counter_counts_every_kernel():
         seen.add(count(lambda: SA.softmax_attention_paged(q, cache, qo, *two, 16)))
         seen.add(count(lambda: SA.softmax_attention_shared_prefix(q, cache, qo, *two, one, p_ids, p_ptr, 16, group_offsets=go)))
     assert seen == {2, 3, 4}
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_page_lists_that_begin_nowhere(new):
+    """Page tables whose ends are out of range: the pages are missing, reported and read as zeros, as the tokens are left out."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    cache, ids, ptr = _cache([300, 300], 16, 2, 64, g)
+    q = torch.randn(2 * new, 4, 64, generator=g, device=DEV).bfloat16()
+    k = torch.randn(2 * new, 2, 64, generator=g, device=DEV).bfloat16()
+    want = SA.softmax_attention_paged(q, cache, _off([new, new]), _off([300, 300]), ids, ptr, 16)
+    b = torch.arange(2, device=DEV).repeat_interleave(new)
+    pos, table = torch.arange(300 - new, 300, device=DEV).repeat(2), SA.rotary_table(300, 64, device=DEV)
+    for begin in ((1 << 31) - 1, ids.numel(), ids.numel() + 1):
+        hurt = torch.stack([ptr[0], ptr[1], torch.tensor(begin, dtype=torch.int32, device=DEV)])       # request 1 ends nowhere: all there
+        assert torch.equal(SA.softmax_attention_paged(q, cache, _off([new, new]), _off([300, 300]), ids, hurt, 16), want)
+        hurt = torch.stack([torch.tensor(begin, dtype=torch.int32, device=DEV), ptr[1], ptr[2]])       # request 0 begins nowhere
+        got = SA.softmax_attention_paged(q, cache, _off([new, new]), _off([300, 300]), ids, hurt, 16)
+        with pytest.raises(_lib.KernelStatusError, match="bounds"):
+            _lib.check_status()
+        assert (got[:new] == 0).all() and torch.equal(got[new:], want[new:])
+        c = cache.clone()
+        SA.append_kv_rotary(q, k, k, c, b, pos, ids, hurt, 16, table)
+        with pytest.raises(_lib.KernelStatusError, match="bounds"):
+            _lib.check_status()
+        assert torch.equal(c[ids[:19].long()], cache[ids[:19].long()]) and not torch.equal(c, cache)
