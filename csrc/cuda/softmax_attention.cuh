@@ -52,7 +52,8 @@ __device__ __forceinline__ Seq seq_of(const Batch& p, int i) {
   // rows outside q are never touched, whatever the offsets say
   r.q_begin = min(max(s.q_offsets[q0], 0), p.Tq);
   r.len_q = min(max(s.q_offsets[q1], r.q_begin), p.Tq) - r.q_begin;
-  r.len_k = max(s.k_offsets[j + 1] - s.k_offsets[j], 0);
+  // (the offsets may have passed 32 bits: their difference is the same)
+  r.len_k = max(static_cast<int>(static_cast<unsigned>(s.k_offsets[j + 1]) - static_cast<unsigned>(s.k_offsets[j])), 0);
   r.page_begin = min(max(s.page_indptr[j], 0), s.num_page_ids);               // (so that no page's number passes 32 bits)
   r.page_end = min(s.page_indptr[j + 1], s.num_page_ids);
   r.page_ids = s.page_ids;

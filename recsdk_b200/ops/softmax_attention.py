@@ -23,6 +23,7 @@ import torch
 from . import _lib
 
 _HEAD_DIMS = (64, 128)
+_INT32, _INT64 = torch.int32, torch.int64
 # the launchers' argument records (KvAppendCall, SoftmaxAttnCall): 8-byte fields, ints, floats
 _APPEND_CALL = struct.Struct("@19q12i")
 _ATTEND_CALL = struct.Struct("@20q12if")
@@ -61,14 +62,18 @@ def _rows(name: str, x: torch.Tensor, heads: Optional[int], dim: int, like: torc
     return x
 
 
-def _ints(name: str, x: torch.Tensor, index: int, n: Optional[int] = None) -> torch.Tensor:
-    """A vector of int32 on device ``index`` (-1: CPU); int64 is converted."""
+def _ints(name: str, x: torch.Tensor, index: int, n: Optional[int] = None, differences: bool = False) -> torch.Tensor:
+    """A vector of int32 on device ``index`` (-1: CPU); int64 is converted: to numbers that do not exist either where it has more
+    than 32 bits, or, ``differences``, so that they stay."""
     shape = x.shape
     if len(shape) != 1 or (n is not None and shape[0] != n):
         raise ValueError("%s must be a vector%s, got %s" % (name, "" if n is None else " of %d" % n, tuple(shape)))
-    if x.get_device() != index or x.dtype not in (torch.int32, torch.int64):
-        raise ValueError("%s must be int32 or int64 on the cache's device, got %s on %s" % (name, x.dtype, x.device))
-    return x if x.dtype is torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+    dtype = x.dtype
+    if x.get_device() != index or (dtype is not _INT32 and dtype is not _INT64):
+        raise ValueError("%s must be int32 or int64 on the cache's device, got %s on %s" % (name, dtype, x.device))
+    if dtype is _INT32:
+        return x if x.is_contiguous() else x.contiguous()
+    return x if index < 0 else (x if differences else x.clamp(-1, (1 << 31) - 1)).to(_INT32).contiguous()
 
 
 def _cache(kv_cache: torch.Tensor, page_size: int, dims=None) -> torch.Tensor:
@@ -262,7 +267,7 @@ def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size,
     B = q_offsets.numel() - 1
     if B < 0:
         raise ValueError("q_offsets must be [requests + 1]")
-    q_offsets, k_offsets = _ints("q_offsets", q_offsets, index), _ints("k_offsets", k_offsets, index, B + 1)
+    q_offsets, k_offsets = _ints("q_offsets", q_offsets, index), _ints("k_offsets", k_offsets, index, B + 1, differences=True)
     page_ids, page_indptr = _ints("page_ids", page_ids, index), _ints("page_indptr", page_indptr, index, B + 1)
     if window < 0 or num_sinks < 0:
         raise ValueError("window and num_sinks must not be negative")
@@ -275,7 +280,7 @@ def _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size,
         groups = p_off.numel() - 1
         if groups < 0 or (g_off is None and groups != 1):
             raise ValueError("prefix_offsets must be [groups + 1], and [2] without group_offsets")
-        p_off, p_ids = _ints("prefix_offsets", p_off, index), _ints("prefix_page_ids", p_ids, index)
+        p_off, p_ids = _ints("prefix_offsets", p_off, index, differences=True), _ints("prefix_page_ids", p_ids, index)
         p_ptr = _ints("prefix_page_indptr", p_ptr, index, groups + 1)
         if g_off is not None:
             g_off = _ints("group_offsets", g_off, index, groups + 1)

@@ -1,4 +1,5 @@
-"""Queries, keys and values as slices of other tensors: the results are those of contiguous ones, bit for bit."""
+"""Queries, keys and values as slices of other tensors, and numbers past 32 bits: the results are those of contiguous tensors and of
+the same lengths, bit for bit."""
 import pytest
 import torch
 
@@ -136,3 +137,46 @@ def test_page_lists_that_begin_nowhere(new):
         with pytest.raises(_lib.KernelStatusError, match="bounds"):
             _lib.check_status()
         assert torch.equal(c[ids[:19].long()], cache[ids[:19].long()]) and not torch.equal(c, cache)
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_offsets_past_32_bits(new):
+    """Many requests that share pages have more keys together than 32 bits count; lengths are differences."""
+    g = torch.Generator(device=DEV).manual_seed(new)
+    keys = [300, 150, 200]
+    cache, ids, ptr = _cache(keys, 16, 2, 64, g)
+    q = torch.randn(3 * new, 4, 64, generator=g, device=DEV).bfloat16()
+    qo, ko = _off([new] * 3), _off(keys).long()
+    want = SA.softmax_attention_paged(q, cache, qo, ko, ids, ptr, 16)
+    for base in ((1 << 31) - 310, (1 << 32) - 400, 1 << 40):
+        assert torch.equal(SA.softmax_attention_paged(q, cache, qo, ko + base, ids, ptr, 16), want)
+    pre = (ids[:7].contiguous(), _off([7]), 16)
+    want = SA.softmax_attention_shared_prefix(q, cache, qo, ko, ids, ptr, _off([100]).long(), *pre)
+    assert torch.equal(SA.softmax_attention_shared_prefix(q, cache, qo, ko, ids, ptr, _off([100]).long() + (1 << 31) - 50, *pre), want)
+    _lib.check_status()
+
+
+@pytest.mark.parametrize("far", [(1 << 32) + 3, -(1 << 32) + 3, (1 << 31) + 3, 1 << 40])
+def test_indices_past_32_bits_do_not_exist(far):
+    """They are reported like any other that does not exist, not taken for what their low bits say."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    cache, ids, ptr = _cache([40, 40], 16, 2, 64, g)
+    q, k, v = (torch.randn(2, h, 64, generator=g, device=DEV).bfloat16() for h in (4, 2, 2))
+    b, pos, table = torch.tensor([0, 1], device=DEV), torch.tensor([5, 6], device=DEV), SA.rotary_table(64, 64, device=DEV)
+    kw = dict(batch_indices=b, positions=pos, page_ids=ids.long(), page_indptr=ptr.long(), slots=pos)
+    for name in kw:
+        if name == "page_indptr":
+            continue
+        hurt = dict(kw)
+        hurt[name] = kw[name].clone()
+        hurt[name][0] = far
+        c = cache.clone()
+        SA.append_kv_rotary(q, k, v, c, page_size=16, table=table, **hurt)
+        with pytest.raises(_lib.KernelStatusError, match="bounds"):
+            _lib.check_status()
+        assert torch.equal(c[ids[0].long()], cache[ids[0].long()]) and not torch.equal(c, cache)
+    hurt = ids.long()
+    hurt[1] = far
+    SA.softmax_attention_paged(q, cache, _off([1, 1]), _off([40, 40]), hurt, ptr, 16)
+    with pytest.raises(_lib.KernelStatusError, match="bounds"):
+        _lib.check_status()

@@ -100,3 +100,16 @@ def test_manager_wants_all_new_tokens():
             m.gpu.append_kvcache_rotary(0, q[:n], k[:n], k[:n], md, table)
     assert not m.gpu.cache.any()
     m.gpu.append_kvcache_rotary(0, q, k, k, md, table)
+
+
+def test_offsets_past_32_bits():
+    g = torch.Generator().manual_seed(3)
+    cache, off = torch.randn(4, 2, 16, 2, 64, generator=g), torch.tensor
+    q = torch.randn(2, 4, 64, generator=g)
+    for k in (off([0, 30, 62]), off([0, 30, 62]) + (1 << 31) - 40, off([0, 30, 62]) + (1 << 40)):
+        o = SA.softmax_attention_paged(q, cache, off([0, 1, 2]), k, off([3, 1, 2, 0]), off([0, 2, 4]), 16)
+        want = o if k[0] == 0 else want
+        assert torch.equal(o, want)
+    q, k = torch.randn(1, 4, 64), torch.randn(1, 2, 64)
+    with pytest.raises(IndexError):
+        SA.append_kv_rotary(q, k, k, cache, off([0]), off([(1 << 32) + 3]), off([3, 1]), off([0, 2]), 16, SA.rotary_table(32, 64))
