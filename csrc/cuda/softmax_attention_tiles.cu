@@ -606,9 +606,9 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;   // scale > 0 in this kernel
           // O and the sum refer to m_ref; only a row whose weights would pass 2^TOP (or its first weight) moves it
           constexpr float START = BF16 ? 0.f : WeightTop<BF16> - GROWTH<BF16>, TOP = START + GROWTH<BF16>;
-          const bool grow = m_new > __fadd_rd(m_ref, TOP) || (m_ref == -INFINITY && m_new > -INFINITY);
+          const bool grow = m_new > (BF16 ? m_ref + TOP : __fadd_rd(m_ref, TOP)) || (m_ref == -INFINITY && m_new > -INFINITY);
           if (__any_sync(0xffffffffu, grow)) {
-            const float m_next = __fsub_ru(m_new, START);
+            const float m_next = BF16 ? m_new : __fsub_ru(m_new, START);
             const float f = grow ? (m_ref == -INFINITY ? 0.f : exp2_approx(m_ref - m_next)) : 1.f;
             if (grow) m_ref = m_next;
             sum *= f;
@@ -659,6 +659,8 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       float f0 = x == 0 ? 1.f : 0.f, f1 = 1.f - f0, l = sum, m_all = m_ref;
       const bool mine = q->tiles[x] > 0;
       const uint32_t had = (q->tiles[0] > 0 ? 1u : 0u) | (q->tiles[1] > 0 ? 2u : 0u);
+      if (fabsf(m_ref) >= FAR && fabsf(m_ref) < INFINITY && my_tok < min(q->tokens - (two ? x * tpt : 0), tpt) && p.status)
+        atomicCAS(p.status, 0, RB_ERR_RANGE);
       if (!two) {
         ml[(x * MT + row) * 2] = m_ref; ml[(x * MT + row) * 2 + 1] = sum;
         arrive(&bars->swap[0]);
@@ -701,7 +703,6 @@ attn_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           lse = lse2 * LN2;
         }
         if (live && c_lo == 0 && dst_lse) *dst_lse = lse;
-        if (live && fabsf(m_ref) >= FAR && fabsf(m_ref) < INFINITY && p.status) atomicCAS(p.status, 0, RB_ERR_RANGE);
 #pragma unroll 1
         for (int c = c_lo; c < c_hi; c += 32) {
           uint32_t a[32];
