@@ -112,9 +112,11 @@ struct Weigher {
     const double w = __hiloint2double(__double2hiint(q) + (((n >> 8) + up) << 20), __double2loint(q));
     return t > -700.0 ? w : 0.0;                                   // (2^-1010; also for -inf)
   }
-  // the weight in units of 2^-up, rounded (up <= 61)
+  // the weight in units of 2^-up, rounded (up <= 61; the passes over all items know whether it is `small`, up to 51)
   __device__ __forceinline__ unsigned long long fixed(float x, int up) const {
-    if (up > 51) return __double2ull_rn((*this)(x, up));
+    return up > 51 ? __double2ull_rn((*this)(x, up)) : small_fixed(x, up);
+  }
+  __device__ __forceinline__ unsigned long long small_fixed(float x, int up) const {
     const double w = (*this)(x, up) + 4503599627370496.0;          // + 2^52
     return static_cast<unsigned long long>(__double_as_longlong(w)) & 0xfffffffffffffULL;
   }
@@ -123,7 +125,7 @@ struct Weigher {
 // In which units a row's weights are summed: 64 bits hold the sum.  Rows of up to SHORT items fit whatever their weights are; the
 // sum of a longer one may be far below its number of items, and many weights that are nothing in units made for the latter can
 // matter together.
-constexpr int SHORT = 1 << 18;
+constexpr int SHORT = 1 << 18, SHORT_SHIFT = 62 - 18;
 __device__ __forceinline__ float rough_weight(float x, float top, float temp) {
   return x == top ? 1.f : x > -INFINITY ? exp2f((x - top) * (1.44269504f / temp)) : 0.f;
 }
@@ -228,7 +230,7 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
       if (keep) x = y;
     };
 
-    int shift_fx = 62 - 18;
+    int shift_fx = SHORT_SHIFT;
     // of the CTA, the same bits for all
     auto sum_of_all = [&](double v) {
 #pragma unroll
@@ -347,24 +349,29 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
               }
               shift_fx = shift_for(sum_of_all(rough));
             }
+            auto kept = [&](uint32_t k, unsigned int m) -> unsigned int { return k > cut16 ? m : k == cut16 ? cut.ties : 0; };
             auto value = [&](uint32_t k, unsigned int m) -> unsigned long long {
-              if (k <= cut16) m = k == cut16 ? cut.ties : 0;
-              return m * (by_mass ? wt.fixed(pattern_value<T>(k), shift_fx) : 1ULL);
+              return kept(k, m) * (by_mass ? wt.fixed(pattern_value<T>(k), shift_fx) : 1ULL);
             };
-            // eight threads per group, eight patterns each
-            for (int i = tid; i < (groups * (GROUP / 8) + 31) / 32 * 32; i += NT) {
-              const int at = i / (GROUP / 8);
-              const int k = group[min(at, groups - 1)] * GROUP + i % (GROUP / 8) * 8;
-              const uint4 w = *reinterpret_cast<const uint4*>(counts + k / 2);
-              const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-              unsigned long long v = 0;
+            auto sum_groups = [&](auto units) {
+              // eight threads per group, eight patterns each
+              for (int i = tid; i < (groups * (GROUP / 8) + 31) / 32 * 32; i += NT) {
+                const int at = i / (GROUP / 8);
+                const int k = group[min(at, groups - 1)] * GROUP + i % (GROUP / 8) * 8;
+                const uint4 w = *reinterpret_cast<const uint4*>(counts + k / 2);
+                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                unsigned long long v = 0;
 #pragma unroll
-              for (int j = 0; j < 8; ++j) v += value(k + j, j & 1 ? ws[j / 2] >> 16 : ws[j / 2] & 0xffffu);
-              v += __shfl_xor_sync(0xffffffffu, v, 1);
-              v += __shfl_xor_sync(0xffffffffu, v, 2);
-              v += __shfl_xor_sync(0xffffffffu, v, 4);
-              if (i % (GROUP / 8) == 0 && at < groups) mass[at] = v;
-            }
+                for (int j = 0; j < 8; ++j) v += kept(k + j, j & 1 ? ws[j / 2] >> 16 : ws[j / 2] & 0xffffu) * units(k + j);
+                v += __shfl_xor_sync(0xffffffffu, v, 1);
+                v += __shfl_xor_sync(0xffffffffu, v, 2);
+                v += __shfl_xor_sync(0xffffffffu, v, 4);
+                if (i % (GROUP / 8) == 0 && at < groups) mass[at] = v;
+              }
+            };
+            if (!by_mass) sum_groups([](uint32_t) { return 1ULL; });
+            else if (n_row <= SHORT) sum_groups([&](uint32_t k) { return wt.small_fixed(pattern_value<T>(k), SHORT_SHIFT); });
+            else sum_groups([&](uint32_t k) { return wt.fixed(pattern_value<T>(k), shift_fx); });
             if (tid == 0) s.u2 = 0;
             __syncthreads();
             const unsigned long long v0 = 2 * tid < groups ? mass[2 * tid] : 0, v1 = 2 * tid + 1 < groups ? mass[2 * tid + 1] : 0;
@@ -743,14 +750,18 @@ __global__ void __launch_bounds__(NT, 1) sample_kernel(const SampleArgs p) {
       sync();                                                      // earlier histograms have been read
       clear();
       if (by_mass) {
-        for_each<T>(x, n, [&](auto& v, int) {
-          constexpr int N = sizeof(v) / sizeof(float);
-          unsigned long long w[N];                                 // all the arithmetic before the first atomic
+        auto weigh = [&](auto units) {
+          for_each<T>(x, n, [&](auto& v, int) {
+            constexpr int N = sizeof(v) / sizeof(float);
+            unsigned long long w[N];                               // all the arithmetic before the first atomic
 #pragma unroll
-          for (int j = 0; j < N; ++j) w[j] = wt.fixed(v[j], shift_fx);
+            for (int j = 0; j < N; ++j) w[j] = units(v[j]);
 #pragma unroll
-          for (int j = 0; j < N; ++j) if (v[j] > cut_f) add64(s, bin_of(v[j]), w[j]);
-        });
+            for (int j = 0; j < N; ++j) if (v[j] > cut_f) add64(s, bin_of(v[j]), w[j]);
+          });
+        };
+        if (n_row <= SHORT) weigh([&](float e) { return wt.small_fixed(e, SHORT_SHIFT); });
+        else weigh([&](float e) { return wt.fixed(e, shift_fx); });
       } else {
         for_each<T>(x, n, [&](auto& v, int) {
           for (float e : v) if (e > cut_f) atomicAdd(&s.lo[bin_of(e)], 1u);
