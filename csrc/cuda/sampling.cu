@@ -21,8 +21,8 @@
 //
 // A row is read from memory once, into the shared memory of a cluster of CTAs (1 to 8 by its size and by how many rows there
 // are), which then exchange histograms and sums through distributed shared memory; rows that do not fit are read again from
-// L2.  Bound: for many long rows shared memory (one CTA, 131071 bf16 items, cycles: counting 19000, the draw's sums out of the
-// table 27000, everything else 25000), not the memory; in fp32 the histogram's atomics and the 64-bit arithmetic, ten
+// L2.  Bound: for many long rows shared memory (one CTA, 131071 bf16 items, 73000 cycles: counting 19000, the draw's sums out of
+// the table 26500, everything else 27500) and the waits of 16 warps for it, not the memory; in fp32 the histogram's atomics and the 64-bit arithmetic, ten
 // operations per item and pass; for few or short rows the chain of short steps between the passes.
 #include <cooperative_groups.h>
 
@@ -1090,7 +1090,8 @@ int launch(SampleArgs p, int num_sms, cudaStream_t st) {
   // 16-bit scores are counted by one CTA per row, however few rows there are: its fixed part (zeroing, listing and weighing the
   // patterns) is 10 us, its two passes 20 us for 131071 items; by weight it took 17 against 14 us at 1500 items a row, 21 against
   // 15 at 8192, 105 against 40 at 131071, and shared by four CTAs still 46.  Small k are left to the list (256 x 131071, k = 50: 81
-  // against 112 us), and the largest score needs no counts.
+  // against 112 us), and the largest score needs no counts.  A k per row is not known here and may be large or 0; where all are
+  // small after all, few rows pay for the one CTA (k = 50 as a number / per row: 16 rows 27 / 51 us, 64 rows 33 / 52, 148 55 / 55).
   p.counted = sizeof(T) == 2 && longest > LIST && (p.temperature || p.temperature_v > 0.f) && (p.top_k || p.top_k_v <= 0 || p.top_k_v > LIST / 2);
   // Otherwise CTAs per row: as many as run at once (one per SM: its 16 warps need 128 registers a thread to keep several items'
   // arithmetic in flight), while each keeps some thousand items.  131071 fp32 items with one / two / four CTAs: 114 / 70 /

@@ -22,7 +22,9 @@
 // at a time.
 //
 // 128 single tokens of 32 heads over 8 key heads of 128, a window of 4096 and uneven histories: 1.9 GB in 320 us, nine tenths of a
-// copy's bandwidth.  Heads of 64 halve the bytes of a tile but not its instructions, and reach six tenths.
+// copy's bandwidth.  Heads of 64 are read in pieces of 128 bytes: 148 sequences of 8000 keys with 8 key heads, where the warps of a
+// CTA stand at the same keys of neighbouring heads, reach 6.0 TB/s, 128 such sequences, where they do not, 4.1 (heads of 128: 6.3
+// and 6.0).
 #include "softmax_attention.cuh"
 
 namespace {
@@ -525,7 +527,9 @@ Space space_of(int n_cta, int D, long long rows, bool with_rows, bool with_tiles
 // Which kernel a list of sequences takes, by the average number of rows that share a key head: the rows kernel reads
 // K and V once for 16 of them, the tiles kernel once for 256 with at least 128 computed.  Heads of 128, 32 sequences of 4000
 // keys, 16 / 24 / 48 / 128 rows: by rows 96 / 177 / 234 / 626 us, by tiles 98 / 101 / 102 / 111; heads of 64, 200 sequences
-// of 1000 keys, 16 / 32 / 48 / 64 rows: by rows 118 / 116 / 153 / 230 us, by tiles 132 / 132 / 133 / 133.
+// of 1000 keys, 16 / 32 / 48 / 64 rows: by rows 118 / 116 / 153 / 230 us, by tiles 132 / 132 / 133 / 133.  Uneven batches go by the average, too: a
+// prompt of 2000 among 200 single tokens over 1000 / 4000 keys, 8 heads of 64, by rows 135 / 426 us, by tiles 164 / 410; among 64 of
+// them, 32 heads over 8 of 128, by rows 483 / 565 us, by tiles (which the average takes) 117 / 223.
 bool by_tiles(long long Tq, int G, int D, int sequences, float scale) {
   return G <= 128 && scale > 0.f && sequences > 0 && Tq * G * D > 2048LL * sequences;
 }

@@ -20,9 +20,9 @@
 // The CTAs are persistent, one per SM, and share the work as in softmax_attention.cu: equal, contiguous pieces of all
 // (block, key head) items laid end to end, in units of a key tile (of two where a block has one row tile).
 //
-// 16384 tokens causal, 32 heads over 8 of 128: 1.8 ms, 1.23 PFLOP/s, three quarters of a large matrix product's rate; 8192: 0.49
-// ms.  What is left: S of 64 keys is held up by shared memory (58 cycles a product instead of 32), and the two row tiles fall into
-// step; a block costs 4 us to finish and begin, which short histories (1000 keys, 17 tiles) feel as a third of their time.
+// 16384 tokens causal, 32 heads over 8 of 128, bf16: 1.8 ms, 1.2 PFLOP/s, three quarters of a large matrix product's rate; 8192: 0.5
+// ms (fp16: 2.0 and 0.57).  What is left: the two row tiles fall into step, and a block costs 4 us to finish and begin, which short
+// histories (1000 keys, 17 tiles) feel as a third of their time.
 #include "softmax_attention.cuh"
 
 namespace {

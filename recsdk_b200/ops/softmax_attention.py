@@ -333,7 +333,10 @@ def softmax_attention_paged(q: torch.Tensor, kv_cache: torch.Tensor, q_offsets: 
     harm; a non-finite VALUE that one query sees can spread to neighbouring queries of the same request that do not.  A
     missing page reads as zeros and is reported by ``_lib.check_status`` (on CPU tensors it is refused).  Where requests
     have many queries, one whose largest score (``scale`` times the product) lies beyond 5 * 10^6 on either side of 0 is reported
-    in the same way; its result is undefined."""
+    in the same way; its result is undefined.
+
+    Scores, weights and their sums are fp32; a weight is rounded to the inputs' type for its product with the values and the
+    result once more, half a step each."""
     return _attend(q, kv_cache, q_offsets, k_offsets, page_ids, page_indptr, page_size, scale, window, num_sinks, return_lse)
 
 
