@@ -127,7 +127,8 @@ struct Weigher {
 // matter together.
 constexpr int SHORT = 1 << 18, SHORT_SHIFT = 62 - 18;
 __device__ __forceinline__ float rough_weight(float x, float top, float temp) {
-  return x == top ? 1.f : x > -INFINITY ? exp2f((x - top) * (1.44269504f / temp)) : 0.f;
+  const float t = (x - top) * (1.44269504f / temp);
+  return x == top ? 1.f : t > -150.f ? exp2f(t) : 0.f;            // (0 where t is NaN)
 }
 __device__ __forceinline__ int shift_for(double rough_sum) {      // (an upper bound of it, as a power of two)
   return 62 - max(1, (__double2hiint(rough_sum * 1.01) >> 20) - 1022);

@@ -95,10 +95,14 @@ def test_weights_past_the_short_rows_units(dtype):
     for t in (1e-3, 0.05, 1.0, 100.0, 3e4, 1e30, 1e-38):
         for kw in (dict(top_p=0.9), dict(top_k=400000, top_p=0.5), dict(top_p=1e-6), dict(top_p=1 - 2.0 ** -24)):
             _same(x, torch.rand(2, generator=g, device=DEV), temperature=t, **kw)
+    _same(x, torch.rand(2, generator=g, device=DEV), temperature=torch.tensor([math.inf, 2.0], device=DEV), top_p=0.7)
     x[:, ::2] = -math.inf
     x[0, 5] = math.inf
     x[1, 7::5] = math.nan
     _same(x, torch.rand(2, generator=g, device=DEV), top_p=0.9)
+    # one infinite score, divided by an infinite temperature: whatever else there is has no weight
+    ids, lp = S.sample_scores(x, torch.rand(2, generator=g, device=DEV), temperature=torch.tensor([math.inf, 1.0], device=DEV), top_p=0.9)
+    assert int(ids[0]) == 5 and float(lp[0]) == 0.0
 
 
 def test_a_row_of_almost_two_to_the_31():
